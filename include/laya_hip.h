@@ -373,6 +373,69 @@ int hb_scan(uintptr_t ctx, int op, int dt_x, uintptr_t x, int64_t outer, int64_t
  * (Backend.meanPool, index.ts:242-243; compose.ts:96-105). */
 int hb_meanpool(uintptr_t ctx, int dt_x, uintptr_t x, uintptr_t mask, int64_t B, int64_t L, int64_t D, uintptr_t out);
 
+/* ---------------------------------------------------------------- packed batches
+ * A packed batch lays the documents of a batch end to end, [T, ...] with T the
+ * sum of their lengths, instead of each padded to the longest.  No counterpart
+ * in the reference, which pads (laya-core/src/agent.ts:131-155). */
+
+/* The plan of a packed batch from its documents' lengths (i32 [B], on the
+ * device): offsets i32 [B + 1] (the first row of each document, and the end of
+ * the last), doc and pos i32 [T] (each row's document and position in it) and,
+ * unless 0, slots i32 [T] (its row in the padded [B, L] batch).  A length below
+ * 0 counts as 0 and, with L > 0, one above L as L; documents are cut off at T
+ * rows.  Rows behind the last document get doc -1, pos 0 and slot -1. */
+int hb_pack_plan(uintptr_t ctx, uintptr_t lengths, int64_t B, int64_t T, int64_t L, uintptr_t offsets, uintptr_t doc,
+                 uintptr_t pos, uintptr_t slots);
+/* Rows of the padded batch x [rows, row_bytes] into the packed out [T,
+ * row_bytes]: row t is x's row slots[t], or zeros where that is outside x. */
+int hb_pack_rows(uintptr_t ctx, uintptr_t x, int64_t rows, int64_t row_bytes, uintptr_t slots, int64_t T,
+                 uintptr_t out);
+/* Rows of the packed batch x [T, row_bytes] into the padded out [B, L,
+ * row_bytes]: documents longer than L are cut off, padding rows are zeros. */
+int hb_unpack_rows(uintptr_t ctx, uintptr_t x, int64_t T, int64_t row_bytes, uintptr_t offsets, int64_t B, int64_t L,
+                   uintptr_t out);
+
+/* Split-half RoPE on x [T, H, D] (element strides xs[3]) at positions given per
+ * token and axis, i32 [axes, T] on the device; y is contiguous.  Of the D / 2
+ * rotation pairs the first sections[0] turn by the first axis' position, the
+ * next sections[1] by the second's, and so on; pair i keeps the frequency it
+ * has in hb_rope, and angles follow the same f32 rule, so one axis with
+ * positions 0, 1, ... gives hb_rope's values.  D even and at most 512, one to
+ * four axes, any positions. */
+int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t y, int64_t T, int64_t H, int64_t D,
+               uintptr_t positions, int64_t axes, const int64_t* sections, double base);
+
+/* Attention inside each document of a packed batch, softmax in f32.  q [Tq, H,
+ * D], k and v [Tk, Hk, D] by element strides (3 each), o contiguous [Tq, H, D];
+ * head h reads key head h / (H / Hk).  Documents are given by q_offsets and
+ * k_offsets (i32 [B + 1], of hb_pack_plan); a document's queries are its last
+ * tokens: query i of n_q is at position i + n_k - n_q among its n_k keys.
+ * Query i sees key j if j < prefix[b] (i32 [B], or 0: none), or if (not causal,
+ * or j <= pos) and (window -1, or |pos - j| <= window / 2).  Scores are scale *
+ * q . k, then cap * tanh(score / cap) unless cap is 0, then less slopes[h] *
+ * |pos - j| (f32 [H]) unless slopes is 0.  Rows without a visible key, and rows
+ * behind the last document, are zeros.  Values of hidden keys are not used,
+ * whatever they hold. */
+int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t* qs, uintptr_t k, const int64_t* ks, uintptr_t v,
+                   const int64_t* vs, uintptr_t o, uintptr_t q_offsets, uintptr_t k_offsets, int64_t B, int64_t Tq,
+                   int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale, int causal, int64_t window,
+                   uintptr_t prefix, float cap, uintptr_t slopes);
+
+/* ---------------------------------------------------------------- adapters
+ * A projection with the low-rank adapter of each row's own request beside it:
+ * y_m = x_m . w^T (+ bias, unless 0) + scales[i] * (x_m . A_i^T) . B_i^T with i =
+ * index[m] (i32 [M]); a row whose index is outside [0, n) has no adapter.  The
+ * bank is a [n, R, K] and b [n, N, R] of x's type and scales f32 [n]; R at
+ * most 1024.  x, w, bias, y as in hb_linear (the reference has no adapters). */
+int hb_lora_linear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t w, uintptr_t bias, uintptr_t y,
+                   int64_t ldy, int64_t M, int64_t N, int64_t K, uintptr_t a, uintptr_t b, uintptr_t scales, int64_t n,
+                   int64_t R, uintptr_t index);
+/* The same on a quantized weight (hb_qlinear's qw, scales, zeros, bits, group
+ * and mode). */
+int hb_lora_qlinear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t qw, uintptr_t qscales, uintptr_t zeros,
+                    uintptr_t bias, uintptr_t y, int64_t ldy, int64_t M, int64_t N, int64_t K, int bits, int group,
+                    int mode, uintptr_t a, uintptr_t b, uintptr_t scales, int64_t n, int64_t R, uintptr_t index);
+
 #ifdef __cplusplus
 }
 #endif

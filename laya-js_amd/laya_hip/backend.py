@@ -509,6 +509,40 @@ class HipGraph:
         self._sts = []
 
 
+# ------------------------------------------------------------------ packed batches and adapters
+
+class PackedDocs:
+    """The plan of a packed batch (HipBackend.packDocs): `offsets` i32 [count +
+    1], `doc` and `pos` i32 [total] (each row's document, -1 behind the last one,
+    and its position there) and, with a padded length, `slots` i32 [total] (its
+    row in the padded [count, padded] batch, -1 behind the last document)."""
+
+    def __init__(self, be: "HipBackend", count: int, total: int, padded: int, offsets, doc, pos, slots):
+        self._be = be
+        self.count, self.total, self.padded = count, total, padded
+        self.offsets, self.doc, self.pos, self.slots = offsets, doc, pos, slots
+
+    def dispose(self) -> None:
+        for t in (self.offsets, self.doc, self.pos, self.slots):
+            self._be.dispose(t)
+
+
+class LoraBank:
+    """Low-rank adapters of one projection (HipBackend.loraBank): `count`
+    adapters of rank `rank`, a [count, rank, in], b [count, out, rank] and f32
+    scales [count]."""
+
+    def __init__(self, be: "HipBackend", a, b, scales):
+        self._be = be
+        self.a, self.b, self.scales = a, b, scales
+        self.count, self.rank, self.inputs = a.shape
+        self.outputs, self.dtype = b.shape[1], a.dtype
+
+    def dispose(self) -> None:
+        for t in (self.a, self.b, self.scales):
+            self._be.dispose(t)
+
+
 # ------------------------------------------------------------------ backend
 
 class HipBackend:
@@ -544,7 +578,9 @@ class HipBackend:
     # kernel-launching entry points (timed per op key while profiling)
     _LAUNCHES = frozenset(("hb_linear", "hb_linear_qkv", "hb_qlinear", "hb_qgather", "hb_layernorm", "hb_layernorm_panel",
                            "hb_panel_unpack", "hb_panel_pack", "hb_rope", "hb_sdpa", "hb_sdpa_mask_info", "hb_geglu",
-                           "hb_unary", "hb_binary", "hb_where", "hb_gather", "hb_reduce", "hb_scan", "hb_meanpool"))
+                           "hb_unary", "hb_binary", "hb_where", "hb_gather", "hb_reduce", "hb_scan", "hb_meanpool",
+                           "hb_pack_plan", "hb_pack_rows", "hb_unpack_rows", "hb_rope_at", "hb_sdpa_packed",
+                           "hb_lora_linear", "hb_lora_qlinear"))
 
     def _call(self, op: str, name: str, *args):
         prof = self._profiling
@@ -1753,6 +1789,262 @@ class HipBackend:
         if out.size:
             self._call("meanPool", "hb_meanpool", self.ctx, DT[x.dtype][0], self._ptr(c), self._ptr(m), B, L, D,
                        out._st.ptr)
+        return out
+
+    # ---------------------------------------------------------------- packed batches
+    def _plain(self, t: HipTensor, dtype: str, tmp: list) -> HipTensor:
+        """t contiguous and of `dtype`: t itself, or a copy added to `tmp`."""
+        for c in ((lambda x: x if x.dtype == dtype else self.cast(x, dtype)), self._contiguous):
+            n = c(t)
+            if n is not t:
+                tmp.append(n)
+            t = n
+        return t
+
+    @staticmethod
+    def _plan(docs, op: str) -> None:
+        if not isinstance(docs, PackedDocs):
+            raise TypeError(f"{op}: expected a plan of packDocs, got {type(docs).__name__}")
+
+    def packDocs(self, lengths: HipTensor, total: int, padded: int = 0) -> PackedDocs:
+        """The plan of a packed batch of `total` rows from its documents' lengths
+        (integers [count], on the device; the host need not know them).  A length
+        below 0 counts as 0 and, with `padded` > 0, one above `padded` as that;
+        documents are cut off at `total` rows.  Recorded into a graph, a replay
+        plans the lengths as they are then."""
+        self._live(lengths, op="packDocs")
+        total, padded = int(total), int(padded)
+        if len(lengths.shape) != 1 or lengths.dtype in FLOAT_DT:
+            raise ValueError(f"packDocs: lengths must be integers [count], got {lengths.dtype}{list(lengths.shape)}")
+        count = lengths.shape[0]
+        if total < 0 or padded < 0 or total >= 1 << 30 or count * padded >= 1 << 31:
+            raise ValueError(f"packDocs: bad sizes (total {total}, padded {padded}, {count} documents)")
+        tmp: list = []
+        n = self._plain(lengths, "i32", tmp)
+        # one block: offsets, then the rows' arrays, each on a 256-byte boundary
+        at, step = (count + 64) // 64 * 64, (total + 63) // 64 * 64
+        st = self._malloc(4 * (at + step * (3 if padded else 2)))
+        parts = [HipTensor((count + 1,), "i32", st)]
+        for i in range(3 if padded else 2):
+            parts.append(HipTensor((total,), "i32", st.retain(), at + i * step))
+        for t in parts:
+            self._track(t)
+        p = st.ptr + 4 * at
+        self._call("packDocs", "hb_pack_plan", self.ctx, self._ptr(n), count, total, padded, st.ptr, p, p + 4 * step,
+                   p + 8 * step if padded else 0)
+        for t in tmp:
+            self.dispose(t)
+        return PackedDocs(self, count, total, padded, *parts, *([] if padded else [None]))
+
+    def packRows(self, x: HipTensor, docs: PackedDocs) -> HipTensor:
+        """Rows of the padded batch x [count, padded, ...] in the packed layout
+        [total, ...]; rows behind the last document are zeros."""
+        self._plan(docs, "packRows")
+        self._live(x, docs.slots, op="packRows")
+        if docs.slots is None or len(x.shape) < 2 or x.shape[:2] != (docs.count, docs.padded):
+            raise ValueError(f"packRows: x [{','.join(map(str, x.shape))}] of a plan of {docs.count} documents padded to "
+                             f"{docs.padded}")
+        c = self._contiguous(x)
+        out = self._new((docs.total,) + x.shape[2:], x.dtype)
+        if out.size:
+            self._call("packRows", "hb_pack_rows", self.ctx, self._ptr(c), docs.count * docs.padded,
+                       _numel(x.shape[2:]) * DT[x.dtype][1], self._ptr(docs.slots), docs.total, out._st.ptr)
+        if c is not x:
+            self.dispose(c)
+        return out
+
+    def unpackRows(self, x: HipTensor, docs: PackedDocs) -> HipTensor:
+        """Rows of the packed batch x [total, ...] in the padded layout [count,
+        padded, ...]; padding rows are zeros."""
+        self._plan(docs, "unpackRows")
+        self._live(x, docs.offsets, op="unpackRows")
+        if not docs.padded or not x.shape or x.shape[0] != docs.total:
+            raise ValueError(f"unpackRows: x [{','.join(map(str, x.shape))}] of a plan of {docs.total} rows padded to "
+                             f"{docs.padded}")
+        c = self._contiguous(x)
+        out = self._new((docs.count, docs.padded) + x.shape[1:], x.dtype)
+        if out.size:
+            self._call("unpackRows", "hb_unpack_rows", self.ctx, self._ptr(c), docs.total,
+                       _numel(x.shape[1:]) * DT[x.dtype][1], self._ptr(docs.offsets), docs.count, docs.padded,
+                       out._st.ptr)
+        if c is not x:
+            self.dispose(c)
+        return out
+
+    def ropeAt(self, x: HipTensor, positions: HipTensor, base: float, sections: Optional[Sequence[int]] = None) -> HipTensor:
+        """Split-half RoPE on x [T, H, Dh] at integer positions [T], or [axes, T]
+        with `sections`, the number of rotation pairs of each axis (Dh / 2 in
+        all).  Pair i turns at the frequency and with the angles of `rope`."""
+        self._live(x, positions, op="ropeAt")
+        if len(x.shape) != 3 or x.shape[2] % 2:
+            raise ValueError(f"ropeAt: x must be [T, H, Dh] with an even Dh, got [{','.join(map(str, x.shape))}]")
+        T, H, D = x.shape
+        axes = positions.shape[0] if len(positions.shape) == 2 else 1
+        if positions.dtype in FLOAT_DT or positions.shape[-1:] != (T,) or len(positions.shape) > 2:
+            raise ValueError(f"ropeAt: positions {positions.dtype}{list(positions.shape)} of {T} rows")
+        sections = [D // 2] if sections is None and axes == 1 else [int(n) for n in sections or ()]
+        if len(sections) != axes or sum(sections) != D // 2 or any(n < 0 for n in sections):
+            raise ValueError(f"ropeAt: sections {sections} of {axes} axes and {D // 2} pairs")
+        tmp: list = []
+        if x.dtype not in FLOAT_DT:
+            x = self.cast(x, "f32")
+            tmp.append(x)
+        pos = self._plain(positions, "i32", tmp)
+        self._ready(x)
+        out = self._new((T, H, D), x.dtype)
+        if out.size:
+            self._call("ropeAt", "hb_rope_at", self.ctx, DT[x.dtype][0], self._ptr(x), F.i64s(x._strides), out._st.ptr,
+                       T, H, D, self._ptr(pos), axes, F.i64s(sections), float(base))
+        for t in tmp:
+            self.dispose(t)
+        return out
+
+    def sdpaPacked(self, q: HipTensor, k: HipTensor, v: HipTensor, docs: PackedDocs, scale: float,
+                   keys: Optional[PackedDocs] = None, causal: bool = False, window: Optional[int] = None,
+                   prefix: Optional[HipTensor] = None, cap: Optional[float] = None,
+                   slopes: Optional[HipTensor] = None) -> HipTensor:
+        """Attention inside each document of a packed batch: q [T, H, Dh], k and v
+        [Tk, Hk, Dh] with H a multiple of Hk (query head h reads key head h // (H
+        // Hk)) -> [T, H, Dh], softmax in f32.
+
+        docs, keys: the plans of the queries' and of the keys' rows (`keys`: docs
+        unless given).  A document's queries are its last tokens: query i of n_q
+        is at position i + n_k - n_q among its n_k keys.
+        causal: keys up to the query's position; window: keys within window // 2
+        of it; prefix: integers [count], the first keys of each document that all
+        its queries see whatever causal and window hide.
+        cap: scores s become cap * tanh(s / cap); slopes: [H], scores lose
+        slopes[h] * |position - key|.
+        Rows that see no key, and rows behind the last document, are zeros."""
+        keys = docs if keys is None else keys
+        self._plan(docs, "sdpaPacked")
+        self._plan(keys, "sdpaPacked")
+        self._live(q, k, v, prefix, slopes, docs.offsets, keys.offsets, op="sdpaPacked")
+        if len(q.shape) != 3 or len(k.shape) != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+            raise ValueError(f"sdpaPacked: q {list(q.shape)} k {list(k.shape)} v {list(v.shape)}")
+        (T, H, D), (Tk, Hk, _) = q.shape, k.shape
+        if docs.total != T or keys.total != Tk or docs.count != keys.count:
+            raise ValueError(f"sdpaPacked: plans of {docs.total} and {keys.total} rows ({docs.count} and {keys.count} "
+                             f"documents) for {T} queries and {Tk} keys")
+        if Hk == 0 or H % Hk or not 0 < D <= 512:
+            raise ValueError(f"sdpaPacked: {H} heads over {Hk} key heads of dimension {D}")
+        if window is not None and window < 0:
+            raise ValueError(f"sdpaPacked: window {window}")
+        if cap is not None and not 0.0 < cap < math.inf or not math.isfinite(scale):
+            raise ValueError(f"sdpaPacked: scale {scale}, cap {cap}")
+        tmp: list = []
+        if prefix is not None:
+            if prefix.shape != (docs.count,) or prefix.dtype in FLOAT_DT:
+                raise ValueError(f"sdpaPacked: prefix {prefix.dtype}{list(prefix.shape)} of {docs.count} documents")
+        if slopes is not None:
+            if slopes.shape != (H,):
+                raise ValueError(f"sdpaPacked: slopes {list(slopes.shape)} of {H} heads")
+            slopes = self._plain(slopes, "f32", tmp)
+        if prefix is not None:
+            prefix = self._plain(prefix, "i32", tmp)
+        dt = q.dtype
+        if not (dt == k.dtype == v.dtype and dt in FLOAT_DT):
+            dt = _promote(_promote(q.dtype, k.dtype), v.dtype)
+            if dt not in FLOAT_DT:
+                dt = "f32"
+            cast = [t if t.dtype == dt else self.cast(t, dt) for t in (q, k, v)]
+            tmp += [c for c, t in zip(cast, (q, k, v)) if c is not t]
+            q, k, v = cast
+        for t in (q, k, v):
+            self._ready(t)
+        out = self._new((T, H, D), dt)
+        if out.size:
+            self.stats["sdpa"] += 1
+            self._call("sdpaPacked", "hb_sdpa_packed", self.ctx, DT[dt][0], self._ptr(q), F.i64s(q._strides),
+                       self._ptr(k), F.i64s(k._strides), self._ptr(v), F.i64s(v._strides), out._st.ptr,
+                       self._ptr(docs.offsets), self._ptr(keys.offsets), docs.count, T, Tk, H, Hk, D, float(scale),
+                       1 if causal else 0, -1 if window is None else int(window),
+                       0 if prefix is None else self._ptr(prefix), float(cap or 0.0),
+                       0 if slopes is None else self._ptr(slopes))
+        for t in tmp:
+            self.dispose(t)
+        return out
+
+    # ---------------------------------------------------------------- adapters
+    def loraBank(self, a: HipTensor, b: HipTensor, scales: Optional[HipTensor] = None) -> LoraBank:
+        """The low-rank adapters of one projection, for loraLinear: a [count,
+        rank, in], b [count, out, rank] of the activations' type, scales [count]
+        (1 each unless given).  The bank holds the tensors; dispose() frees it."""
+        self._live(a, b, scales, op="loraBank")
+        if (len(a.shape) != 3 or len(b.shape) != 3 or a.dtype != b.dtype or a.dtype not in FLOAT_DT
+                or (a.shape[0], a.shape[1]) != (b.shape[0], b.shape[2])):
+            raise ValueError(f"loraBank: a {a.dtype}{list(a.shape)}, b {b.dtype}{list(b.shape)}")
+        if a.shape[1] > 1024:
+            raise ValueError(f"loraBank: rank {a.shape[1]} above 1024")
+        if scales is not None and scales.shape != (a.shape[0],):
+            raise ValueError(f"loraBank: scales {list(scales.shape)} of {a.shape[0]} adapters")
+        if scales is None:
+            s = self.fromHost(HostTensor("f32", (a.shape[0],), np.ones(a.shape[0], np.float32)))
+        else:
+            s = self._held(scales if scales.dtype == "f32" else self.cast(scales, "f32"))
+        return LoraBank(self, self._held(a), self._held(b), s)
+
+    def _held(self, t: HipTensor) -> HipTensor:
+        """A contiguous tensor of t's values with a reference of its own."""
+        c = self._contiguous(t)
+        return self._view(c, c.shape, _contig(c.shape), c._off) if c is t else c
+
+    def _lora_operands(self, op: str, x: HipTensor, N: int, K: int, bank: LoraBank, index: HipTensor, bias, tmp: list):
+        if not isinstance(bank, LoraBank):
+            raise TypeError(f"{op}: expected a bank of loraBank, got {type(bank).__name__}")
+        self._live(x, bank.a, bank.b, bank.scales, index, bias, op=op)
+        if not x.shape or x.shape[-1] != K or (bank.inputs, bank.outputs) != (K, N):
+            raise ValueError(f"{op}: x [{','.join(map(str, x.shape))}], w [{N}, {K}], adapters [{bank.outputs}, "
+                             f"{bank.inputs}]")
+        if x.dtype != bank.dtype:
+            raise TypeError(f"{op}: x is {x.dtype}, the adapters are {bank.dtype}")
+        if index.dtype in FLOAT_DT or index.shape not in (x.shape[:-1], (_numel(x.shape[:-1]),)):
+            raise ValueError(f"{op}: index {index.dtype}{list(index.shape)} for x [{','.join(map(str, x.shape))}]")
+        if bias is not None and bias.shape != (N,):
+            raise ValueError(f"{op}: bias [{','.join(map(str, bias.shape))}] vs out {N}")
+        idx = self._plain(index, "i32", tmp)
+        if bias is not None:
+            bias = self._plain(bias, x.dtype, tmp)
+        _, xp, M, _, ldx = self._rows(x)
+        out = self._new(x.shape[:-1] + (N,), x.dtype)
+        tail = (self._ptr(bank.a), self._ptr(bank.b), self._ptr(bank.scales), bank.count, bank.rank, self._ptr(idx))
+        return xp, M, ldx, self._ptr(bias) if bias is not None else 0, out, tail
+
+    def loraLinear(self, x: HipTensor, w: HipTensor, bank: LoraBank, index: HipTensor,
+                   bias: Optional[HipTensor] = None) -> HipTensor:
+        """linear with the low-rank adapter of each row's own request beside it: y
+        = x . w^T (+ bias) + scales[i] * (x . a[i]^T) . b[i]^T, i = index[row]
+        (integers, one per row of x).  Rows whose index is outside [0, count) have
+        none."""
+        self._live(w, op="loraLinear")
+        if len(w.shape) != 2:
+            raise ValueError(f"loraLinear: w [{','.join(map(str, w.shape))}]")
+        N, K = w.shape
+        tmp: list = []
+        xp, M, ldx, bp, out, tail = self._lora_operands("loraLinear", x, N, K, bank, index, bias, tmp)
+        w = self._plain(w, x.dtype, tmp)
+        if out.size:
+            self.stats["linear"] += 1
+            self._call("loraLinear", "hb_lora_linear", self.ctx, DT[x.dtype][0], xp, ldx, self._ptr(w), bp, out._st.ptr,
+                       N, M, N, K, *tail)
+        for t in tmp:
+            self.dispose(t)
+        return out
+
+    def quantizedLoraLinear(self, x: HipTensor, w: HipTensor, scales: HipTensor, biases: Optional[HipTensor], opts,
+                            bank: LoraBank, index: HipTensor, bias: Optional[HipTensor] = None) -> HipTensor:
+        """loraLinear on a quantized weight (as quantizedLinear takes it)."""
+        self._live(w, scales, biases, op="quantizedLoraLinear")
+        N, K = w.shape[0], w.shape[1] * 8 // opts.bits
+        tmp: list = []
+        xp, M, ldx, bp, out, tail = self._lora_operands("quantizedLoraLinear", x, N, K, bank, index, bias, tmp)
+        if out.size:
+            self.stats["linear"] += 1
+            self._call("quantizedLoraLinear", "hb_lora_qlinear", self.ctx, DT[x.dtype][0], xp, ldx, self._ptr(w),
+                       self._ptr(scales), self._ptr(biases) if biases is not None else 0, bp, out._st.ptr, N, M, N, K,
+                       opts.bits, opts.groupSize, 1 if opts.mode == "affine" else 0, *tail)
+        for t in tmp:
+            self.dispose(t)
         return out
 
     # ---------------------------------------------------------------- quantized weights

@@ -394,3 +394,15 @@ def linear_any(b, x, w, bias=None):
 
 def embedding_any(b, table, ids):
     return quantized_embedding(b, table, ids) if is_quantized(table) else b.embedding(table, ids)
+
+
+# ---------------------------------------------------------------- adapters
+
+def lora_linear_any(b, x, w, bank, index, bias=None):
+    """linear_any with the low-rank adapter of each row's request beside it
+    (HipBackend.loraLinear): `w` may be quantized."""
+    if not is_quantized(w):
+        return b.loraLinear(x, w, bank, index, bias)
+    if not w.native:
+        raise RuntimeError(f"loraLinear: the {b.name} backend holds this matrix dequantized per call")
+    return b.quantizedLoraLinear(x, w.w, w.scales, w.biases, w, bank, index, bias)

@@ -10,7 +10,8 @@ from typing import Callable, Optional
 
 import numpy as np
 
-from .compose import dispose_quantized, embedding_any, geglu, is_quantized, linear_any, mean_pool, upload_quantized
+from .compose import (dispose_quantized, embedding_any, geglu, is_quantized, linear_any, lora_linear_any, mean_pool,
+                      upload_quantized)
 from .host import HostQuantized, HostTensor, to_f32
 
 FLOATS = ("f32", "f16", "bf16")
@@ -243,6 +244,92 @@ class ModernBert:
             return b.scope(lambda: mean_pool(b, self.encode(inp), inp["mask"]))
         finally:
             self.disposeInputs(inp)
+
+    # ---- packed batches: the same forward on documents laid end to end, without
+    # padding.  No counterpart in the reference, which pads each batch to its
+    # longest document (laya-core/src/agent.ts:131-155).
+
+    def uploadPacked(self, documents, adapters=None, padded: int = 0) -> dict:
+        """The inputs of encodePacked: `documents`, one array of token ids each.
+        adapters: one adapter number per document (any outside the banks for
+        none).  padded: the row length that unpackRows gives back."""
+        b = self.backend
+        documents = [np.asarray(d, np.int32).reshape(-1) for d in documents]
+        lengths = np.array([d.size for d in documents], np.int32)
+        if padded and lengths.size and lengths.max() > padded:
+            raise ValueError(f"modernbert: a document of {lengths.max()} tokens in rows of {padded}")
+        if adapters is not None and len(adapters) != len(documents):
+            raise ValueError(f"modernbert: {len(adapters)} adapter numbers for {len(documents)} documents")
+        total = int(lengths.sum())
+        ids = np.concatenate(documents) if documents else np.zeros(0, np.int32)
+
+        def f():
+            docs = b.packDocs(b.fromHost(HostTensor("i32", lengths.shape, lengths)), total, padded)
+            out = [b.fromHost(HostTensor("i32", (total,), ids)), docs.offsets, docs.doc, docs.pos]
+            out += [docs.slots] if docs.slots is not None else []
+            idx = None
+            if adapters is not None:
+                idx = b.fromHost(HostTensor("i32", (total,), np.repeat(np.asarray(adapters, np.int32), lengths)))
+                out.append(idx)
+            done.update(ids=out[0], docs=docs, adapters=idx)
+            return out  # (kept beyond the scope)
+        done: dict = {}
+        b.scope(f)
+        return done
+
+    def disposePacked(self, inp: dict) -> None:
+        self.backend.dispose(inp["ids"])
+        inp["docs"].dispose()
+        if inp["adapters"] is not None:
+            self.backend.dispose(inp["adapters"])
+
+    def layerPacked(self, i: int, x, docs, banks: Optional[dict] = None, index=None):
+        """One encoder layer on packed rows x [T, H].  banks: the adapters
+        (HipBackend.loraBank) beside any of "Wqkv", "Wo", "Wi" and "WoMlp", with
+        `index` the adapter of each row."""
+        b, c, w = self.backend, self.config, self.weights["layers"][i]
+
+        def linear(name, h):
+            bank = (banks or {}).get(name)
+            if bank is None:
+                return linear_any(b, h, w[name], w.get(name + "_b"))
+            return lora_linear_any(b, h, w[name], bank, index, w.get(name + "_b"))
+
+        def f():
+            T, H = x.shape
+            nh, hd = c.numAttentionHeads, c.headDim
+            h = b.layerNorm(x, w["attn_norm"], w.get("attn_norm_b"), c.normEps) if w["attn_norm"] is not None else x
+            qkv = b.reshape(linear("Wqkv", h), [T, 3 * nh, hd])
+            # q and k lie side by side: one rotation
+            qk = b.ropeAt(b.slice(qkv, [0, 0, 0], [T, 2 * nh, hd]), docs.pos, c.ropeBase[w["kind"]])
+            q, k = b.slice(qk, [0, 0, 0], [T, nh, hd]), b.slice(qk, [0, nh, 0], [T, 2 * nh, hd])
+            v = b.slice(qkv, [0, 2 * nh, 0], [T, 3 * nh, hd])
+            window = c.localAttention if w["kind"] == "sliding_attention" else None
+            att = b.sdpaPacked(q, k, v, docs, hd ** -0.5, window=window)
+            x1 = b.add(x, linear("Wo", b.reshape(att, [T, H])))
+            m = linear("Wi", b.layerNorm(x1, w["mlp_norm"], w.get("mlp_norm_b"), c.normEps))
+            return b.add(x1, linear("WoMlp", geglu(b, m)))
+        return b.scope(f)
+
+    def encodePacked(self, inp: dict, adapters: Optional[list] = None):
+        """embeddings -> layers -> final norm on a packed batch (uploadPacked):
+        [T, H], a row per token, each document's the values encode gives it.
+        adapters: per layer, the banks beside its projections (layerPacked)."""
+        b, c = self.backend, self.config
+        if adapters is not None and (len(adapters) != c.numHiddenLayers or inp["adapters"] is None):
+            raise ValueError(f"modernbert: adapters of {len(adapters)} layers for {c.numHiddenLayers}, with a number per "
+                             "document in uploadPacked")
+
+        def f():
+            x = self.embeddings(inp["ids"])
+            for i in range(c.numHiddenLayers):
+                nxt = self.layerPacked(i, x, inp["docs"], adapters[i] if adapters is not None else None, inp["adapters"])
+                b.dispose(x)
+                x = nxt
+            y = self.finalNorm(x)
+            b.dispose(x)
+            return y
+        return b.scope(f)
 
     def dispose(self) -> None:
         b, w = self.backend, self.weights

@@ -1,0 +1,174 @@
+"""Low-rank adapters beside a shared projection, against a plain 64-bit
+implementation.
+
+Tolerances: u is half a step of the stored type.  The result's rounding u |y|; the
+inner products rounded to the 16-bit type on their way to the second product, u
+times the adapter's absolute products; sums of n f32 products n 2^-23 of their
+absolute products; and, where the projection is rounded before the adapter's part
+is added (f32, odd sizes), another u |projection|, at most u times all absolute
+products."""
+import numpy as np
+import pytest
+
+import packed_ref as ref
+from gpu_util import read32, rounded, to_host
+from laya_hip.compose import lora_linear_any
+from laya_hip.host import HostQuantized, HostTensor
+
+pytestmark = pytest.mark.gpu
+U = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+TYPES = ["f32", "f16", "bf16"]
+
+
+@pytest.fixture(scope="module")
+def b():
+    from laya_hip.backend import HipBackend
+    be = HipBackend(0)
+    yield be
+    be.destroy()
+
+
+def i32(b, a):
+    a = np.asarray(a, np.int32)
+    return b.fromHost(HostTensor("i32", a.shape, a))
+
+
+def case(rng, dtype, M, N, K, n, R, index=None, bias=False):
+    c = {"x": rounded(rng.standard_normal((M, K)), dtype), "w": rounded(rng.standard_normal((N, K)) * 0.05, dtype),
+         "a": rounded(rng.standard_normal((n, R, K)) * max(K, 1) ** -0.5, dtype),
+         "b": rounded(rng.standard_normal((n, N, R)) * 0.05, dtype),
+         "scales": rng.uniform(-2, 2, n).astype(np.float32),
+         "index": rng.integers(-1, n + 1, M) if index is None else np.asarray(index),
+         "bias": rounded(rng.standard_normal(N), dtype) if bias else None}
+    return c
+
+
+def quantized(rng, N, K, bits, mode, group):
+    """Random codes with scales (and zeros) of weights around 0.05."""
+    data = rng.integers(0, 256, N * K * bits // 8).astype(np.uint8)
+    data[data == 128] = 127
+    G = -(-K // group)
+    s = (rng.uniform(0.5, 1, (N, G)) * 0.1 / 2 ** (bits - 1)).astype(np.float16)
+    z = (-s.astype(np.float32) * 2 ** (bits - 1)).astype(np.float16)
+    return HostQuantized((N, K), bits, group, mode, data, HostTensor("f16", (N, G), s),
+                         HostTensor("f16", (N, G), z) if mode == "affine" else None)
+
+
+def dev(b, c, dtype):
+    bank = b.loraBank(b.fromHost(to_host(c["a"], dtype)), b.fromHost(to_host(c["b"], dtype)),
+                      b.fromHost(HostTensor("f32", c["scales"].shape, c["scales"])))
+    bias = None if c["bias"] is None else b.fromHost(to_host(c["bias"], dtype))
+    return b.fromHost(to_host(c["x"], dtype)), bank, i32(b, c["index"]), bias
+
+
+def check(got, c, dtype, w=None):
+    y, mass, delta = ref.lora_linear(c["x"], c["w"] if w is None else w, c["bias"], c["a"], c["b"],
+                                     c["scales"].astype(np.float64), c["index"])
+    K, R = c["x"].shape[1], c["a"].shape[1]
+    u = U[dtype]
+    tol = u * np.abs(y) + u * delta + u * np.minimum(mass, np.abs(y) + 2 * delta) + (K + R + 8) * 2.0 ** -23 * (mass + delta)
+    bad = np.abs(got - y) > tol + 1e-30
+    assert not bad.any(), f"{bad.sum()} of {bad.size}, first at {np.argwhere(bad)[0]}, worst {np.abs(got - y).max()}"
+
+
+SIZES = [(1, 64, 64, 1, 8), (48, 2304, 768, 24, 16), (1, 1, 1, 1, 1), (5, 33, 70, 3, 4), (130, 200, 192, 4, 64),
+         (300, 768, 1152, 5, 8), (64, 256, 128, 64, 32), (17, 100, 64, 2, 3), (200, 72, 256, 3, 100), (4100, 192, 128, 6, 16),
+         (33, 520, 64, 40, 72), (700, 1024, 1024, 2, 24), (129, 130, 136, 2, 8), (1000, 640, 320, 3, 128)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K,n,R", SIZES)
+def test_lora_linear(b, dtype, M, N, K, n, R):
+    rng = np.random.default_rng(M + N)
+    c = case(rng, dtype, M, N, K, n, R, bias=M % 2 == 0)
+    x, bank, index, bias = dev(b, c, dtype)
+    w = b.fromHost(to_host(c["w"], dtype))
+    check(read32(b, b.loraLinear(x, w, bank, index, bias)), c, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["sorted", "one", "none", "alternating", "each its own"])
+def test_lora_orders_of_rows(b, dtype, kind):
+    rng = np.random.default_rng(1)
+    M, n = 290, 300
+    index = {"sorted": np.sort(rng.integers(-1, 6, M)), "one": np.full(M, 3), "none": np.where(np.arange(M) % 2, -1, n),
+             "alternating": np.arange(M) % 2 * 7, "each its own": rng.permutation(n)[:M]}[kind]
+    c = case(rng, dtype, M, 128, 128, n, 8, index)
+    x, bank, idx, _ = dev(b, c, dtype)
+    got = read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, idx))
+    check(got, c, dtype)
+    if kind == "none":  # no row has one: the projection's bits
+        np.testing.assert_array_equal(got, read32(b, b.linear(x, b.fromHost(to_host(c["w"], dtype)))))
+
+
+@pytest.mark.parametrize("bits,mode,group", [(8, "symmetric", 64), (4, "affine", 64), (8, "affine", 32), (4, "symmetric", 48)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K,n,R", [(40, 192, 128, 4, 8), (500, 96, 256, 3, 16), (3, 50, 96, 2, 5)])
+def test_lora_on_quantized_weights(b, dtype, M, N, K, n, R, bits, mode, group):
+    rng = np.random.default_rng(bits + M)
+    c = case(rng, dtype, M, N, K, n, R, bias=True)
+    q = b.fromHostQuantized(quantized(rng, N, K, bits, mode, group), dtype)
+    x, bank, index, bias = dev(b, c, dtype)
+    got = read32(b, lora_linear_any(b, x, q, bank, index, bias))
+    # the weights the backend multiplies with, read through one-hot rows
+    eye = b.fromHost(to_host(np.eye(K), dtype))
+    w = read32(b, b.quantizedLinear(eye, q.w, q.scales, q.biases, q)).T
+    check(got, c, dtype, w=w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lora_of_views(b, dtype):
+    """x as a slice of wider rows and as a [B, L, K] batch, banks and weights that
+    are views: the bits of contiguous operands."""
+    rng = np.random.default_rng(7)
+    c = case(rng, dtype, 60, 96, 128, 3, 8)
+    x, bank, index, _ = dev(b, c, dtype)
+    w = b.fromHost(to_host(c["w"], dtype))
+    want = read32(b, b.loraLinear(x, w, bank, index))
+    wide = np.concatenate([c["x"], c["x"]], 1)
+    part = b.slice(b.fromHost(to_host(wide, dtype)), [0, 128], [60, 256])
+    np.testing.assert_array_equal(read32(b, b.loraLinear(part, w, bank, index)), want)
+    batch = b.reshape(x, [4, 15, 128])
+    np.testing.assert_array_equal(read32(b, b.loraLinear(batch, w, bank, index)).reshape(60, 96), want)
+    at = b.transpose(b.fromHost(to_host(c["a"].transpose(0, 2, 1), dtype)), [0, 2, 1])
+    bt = b.transpose(b.fromHost(to_host(c["b"].transpose(0, 2, 1), dtype)), [0, 2, 1])
+    turned = b.loraBank(at, bt, b.fromHost(HostTensor("f32", (3,), c["scales"])))
+    wt = b.transpose(b.fromHost(to_host(c["w"].T, dtype)), [1, 0])
+    np.testing.assert_array_equal(read32(b, b.loraLinear(x, wt, turned, index)), want)
+    odd = b.slice(b.fromHost(to_host(np.pad(c["x"], ((0, 0), (3, 0))), dtype)), [0, 3], [60, 131])
+    check(read32(b, b.loraLinear(odd, w, bank, index)), c, dtype)
+
+
+def test_lora_empty(b):
+    """No rows, no adapters, rank 0, and weights of no inputs."""
+    rng = np.random.default_rng(0)
+    for M, n, R in ((0, 2, 4), (5, 0, 4), (5, 2, 0)):
+        c = case(rng, "f16", M, 32, 64, n, R, index=np.zeros(M, int))
+        x, bank, index, _ = dev(b, c, "f16")
+        w = b.fromHost(to_host(c["w"], "f16"))
+        got = read32(b, b.loraLinear(x, w, bank, index))
+        np.testing.assert_array_equal(got, read32(b, b.linear(x, w)))
+
+
+@pytest.mark.parametrize("M", [48, 600])
+def test_lora_recorded(b, M):
+    """Two layers recorded into a graph share scratch; replays with other rows
+    and adapter numbers, eager calls in between, give the eager bits."""
+    rng = np.random.default_rng(5)
+    c1, c2 = case(rng, "f16", M, 256, 128, 4, 8), case(rng, "f16", M, 128, 256, 3, 16)
+    x, bank1, index, _ = dev(b, c1, "f16")
+    _, bank2, _, _ = dev(b, c2, "f16")
+    w1, w2 = (b.fromHost(to_host(c["w"], "f16")) for c in (c1, c2))
+
+    def f():
+        return b.scope(lambda: b.loraLinear(b.loraLinear(x, w1, bank1, index), w2, bank2, index))
+    g = b.capture(f)
+    for i in range(3):
+        b.write(index, HostTensor("i32", (M,), rng.integers(-1, 4, M).astype(np.int32)))
+        got = read32(b, g.run()).copy()
+        want = f()
+        np.testing.assert_array_equal(got, read32(b, want))
+        b.dispose(want)
+    out = g.out
+    g.destroy()
+    b.dispose(out)

@@ -1,0 +1,421 @@
+"""Packed batches on the GPU against plain 64-bit implementations: the plan of a
+batch and rows moved by it, rotary positions given per token, attention inside
+documents, and the packed encoder forward.
+
+Tolerances: u is half a step of the stored type (f16 2^-11, bf16 2^-8, f32
+2^-24).  Attention: the output's rounding, u |o|; the weights', u sum p |v| (16-bit
+types; f32 weights stay f32); and the f32 arithmetic, relative to sum p |v|: a score
+of D products is off by at most (D + 8) 2^-24 sum |q k| (8: scale, cap, slope, the
+change to base 2, its exponential), which counts twice (weight and sum), and sums
+over n keys by n 2^-23.  A capped score's tanh is off by at most 2^-21 cap.  Rotation:
+u |y| and two products and cosines in f32, 2^-22 (|x0| + |x1|)."""
+import numpy as np
+import pytest
+
+import packed_ref as ref
+from gpu_util import read32, rounded, to_host
+from laya_hip.host import HostTensor
+
+pytestmark = pytest.mark.gpu
+U = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+TYPES = ["f32", "f16", "bf16"]
+
+
+@pytest.fixture(scope="module")
+def b():
+    from laya_hip.backend import HipBackend
+    be = HipBackend(0)
+    yield be
+    be.destroy()
+
+
+def i32(b, a):
+    a = np.asarray(a, np.int32)
+    return b.fromHost(HostTensor("i32", a.shape, a))
+
+
+def ints(b, t):
+    return np.asarray(b.read(t).data).reshape(t.shape).astype(np.int64)
+
+
+# ------------------------------------------------------------------ plan and rows
+
+PLANS = [([5], 5, 8), ([1], 1, 1), ([0, 3, 0, 0, 4, 0], 7, 4), ([], 0, 3), ([], 4, 3), ([3, 2], 9, 4),
+         ([3, 9, 2], 9, 5), ([4, -7, 4], 8, 4), ([6, 6, 6], 10, 6), ([2 ** 31 - 1, 2 ** 31 - 1, 5], 2000, 0),
+         ([1000, 30, 24, 1, 993], 2048, 1000), ([7] * 1024, 7 * 1024, 7), ([3] * 1025 + [0] * 10 + [5] * 1100, 8575, 9),
+         ([0] * 3000 + [2], 2, 2)]
+
+
+@pytest.mark.parametrize("lengths,total,padded", PLANS)
+def test_plan(b, lengths, total, padded):
+    p = b.packDocs(i32(b, lengths), total, padded)
+    off, doc, pos, slots = ref.plan(lengths, total, padded)
+    np.testing.assert_array_equal(ints(b, p.offsets), off)
+    np.testing.assert_array_equal(ints(b, p.doc), doc)
+    np.testing.assert_array_equal(ints(b, p.pos), pos)
+    if padded:
+        np.testing.assert_array_equal(ints(b, p.slots), slots)
+    else:
+        assert p.slots is None
+    p.dispose()
+
+
+@pytest.mark.parametrize("dtype,tail", [("f16", (64,)), ("f16", (5,)), ("f16", (3, 8)), ("f32", (768,)), ("f32", (1,)),
+                                        ("u8", (3,)), ("u8", (16,)), ("i32", (2, 3)), ("bf16", (1030,)), ("f32", ())])
+@pytest.mark.parametrize("lengths,total,padded", [([5, 0, 7, 1], 13, 7), ([5, 7, 1], 17, 9), ([40] * 9, 360, 40)])
+def test_rows_there_and_back(b, lengths, total, padded, dtype, tail):
+    rng = np.random.default_rng(len(lengths))
+    count = len(lengths)
+    np_t = {"f16": np.float16, "f32": np.float32, "u8": np.uint8, "i32": np.int32, "bf16": np.uint16}[dtype]
+    x = rng.integers(1, 100, (count, padded) + tail).astype(np_t)
+    p = b.packDocs(i32(b, lengths), total, padded)
+    slots = ref.plan(lengths, total, padded)[3]
+    want = np.zeros((total,) + tail, np_t)
+    want[slots >= 0] = x.reshape((count * padded,) + tail)[slots[slots >= 0]]
+    packed = b.packRows(b.fromHost(HostTensor(dtype, x.shape, x)), p)
+    np.testing.assert_array_equal(b.read(packed).data.reshape(want.shape), want)
+    back = np.zeros((count * padded,) + tail, np_t)
+    back[slots[slots >= 0]] = want[slots >= 0]
+    np.testing.assert_array_equal(b.read(b.unpackRows(packed, p)).data.reshape(back.shape), back)
+
+
+def test_rows_of_views(b):
+    """Strided operands: a transposed batch packed, a column slice unpacked."""
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((6, 3, 32)).astype(np.float32)
+    p = b.packDocs(i32(b, [6, 2, 4]), 12, 6)
+    slots = ref.plan([6, 2, 4], 12, 6)[3]
+    packed = b.packRows(b.transpose(b.fromHost(HostTensor("f32", x.shape, x)), [1, 0, 2]), p)
+    want = x.transpose(1, 0, 2).reshape(18, 32)[slots]
+    np.testing.assert_array_equal(read32(b, packed), want)
+    half = read32(b, b.unpackRows(b.slice(packed, [0, 8], [12, 24]), p)).reshape(18, 16)
+    np.testing.assert_array_equal(half[slots], want[:, 8:24])
+
+
+# ------------------------------------------------------------------ rotary positions
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H,D,sections,far", [(1, 1, 64, (32,), 10), (7, 3, 64, (32,), 9000), (93, 24, 64, (8, 12, 12), 500),
+                                                (33, 2, 16, (8,), 100), (5, 4, 6, (1, 2), 50), (64, 5, 128, (16, 24, 24), 300000),
+                                                (130, 12, 64, (0, 32), 2 ** 31 - 1), (9, 2, 80, (40,), 64), (17, 1, 2, (1,), 40),
+                                                (21, 3, 512, (100, 100, 50, 6), 4096), (1000, 4, 64, (16, 16), 2000)])
+def test_rope_at(b, T, H, D, sections, far, dtype):
+    rng = np.random.default_rng(T)
+    x = rounded(rng.standard_normal((T, H, D)), dtype)
+    pos = rng.integers(-far, far, (len(sections), T))
+    got = read32(b, b.ropeAt(b.fromHost(to_host(x, dtype)), i32(b, pos), 10000.0, sections))
+    want = ref.rope_at(x, pos, 10000.0, sections)
+    a, c = np.split(np.abs(x), 2, -1)
+    tol = U[dtype] * np.abs(want) + 2.0 ** -22 * np.concatenate([a + c, a + c], -1)
+    assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [16, 64, 96])
+def test_rope_at_of_counted_positions_is_rope(b, dtype, D):
+    """Positions 0, 1, ... on one axis: Backend.rope's bits; two axes of the same
+    positions too."""
+    rng = np.random.default_rng(D)
+    T, H = 150, 3
+    x = b.fromHost(to_host(rng.standard_normal((T, H, D)), dtype))
+    want = read32(b, b.transpose(b.rope(b.transpose(x, [1, 0, 2]), 160000.0), [1, 0, 2]))
+    np.testing.assert_array_equal(read32(b, b.ropeAt(x, i32(b, np.arange(T)), 160000.0)), want)
+    two = i32(b, np.stack([np.arange(T)] * 2))
+    np.testing.assert_array_equal(read32(b, b.ropeAt(x, two, 160000.0, [D // 2 - 3, 3])), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rope_at_of_views(b, dtype):
+    """Heads sliced out of a projection's rows, transposed heads, and columns that
+    are not contiguous: the bits of contiguous operands."""
+    rng = np.random.default_rng(3)
+    T, pos = 45, None
+    x = rounded(rng.standard_normal((T, 9, 64)), dtype)
+    pos = i32(b, rng.integers(0, 777, T))
+    t = b.fromHost(to_host(x, dtype))
+    whole = read32(b, b.ropeAt(t, pos, 10000.0))
+    np.testing.assert_array_equal(read32(b, b.ropeAt(b.slice(t, [0, 2, 0], [T, 7, 64]), pos, 10000.0)), whole[:, 2:7])
+    h = b.fromHost(to_host(x.transpose(1, 0, 2), dtype))
+    np.testing.assert_array_equal(read32(b, b.ropeAt(b.transpose(h, [1, 0, 2]), pos, 10000.0)), whole)
+    c = b.fromHost(to_host(x.transpose(0, 2, 1), dtype))
+    np.testing.assert_array_equal(read32(b, b.ropeAt(b.transpose(c, [0, 2, 1]), pos, 10000.0)), whole)
+
+
+# ------------------------------------------------------------------ attention
+
+def attn_tolerance(dtype, o, w, e, D, nk, cap=None):
+    soft = 2 * (D + 8) * 2.0 ** -24 * e + (nk + 16) * 2.0 ** -23 + (2.0 ** -20 * cap if cap else 0.0)
+    return U[dtype] * np.abs(o) + ((0.0 if dtype == "f32" else U[dtype]) + soft) * w + 1e-30
+
+
+def run_attn(b, dtype, nq, nk, heads, kv, D, seed, total=None, ktotal=None, scale=None, mangle=None, **opts):
+    """Random documents of nq queries and nk keys (None: the same) against the
+    plain form."""
+    rng = np.random.default_rng(seed)
+    T = sum(nq) if total is None else total
+    own_keys = nk is not None
+    Tk = T if not own_keys else (sum(nk) if ktotal is None else ktotal)
+    q = rounded(2 * rng.standard_normal((T, heads, D)), dtype)
+    k, v = (rounded(rng.standard_normal((Tk, kv, D)), dtype) for _ in range(2))
+    if mangle:
+        mangle(q, k, v)
+    scale = D ** -0.5 if scale is None else scale
+    docs = b.packDocs(i32(b, nq), T)
+    keys = b.packDocs(i32(b, nk), Tk) if own_keys else None
+    dev = dict(opts)
+    if opts.get("prefix") is not None:
+        dev["prefix"] = i32(b, opts["prefix"])
+    if opts.get("slopes") is not None:
+        s = np.asarray(opts["slopes"], np.float32)
+        dev["slopes"] = b.fromHost(HostTensor("f32", s.shape, s))
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, scale, keys=keys, **dev))
+    qoff = ref.offsets(nq, T)
+    koff = ref.offsets(nk, Tk) if own_keys else qoff
+    o, w, e = ref.sdpa_packed(q, k, v, qoff, koff, scale, **opts)
+    bad = np.abs(got - o) > attn_tolerance(dtype, o, w, e, D, int(np.max(np.diff(koff), initial=0)), opts.get("cap"))
+    assert np.isfinite(got).all()
+    assert not bad.any(), f"{bad.sum()} of {bad.size}, first at {np.argwhere(bad)[0]}, worst {np.abs(got - o).max()}"
+    return got
+
+
+MASKS = [dict(), dict(window=128), dict(causal=True), dict(causal=True, window=10), dict(window=0), dict(window=1),
+         dict(causal=True, prefix=[3, 70, 0, 500, 65]), dict(window=20, prefix=[1, 200, 64, 0, 7]),
+         dict(cap=5.0), dict(cap=30.0, causal=True), dict(slopes=[0.5, 0.0, 0.03, 2.0]),
+         dict(slopes=[0.1, 0.2, 0.3, 0.4], window=128, cap=2.0, causal=True, prefix=[5, 5, 5, 5, 5])]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", range(len(MASKS)))
+def test_attention_masks(b, dtype, mask):
+    run_attn(b, dtype, [65, 200, 1, 131, 64], None, 4, 4, 64, mask, **MASKS[mask])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", [0, 1, 2, 3, 6, 8, 11])
+def test_attention_of_new_tokens(b, dtype, mask):
+    """Chunks of new tokens over longer keys, one token to more than there are
+    keys, grouped heads."""
+    opts = MASKS[mask]
+    run_attn(b, dtype, [1, 40, 0, 129, 9], [300, 40, 17, 333, 5], 4, 2, 64, mask, **opts)
+    run_attn(b, dtype, [1, 1, 1, 1, 1], [300, 64, 1, 0, 1029], 4, 1, 64, mask, **opts)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,D", [(1, 1, 64), (12, 4, 64), (5, 1, 64), (3, 3, 16), (2, 1, 80), (2, 2, 128), (1, 1, 1),
+                                        (2, 2, 65), (1, 1, 512)])
+def test_attention_heads(b, dtype, heads, kv, D):
+    run_attn(b, dtype, [33, 0, 70], None, heads, kv, D, D)
+    run_attn(b, dtype, [1, 2, 30], [90, 64, 129], heads, kv, D, D, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_long(b, dtype):
+    run_attn(b, dtype, [1500, 700], None, 2, 2, 64, 5, window=128)
+    run_attn(b, dtype, [1, 3], [4000, 2500], 4, 1, 64, 6, causal=True)
+    run_attn(b, dtype, [300, 64, 1], [2100, 64, 2047], 2, 2, 64, 7, causal=True, prefix=[130, 64, 1], cap=20.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_many_documents(b, dtype):
+    rng = np.random.default_rng(8)
+    n = rng.integers(0, 9, 700).tolist()
+    run_attn(b, dtype, n, None, 2, 2, 64, 8)
+    run_attn(b, dtype, [min(1, m) for m in n], n, 2, 1, 64, 9)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_rows_behind_the_last_document(b, dtype):
+    """Rows of no document give zeros, and their keys (NaN here) reach nobody."""
+    def mangle(q, k, v):
+        k[50:], v[50:] = np.nan, np.inf
+        q[50:] = np.nan
+    got = run_attn(b, dtype, [20, 30], None, 2, 2, 64, 1, total=300, mangle=mangle)
+    assert (got[50:] == 0).all()
+    got = run_attn(b, dtype, [], None, 2, 2, 64, 1, total=130, mangle=lambda q, k, v: v.fill(np.nan))
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_attention_hidden_keys_hold_anything(b, dtype, what):
+    """Non-finite keys and values that no mask shows: the finite result."""
+    rng = np.random.default_rng(4)
+    q, k, v = (rounded(rng.standard_normal((230, 2, 64)), dtype) for _ in range(3))
+    hide = [5, 64, 100, 150, 229]
+    k[hide], v[hide] = what, what
+    # documents of 230 tokens; every row that sees a hidden key is left out of the comparison
+    docs = b.packDocs(i32(b, [230]), 230)
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, 0.125, window=8))
+    off = [0, 230]
+    o, w, e = ref.sdpa_packed(q, k, v, off, off, 0.125, window=8)
+    clean = np.array([all(abs(i - h) > 4 for h in hide) for i in range(230)])
+    bad = np.abs(got - o) > attn_tolerance(dtype, o, w, e, 64, 230)
+    assert clean.sum() > 150 and not bad[clean].any()
+    # causal: rows before the first mangled key
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, 0.125, causal=True))
+    o, w, e = ref.sdpa_packed(q, k, v, off, off, 0.125, causal=True)
+    assert not (np.abs(got - o) > attn_tolerance(dtype, o, w, e, 64, 230))[:5].any()
+    assert not np.isfinite(got[229]).all()  # the last row sees them all
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_scales(b, dtype):
+    """A negative scale, zero, and scores that underflow to one key."""
+    for scale in (-0.125, 0.0, 3.0):
+        run_attn(b, dtype, [70, 33], None, 2, 2, 64, 3, scale=scale)
+    run_attn(b, dtype, [70, 33], None, 2, 2, 64, 3, scale=-0.125, cap=4.0, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_views(b, dtype):
+    """q, k, v as slices of one projection, transposed heads, and unaligned
+    slices: the values of contiguous operands."""
+    rng = np.random.default_rng(2)
+    T, H = 150, 3
+    qkv = rounded(rng.standard_normal((T, 3 * H, 64)), dtype)
+    docs = b.packDocs(i32(b, [100, 50]), T)
+    t = b.fromHost(to_host(qkv, dtype))
+    views = [b.slice(t, [0, i * H, 0], [T, (i + 1) * H, 64]) for i in range(3)]
+    got = read32(b, b.sdpaPacked(*views, docs, 0.125))
+    parts = [b.fromHost(to_host(qkv[:, i * H:(i + 1) * H], dtype)) for i in range(3)]
+    np.testing.assert_array_equal(got, read32(b, b.sdpaPacked(*parts, docs, 0.125)))
+    heads = [b.transpose(b.fromHost(to_host(qkv[:, i * H:(i + 1) * H].transpose(1, 0, 2), dtype)), [1, 0, 2])
+             for i in range(3)]
+    np.testing.assert_array_equal(got, read32(b, b.sdpaPacked(*heads, docs, 0.125)))
+    wide = rounded(rng.standard_normal((T, H, 67)), dtype)
+    odd = b.slice(b.fromHost(to_host(wide, dtype)), [0, 0, 3], [T, H, 67])
+    o, w, e = ref.sdpa_packed(wide[..., 3:], wide[..., 3:], wide[..., 3:], [0, 100, 150], [0, 100, 150], 0.125)
+    got = read32(b, b.sdpaPacked(odd, odd, odd, docs, 0.125))
+    assert (np.abs(got - o) <= attn_tolerance(dtype, o, w, e, 64, 100)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_document_alone_gives_its_values_in_the_batch(b, dtype):
+    """Nothing of a batch reaches into another document."""
+    rng = np.random.default_rng(12)
+    n = [90, 257, 40]
+    qkv = rounded(rng.standard_normal((3, sum(n), 2, 64)), dtype)
+    both = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in qkv), b.packDocs(i32(b, n), sum(n)), 0.125,
+                                  window=100))
+    one = qkv[:, 90:347]
+    alone = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in one), b.packDocs(i32(b, [257]), 257), 0.125,
+                                   window=100))
+    o, w, e = ref.sdpa_packed(*one, [0, 257], [0, 257], 0.125, window=100)
+    tol = attn_tolerance(dtype, o, w, e, 64, 257)
+    assert (np.abs(both[90:347] - alone) <= 2 * tol).all() and (np.abs(alone - o) <= tol).all()
+
+
+# ------------------------------------------------------------------ recorded, and together
+
+def test_recorded_plan_and_attention_follow_the_lengths(b):
+    """One recording of plan, rotation and attention replayed with new lengths
+    written into its input: each replay gives the eager result, with eager work
+    in between."""
+    rng = np.random.default_rng(6)
+    T, H = 300, 2
+    lens = i32(b, [100, 120, 80])
+    x = b.fromHost(to_host(rng.standard_normal((T, 3 * H, 64)), "f16"))
+
+    def f():
+        def g():
+            p = b.packDocs(lens, T, 150)
+            qk = b.ropeAt(b.slice(x, [0, 0, 0], [T, 2 * H, 64]), p.pos, 10000.0)
+            q, k = b.slice(qk, [0, 0, 0], [T, H, 64]), b.slice(qk, [0, H, 0], [T, 2 * H, 64])
+            o = b.sdpaPacked(q, k, b.slice(x, [0, 2 * H, 0], [T, 3 * H, 64]), p, 0.125, window=64)
+            return [o, b.unpackRows(o, p)]
+        return b.scope(g)
+    g = b.capture(f)
+    for n in ([100, 120, 80], [10, 140, 150], [0, 1, 299], [150, 150, 0]):
+        b.write(lens, HostTensor("i32", (3,), np.array(n, np.int32)))
+        got = [read32(b, t).copy() for t in g.run()]
+        want = f()
+        for a, w in zip(got, want):
+            np.testing.assert_array_equal(a, read32(b, w))
+            b.dispose(w)
+    out = g.out
+    g.destroy()
+    for t in out:
+        b.dispose(t)
+
+
+def _model(b, dtype, seed=0):
+    from laya_hip.modernbert import loadModernBert, parseModernBertConfig
+    cfg = {"vocab_size": 500, "hidden_size": 256, "intermediate_size": 384, "num_hidden_layers": 4,
+           "num_attention_heads": 4, "local_attention": 32}
+    rng = np.random.default_rng(seed)
+    H, I = 256, 384
+    W = {"embeddings.tok_embeddings.weight": rng.standard_normal((500, H)), "embeddings.norm.weight": np.ones(H),
+         "final_norm.weight": np.ones(H)}
+    for i in range(4):
+        p = f"layers.{i}."
+        W[p + "mlp_norm.weight"] = np.ones(H)
+        if i:
+            W[p + "attn_norm.weight"] = np.ones(H)
+        for n, s in (("attn.Wqkv", (3 * H, H)), ("attn.Wo", (H, H)), ("mlp.Wi", (2 * I, H)), ("mlp.Wo", (H, I))):
+            W[p + n + ".weight"] = rng.standard_normal(s) * 0.05
+    return loadModernBert(b, parseModernBertConfig(cfg), lambda n: to_host(W[n], dtype) if n in W else None, dtype=dtype,
+                          prefix=""), W
+
+
+# f32: sums in another order, a few 1e-6 after four layers of values up to 5; f16:
+# both forwards round every op, 2^-11 of values up to 8 at 30 places, in
+# quadrature 2e-2, doubled
+@pytest.mark.parametrize("dtype,tol", [("f32", 1e-4), ("f16", 4e-2)])
+def test_encode_packed_is_encode(b, dtype, tol):
+    enc, _ = _model(b, dtype)
+    rng = np.random.default_rng(1)
+    n, L = [50, 1, 0, 83, 64, 29], 83
+    docs = [rng.integers(0, 500, k) for k in n]
+    ids, valid = np.zeros((len(n), L), np.int32), np.zeros((len(n), L), np.uint8)
+    for i, d in enumerate(docs):
+        ids[i, :d.size], valid[i, :d.size] = d, 1
+    ids[2], valid[2, 0] = 0, 1  # (an empty row has no defined padded forward)
+    want = read32(b, enc.forward(ids, valid, len(n), L))
+    inp = enc.uploadPacked(docs, padded=L)
+    y = enc.encodePacked(inp)
+    got = read32(b, b.unpackRows(y, inp["docs"]))
+    for i, k in enumerate(n):
+        assert np.abs(got[i, :k] - want[i, :k]).max(initial=0) <= tol
+        assert (got[i, k:] == 0).all()
+    b.dispose(y)
+    enc.disposePacked(inp)
+    enc.dispose()
+
+
+def test_encode_packed_with_adapters_is_merged_weights(b):
+    """Each document through its own adapters equals the encoder with that
+    adapter merged into its weights, in f32 (tolerance as above)."""
+    from laya_hip.modernbert import loadModernBert
+    enc, W = _model(b, "f32")
+    rng = np.random.default_rng(2)
+    H, I, R, n = 256, 384, 4, 2
+    sizes = {"Wqkv": ("attn.Wqkv", 3 * H, H), "Wo": ("attn.Wo", H, H), "Wi": ("mlp.Wi", 2 * I, H),
+             "WoMlp": ("mlp.Wo", H, I)}
+    host = [{k: (rng.standard_normal((n, R, i)) * i ** -0.5, rng.standard_normal((n, o, R)) * 0.05)
+             for k, (_, o, i) in sizes.items()} for _ in range(4)]
+    scales = np.array([1.5, -0.5], np.float32)
+    banks = [{k: b.loraBank(b.fromHost(to_host(a, "f32")), b.fromHost(to_host(c, "f32")),
+                            b.fromHost(HostTensor("f32", (n,), scales))) for k, (a, c) in layer.items()} for layer in host]
+    lens, which = [40, 64, 17, 33], [1, -1, 0, 5]
+    docs = [rng.integers(0, 500, k) for k in lens]
+    inp = enc.uploadPacked(docs, adapters=which)
+    got = read32(b, enc.encodePacked(inp, banks))
+    at = 0
+    for d, k, a in zip(docs, lens, which):
+        merged = dict(W)
+        if 0 <= a < n:
+            for i in range(4):
+                for key, (name, _, _) in sizes.items():
+                    A, C = (np.asarray(t[a], np.float32).astype(np.float64) for t in host[i][key])
+                    full = f"layers.{i}.{name}.weight"
+                    merged[full] = np.asarray(W[full], np.float32).astype(np.float64) + float(scales[a]) * C @ A
+        one = loadModernBert(b, enc.config, lambda m: to_host(merged[m], "f32") if m in merged else None, prefix="")
+        want = read32(b, one.forward(d[None], np.ones((1, k), np.uint8), 1, k))[0]
+        assert np.abs(got[at:at + k] - want).max() <= 1e-4
+        one.dispose()
+        at += k
+    for layer in banks:
+        for bank in layer.values():
+            bank.dispose()
+    enc.disposePacked(inp)
+    enc.dispose()
