@@ -13,10 +13,26 @@
 // A query without a visible key gives zeros, and so do rows behind the last
 // document.
 //
+// packed_attn_rows, packed_attn_few: f16 / bf16 with head dimension 64, flash
+// attention on v_mfma_f32_32x32x16 with 32 rows per wave.  A row is a query and
+// one of the G heads that share a key head, G rows a query, so grouped heads
+// share what they read.  A block finds its document by its slot: document b has
+// slots from off_b G / R + b on (R rows a block, rounded down), which leaves every
+// document enough of them without a table, whatever the lengths.
+// Both go through the 64-key tiles that some row of the block can see: those of
+// the prefix, then the run from the first row's lowest key to the last row's
+// highest.  A long run may be split over `splits` blocks; packed_attn_join adds up
+// their parts.
+//
+// packed_attn_f32: f32, on v_mfma_f32_32x32x2_f32.
+//
 // packed_attn_any: any head dimension, type and strides.
 #include <math.h>
 
+#include <algorithm>
+#include <atomic>
 #include <stdexcept>
+#include <type_traits>
 
 #include "attention_common.h"
 
@@ -61,11 +77,471 @@ __device__ __forceinline__ void packed_range(const Packed& p, int nk, int pos, i
   if (p.causal) *hi = min(*hi, pos);
 }
 
+// ------------------------------------------------------------------ rows and tiles
+
+// The document of slot `slot`: the last b with off_b * G / R + b <= slot (the
+// documents' first slots; document B holds the rows behind the last one).  All
+// 64 lanes probe at once, so up to 63 documents take one round of loads.
+template <int R>
+__device__ __forceinline__ int slot_doc(const Packed& p, int64_t slot, int lane, int64_t* first) {
+  auto base = [&](int b) { return (int64_t)min(max(p.qoff[b], 0), p.Tq) * p.G / R + b; };
+  int lo = 0, n = p.B + 1;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, at = lane * step;
+    const int cnt = __popcll(__ballot(at < n && base(lo + (at < n ? at : 0)) <= slot));
+    lo += (cnt - 1) * step;
+    n = min(step, n - (cnt - 1) * step);
+  }
+  *first = base(lo);
+  return lo;
+}
+
+// The tiles of KT keys that rows at positions pb0 .. pb1 can see: `pre` tiles of
+// the prefix, then those from run0 on, `n` in all.
+struct Tiles {
+  int pre, run0, n;
+  __device__ __forceinline__ int at(int i) const { return i < pre ? i : run0 + i - pre; }
+};
+template <int KT>
+__device__ __forceinline__ Tiles row_tiles(const Packed& p, const Doc& d, int pb0, int pb1) {
+  Tiles t;
+  int lo, hi, x;
+  packed_range(p, d.nk, pb0, &lo, &x);
+  packed_range(p, d.nk, pb1, &x, &hi);
+  t.pre = (d.prefix + KT - 1) / KT;
+  t.run0 = max(lo / KT, t.pre);
+  t.n = t.pre + (hi >= lo ? max(hi / KT + 1 - t.run0, 0) : 0);
+  return t;
+}
+
+// One lane's row, and the visibility of a tile for all rows of its wave
+struct Row {
+  int pos, lo, span;  // key j is visible if j < prefix or j - lo <= span, unsigned
+  int lo0, lo1, hi0, hi1;  // ranges of the wave's first and last rows' positions
+  float slope;
+};
+__device__ __forceinline__ Row packed_row(const Packed& p, const Doc& d, int r, int rw0, int rows, int hk) {
+  // (a wave without rows, rw0 >= rows, repeats the last one: its caller skips it)
+  Row w;
+  const int shift = d.nk - d.nq, last = min(rw0 + 31, rows - 1);
+  int hi, x;
+  w.pos = r / p.G + shift;
+  packed_range(p, d.nk, w.pos, &w.lo, &hi);
+  if (hi < w.lo) w.lo = 1 << 30, hi = w.lo;  // sees nothing of the run: keys are below 2^30
+  w.span = hi - w.lo;
+  packed_range(p, d.nk, min(rw0, rows - 1) / p.G + shift, &w.lo0, &w.hi0);
+  packed_range(p, d.nk, last / p.G + shift, &w.lo1, &w.hi1);
+  w.slope = p.slopes == nullptr ? 0.f : p.slopes[hk * p.G + r % p.G];
+  return w;
+}
+// 0: no row sees a key of the tile, 1: every row sees every key, 2: neither
+template <int KT>
+__device__ __forceinline__ int tile_class(const Doc& d, const Row& w, int k0) {
+  if (k0 + KT <= d.prefix) return 1;
+  if (k0 >= d.prefix && (k0 > w.hi1 || k0 + KT - 1 < w.lo0)) return 0;
+  return k0 + KT <= d.nk && k0 >= w.lo1 && k0 + KT - 1 <= w.hi0 ? 1 : 2;
+}
+__device__ __forceinline__ bool key_seen(const Doc& d, const Row& w, int j) {
+  return j < d.prefix || (uint32_t)(j - w.lo) <= (uint32_t)w.span;
+}
+
+// Parts of a split run: per split and row (token * H + head) the unscaled output,
+// its maximum score and its sum of weights.
+struct Parts {
+  float* o;    // [splits][rows][64]
+  float2* ml;  // [splits][rows]
+};
+
+// ------------------------------------------------------------------ f16 / bf16 (D = 64)
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A wave's 32 rows (lane l holds row l % 32; the halves split its columns and its
+// keys).  Scores are in base 2 once `mul` is applied: mul is 1 where a cap or a
+// slope has made them so beforehand.
+struct Wave {
+  uint4v qf[4];   // columns 16 s + 8 lg .. of the query per MFMA step s
+  float16v o[2];  // columns 32 d + 8 (r / 4) + 4 lg + r % 4
+  float m, l;     // running maximum (before mul), the lane's sum of weights
+};
+struct Score {
+  float mul, c1, c2;  // capped: c2 tanh, computed as c2 - 2 c2 / (1 + 2^(c1 score))
+  uint32_t flip;      // a negative scale turns the query round instead
+};
+__device__ __forceinline__ Score score_of(const Packed& p, bool cap, bool bias) {
+  Score s;
+  // (scale 0: any tiny factor; 0 * -inf would not be a maximum)
+  const float sl = fmaxf(fabsf(p.scale), 1e-30f) * kLog2e;
+  s.mul = cap || bias ? 1.f : sl;
+  s.c1 = cap ? 2.f * sl / p.cap : sl;
+  s.c2 = p.cap * kLog2e;
+  s.flip = p.scale < 0.f ? 0x80008000u : 0u;
+  return s;
+}
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float score(const Score& s, float slope, int pos, int key, float x) {
+  if constexpr (CAP) x = fmaf(-2.f * s.c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * s.c1)), s.c2);
+  else if constexpr (BIAS) x *= s.c1;
+  if constexpr (BIAS) x = fmaf(-slope, fabsf((float)(pos - key)), x);
+  return x;
+}
+
+__device__ __forceinline__ void wave_init(Wave& w, const Score& sc, const uint16_t* qrow, int lg) {
+#pragma unroll
+  for (int s = 0; s < 4; s++) {
+    w.qf[s] = *(const uint4v*)(qrow + 8 * lg + 16 * s);
+#pragma unroll
+    for (int e = 0; e < 4; e++) w.qf[s][e] ^= sc.flip;
+  }
+#pragma unroll
+  for (int d = 0; d < 2; d++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) w.o[d][r] = 0.f;
+  w.m = -INFINITY;
+  w.l = 0.f;
+}
+
+// One tile of 64 keys in LDS: scores, mask (`mixed`), online softmax, O += P V.
+// Weights are rounded to the 16-bit type for the second product, as MFMA takes
+// them; their sum is of the unrounded ones.
+template <bool BF16, bool CAP, bool BIAS>
+__device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16_t* Kc, const uint16_t* Vc, int k0,
+                                          const Doc& d, const Row& row, bool mixed, const Score& sc, int lg) {
+  float16v st[2];
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) st[kb][r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; s++) st[kb] = mfma32x16<BF16>(*(const uint4v*)(Kc + f.ka[s] + kb * 2048), w.qf[s], st[kb]);
+  }
+  if constexpr (CAP || BIAS) {
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        st[kb][r] = score<CAP, BIAS>(sc, row.slope, row.pos, k0 + 32 * kb + 8 * (r >> 2) + 4 * lg + (r & 3), st[kb][r]);
+  }
+  if (mixed) {
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        st[kb][r] = key_seen(d, row, k0 + 32 * kb + 8 * (r >> 2) + 4 * lg + (r & 3)) ? st[kb][r] : -INFINITY;
+  }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[kb][r]);
+  mx = max_xor32(mx);
+  const float mnew = fmaxf(w.m, mx);
+  const float mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
+  const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc);
+  w.m = mnew;
+  float psum = 0.f;
+  uint4v pf[4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    uint32_t pk[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t >> 1][8 * (t & 1) + e], sc.mul, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t >> 1][8 * (t & 1) + e + 1], sc.mul, -mc));
+      psum += p0 + p1;
+      pk[e >> 1] = pack2<BF16>(p0, p1);
+    }
+    pf[t] = uint4v{pk[0], pk[1], pk[2], pk[3]};
+  }
+  w.l = w.l * alpha + psum;
+  if (!__all(alpha == 1.0f)) {  // rescale O only when some row max of this wave moved
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) w.o[e][r] *= alpha;
+  }
+#pragma unroll
+  for (int t = 0; t < 4; t++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const uint2v v0 = lds_tr16(Vc + f.va[0][e] + t * 1024), v1 = lds_tr16(Vc + f.va[1][e] + t * 1024);
+      w.o[e] = mfma32x16<BF16>(uint4v{v0.x, v0.y, v1.x, v1.y}, pf[t], w.o[e]);
+    }
+}
+
+// A non-finite value must not reach a row whose weight for its key is 0 (hidden,
+// or underflowed), as 0 * inf in the product does.  Where a wave's output has
+// come out non-finite it is computed again, key by key, zero weights skipped:
+// slow, and never run on finite data.  tiles [i0, i1) in steps of `step`.
+template <bool BF16, bool CAP, bool BIAS>
+__device__ __forceinline__ Wave wave_again(Wave w, const uint16_t* Kb, int64_t kst, const uint16_t* Vb, int64_t vst,
+                                        Doc d, Row row, Tiles ti, int i0, int i1, int step,
+                                        Score sc, int lg) {
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) w.o[e][r] = 0.f;
+  w.m = -INFINITY;
+  w.l = 0.f;
+#pragma unroll 1
+  for (int i = i0; i < i1; i += step) {
+    const int k0 = ti.at(i) * 64, k1 = min(k0 + 64, d.nk);
+#pragma unroll 1
+    for (int j = k0; j < k1; j++) {
+      const uint16_t* kr = Kb + j * kst + 8 * lg;
+      float x = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const uint4v kv = *(const uint4v*)(kr + 16 * s);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x = fmaf(tof<BF16>(kv[e] & 0xffff), tof<BF16>(w.qf[s][e] & 0xffff), x);
+          x = fmaf(tof<BF16>(kv[e] >> 16), tof<BF16>(w.qf[s][e] >> 16), x);
+        }
+      }
+      x = score<CAP, BIAS>(sc, row.slope, row.pos, j, sum_xor32(x));
+      x = key_seen(d, row, j) ? x : -INFINITY;
+      const float mnew = fmaxf(w.m, x), mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
+      const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc), pr = __builtin_amdgcn_exp2f(fmaf(x, sc.mul, -mc));
+      w.m = mnew;
+      w.l = w.l * alpha + (lg == 0 ? pr : 0.f);  // (the halves' sums are added up later)
+      const float p16 = tof<BF16>(fromf<BF16>(pr));
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+          const uint2v vv = *(const uint2v*)(Vb + j * vst + 32 * e + 8 * r4 + 4 * lg);
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const float v = tof<BF16>(((c & 2) ? vv.y : vv.x) >> (16 * (c & 1)) & 0xffff);
+            const float o = w.o[e][4 * r4 + c] * alpha;
+            w.o[e][4 * r4 + c] = p16 == 0.f ? o : fmaf(p16, v, o);
+          }
+        }
+    }
+  }
+  return w;
+}
+__device__ __forceinline__ bool wave_finite(const Wave& w) {
+  float z = w.l * 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) z = fmaf(w.o[e][r], 0.f, z);
+  return !__any(z != 0.f);  // 0 * finite = 0, 0 * (inf or NaN) = NaN
+}
+
+__device__ __forceinline__ int64_t row_index(const Packed& p, const Doc& d, int r, int hk) {
+  return (int64_t)(d.q0 + r / p.G) * p.H + hk * p.G + r % p.G;
+}
+
+// 128 rows a block, four waves of 32, K and V tiles in a two-buffer LDS ring with
+// one barrier per tile.
+constexpr int kRowsB = 128;
+template <bool BF16, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void packed_attn_rows(Packed p, Parts part,
+                                                                                                int splits) {
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][64 * 64];
+  __shared__ __attribute__((aligned(16))) uint16_t Vs[2][64 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, lg = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Hk = p.H / p.G, hk = blockIdx.x % Hk;
+  const int64_t slot = blockIdx.x / Hk;
+  int64_t first;
+  const int b = slot_doc<kRowsB>(p, slot, lane, &first);
+  const Doc d = packed_doc(p, b);
+  const int64_t at = (slot - first) * kRowsB;
+  if (at >= (int64_t)d.nq * p.G) return;  // (the whole block)
+  const int rows = d.nq * p.G, r0 = (int)at, rw0 = r0 + 32 * wave;
+  const int r = rw0 + (lane & 31), rc = min(r, rows - 1);
+  const Score sc = score_of(p, CAP, BIAS);
+  Row row = packed_row(p, d, rc, rw0, rows, hk);
+  row.slope *= kLog2e;
+  const int shift = d.nk - d.nq;
+  const Tiles ti = row_tiles<64>(p, d, r0 / p.G + shift, min(r0 + kRowsB - 1, rows - 1) / p.G + shift);
+  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits), i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const uint16_t* Kb = (const uint16_t*)p.K + d.k0 * p.ks[0] + hk * p.ks[1];
+  const uint16_t* Vb = (const uint16_t*)p.V + d.k0 * p.vs[0] + hk * p.vs[1];
+  Wave w;
+  wave_init(w, sc, (const uint16_t*)p.Q + (d.q0 + rc / p.G) * p.qs[0] + (hk * p.G + rc % p.G) * p.qs[1], lg);
+  auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
+    const int k0 = ti.at(i) * 64;
+#pragma unroll
+    for (int q = 0; q < 2; q++) dma_piece(Vb, p.vs[0], k0, wave * 2 + q, d.nk, Vs[bf], lane);
+#pragma unroll
+    for (int q = 0; q < 2; q++) dma_piece(Kb, p.ks[0], k0, wave * 2 + q, d.nk, Ks[bf], lane);
+  };
+  if (i0 < i1) fetch(i0, 0);
+  const Frag32 f = frag32(lane);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int bf = 0;
+  for (int i = i0; i < i1; i++) {
+    // the next tile into the other buffer (free since the last barrier)
+    if (i + 1 < i1) fetch(i + 1, bf ^ 1);
+    const int k0 = ti.at(i) * 64, cl = rw0 < rows ? tile_class<64>(d, row, k0) : 0;
+    if (cl != 0) wave_tile<BF16, CAP, BIAS>(w, f, Ks[bf], Vs[bf], k0, d, row, cl == 2, sc, lg);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bf ^= 1;
+    __syncthreads();
+  }
+  if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], d, row, ti, i0, i1, 1, sc, lg);
+  const float lt = sum_xor32(w.l);
+  if (r >= rows) return;
+  const int64_t ri = row_index(p, d, r, hk);
+  if (splits > 1) {
+    const int64_t pr = (int64_t)s * p.Tq * p.H + ri;
+    if (lg == 0) part.ml[pr] = float2{w.m * sc.mul, lt};
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        *(float4v*)(part.o + pr * 64 + 32 * e + 8 * j + 4 * lg) =
+            float4v{w.o[e][4 * j], w.o[e][4 * j + 1], w.o[e][4 * j + 2], w.o[e][4 * j + 3]};
+    return;
+  }
+  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  uint16_t* op = (uint16_t*)p.O + ri * 64 + 4 * lg;
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      *(uint2v*)(op + 32 * e + 8 * j) = uint2v{pack2<BF16>(w.o[e][4 * j] * inv, w.o[e][4 * j + 1] * inv),
+                                               pack2<BF16>(w.o[e][4 * j + 2] * inv, w.o[e][4 * j + 3] * inv)};
+}
+
+// 32 rows a block, for few queries a document: the block's four waves hold the
+// same rows and take its tiles in turn, each through an LDS ring of its own with
+// no barrier, so the block has 64 KB of keys and values on their way; then the
+// waves' parts are joined.  Bound by reading K and V once.
+constexpr int kRowsF = 32, kFewLds = 4 * 2 * 2 * 64 * 64 * 2;  // four rings of two K and V tiles
+template <bool BF16, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void packed_attn_few(Packed p, Parts part,
+                                                                                               int splits) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t ring[];
+  __shared__ float part_m[4][kRowsF], part_l[4][kRowsF];
+  const int tid = threadIdx.x, lane = tid & 63, lg = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Hk = p.H / p.G, hk = blockIdx.x % Hk;
+  const int64_t slot = blockIdx.x / Hk;
+  int64_t first;
+  const int b = slot_doc<kRowsF>(p, slot, lane, &first);
+  const Doc d = packed_doc(p, b);
+  const int64_t at = (slot - first) * kRowsF;
+  if (at >= (int64_t)d.nq * p.G) return;  // (the whole block)
+  const int rows = d.nq * p.G, r0 = (int)at, r = r0 + l32, rc = min(r, rows - 1);
+  const Score sc = score_of(p, CAP, BIAS);
+  Row row = packed_row(p, d, rc, r0, rows, hk);
+  row.slope *= kLog2e;
+  const int shift = d.nk - d.nq;
+  const Tiles ti = row_tiles<64>(p, d, r0 / p.G + shift, min(r0 + kRowsF - 1, rows - 1) / p.G + shift);
+  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits) + wave, i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const uint16_t* Kb = (const uint16_t*)p.K + d.k0 * p.ks[0] + hk * p.ks[1];
+  const uint16_t* Vb = (const uint16_t*)p.V + d.k0 * p.vs[0] + hk * p.vs[1];
+  uint16_t* mine = ring + wave * (4 * 64 * 64);  // K, V, K, V
+  auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
+    const int k0 = ti.at(i) * 64;
+    // this wave's reads of the tile that was there are done
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < 8; q++) dma_piece(Kb, p.ks[0], k0, q, d.nk, mine + bf * 8192, lane);
+#pragma unroll
+    for (int q = 0; q < 8; q++) dma_piece(Vb, p.vs[0], k0, q, d.nk, mine + bf * 8192 + 4096, lane);
+  };
+  Wave w;
+  wave_init(w, sc, (const uint16_t*)p.Q + (d.q0 + rc / p.G) * p.qs[0] + (hk * p.G + rc % p.G) * p.qs[1], lg);
+  const Frag32 f = frag32(lane);
+  if (i0 < i1) fetch(i0, 0);
+  int bf = 0;
+  for (int i = i0; i < i1; i += 4) {
+    if (i + 4 < i1) {
+      fetch(i + 4, bf ^ 1);
+      asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // all but the 16 loads just requested
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const int k0 = ti.at(i) * 64, cl = tile_class<64>(d, row, k0);
+    if (cl != 0)
+      wave_tile<BF16, CAP, BIAS>(w, f, mine + bf * 8192, mine + bf * 8192 + 4096, k0, d, row, cl == 2, sc, lg);
+    bf ^= 1;
+  }
+  if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], d, row, ti, i0, i1, 4, sc, lg);
+  // join the waves: weights 2^(m_w - max); wave w finishes registers [8 w, 8 w + 8)
+  // of the 32
+  const float lw = sum_xor32(w.l);
+  if (lg == 0) {
+    part_m[wave][l32] = w.m * sc.mul;
+    part_l[wave][l32] = lw;
+  }
+  float* buf = (float*)ring;
+  __syncthreads();  // every wave is done with its ring
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) buf[wave * 2048 + (e * 16 + i) * 64 + lane] = w.o[e][i];
+  __syncthreads();
+  float mt = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; i++) mt = fmaxf(mt, part_m[i][l32]);
+  const float mc = mt == -INFINITY ? 0.f : mt;
+  float wt[4], lt = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    wt[i] = __builtin_amdgcn_exp2f(part_m[i][l32] - mc);
+    lt += part_l[i][l32] * wt[i];
+  }
+  if (r >= rows) return;
+  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  const int64_t ri = row_index(p, d, r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
+  if (splits > 1 && wave == 0 && lg == 0) part.ml[pr] = float2{mt, lt};
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int x = wave * 8 + h * 4, col = 32 * (x >> 4) + 8 * ((x & 15) >> 2) + 4 * lg;
+    float4v ov;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) a += wt[i] == 0.f ? 0.f : buf[i * 2048 + (x + e) * 64 + lane] * wt[i];
+      ov[e] = a;
+    }
+    if (splits > 1) {
+      *(float4v*)(part.o + pr * 64 + col) = ov;
+    } else {
+      *(uint2v*)((uint16_t*)p.O + ri * 64 + col) =
+          uint2v{pack2<BF16>(ov[0] * inv, ov[1] * inv), pack2<BF16>(ov[2] * inv, ov[3] * inv)};
+    }
+  }
+}
+
+// Joins the parts of split runs: one wave a row, a lane per column.  E2: maxima in
+// base 2 (the 16-bit kernels), else natural.
+template <bool E2>
+__global__ __launch_bounds__(256) void packed_attn_join(int dt, Parts part, int splits, int64_t rows,
+                                                        void* __restrict__ O) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < splits; s++) m = fmaxf(m, part.ml[s * rows + r].x);
+  const float mc = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o = 0.f;
+  for (int s = 0; s < splits; s++) {
+    const float2 ml = part.ml[s * rows + r];
+    const float w = E2 ? __builtin_amdgcn_exp2f(ml.x - mc) : expf(ml.x - mc);
+    l = fmaf(ml.y, w, l);
+    if (w != 0.f) o = fmaf(part.o[(s * rows + r) * 64 + lane], w, o);
+  }
+  store_f(O, r * 64 + lane, dt, l == 0.f ? 0.f : o / l);
+}
+
+// ------------------------------------------------------------------ any type
+
 // One wave per query and head: 64 keys at a time, a score per lane, then the
 // lanes share out the columns of the output.
 constexpr int kAnyCols = 8;  // columns per lane: D <= 512
 __global__ __launch_bounds__(64) void packed_attn_any(Packed p, int dt) {
-  extern __shared__ float sh[];  // [D] query, [64] weights, [64] visibility
+  extern __shared__ float sh[];  // [D] query, [64] weights
   float* w = sh + p.D;
   const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, D = p.D;
   int b = 0, e = p.B + 1;  // the last document that begins at or before t
@@ -104,19 +580,90 @@ __global__ __launch_bounds__(64) void packed_attn_any(Packed p, int dt) {
     l = l * alpha + wave_sum(pr);
     __syncthreads();  // the last keys' weights are used up
     w[lane] = pr;
-    w[64 + lane] = seen ? 1.f : 0.f;
     __syncthreads();
     for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++) {
       float a = o[i] * alpha;
       const int64_t col = vh + (i * 64 + lane) * p.vs[2];
       for (int k = 0; k < 64 && j0 + k < d.nk; k++)
-        if (w[64 + k] != 0.f) a = fmaf(w[k], load_f(p.V, (int64_t)(d.k0 + j0 + k) * p.vs[0] + col, dt), a);
+        if (w[k] != 0.f) a = fmaf(w[k], load_f(p.V, (int64_t)(d.k0 + j0 + k) * p.vs[0] + col, dt), a);
       o[i] = a;
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++)
     store_f(p.O, ((int64_t)t * p.H + h) * D + i * 64 + lane, dt, o[i] * inv);
+}
+
+// ------------------------------------------------------------------ dispatch
+
+// The MFMA kernels' conditions: D = 64, unit column strides, 16-byte aligned rows
+// (`per` elements), and K / V row strides that 32-bit offsets within a tile reach.
+static bool packed_takes_mfma(const Packed& p, int per) {
+  auto rows16 = [&](const void* t, const int64_t* s) {
+    return (uintptr_t)t % 16 == 0 && s[2] == 1 && s[0] % per == 0 && s[1] % per == 0;
+  };
+  auto near = [](int64_t s) { return s >= 0 && s < (1 << 23); };
+  return p.D == 64 && (int64_t)p.Tq * p.G < (1ll << 30) && rows16(p.Q, p.qs) && rows16(p.K, p.ks) && rows16(p.V, p.vs) && near(p.ks[0]) && near(p.vs[0]) &&
+         (uintptr_t)p.O % 16 == 0;
+}
+
+static void packed_any(uintptr_t ctx, int dt, const Packed& p) {
+  packed_attn_any<<<dim3((unsigned)p.Tq, (unsigned)p.H), 64, (size_t)(p.D + 64) * 4, stream_of(ctx)>>>(p, dt);
+}
+
+template <class K>
+static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, int lds, int rows, const Packed& p, int splits,
+                          const Parts& part) {
+  if (lds > 64 * 1024)
+    once_per_device(attr, [&] {
+      HB_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    });
+  const int64_t grid = ((int64_t)p.Tq * p.G / rows + p.B + 1) * (p.H / p.G);
+  HB_REQUIRE(grid < (1ll << 31), "hb_sdpa_packed: too many rows and heads");
+  kern<<<dim3((unsigned)grid, (unsigned)splits), 256, (size_t)lds, stream_of(ctx)>>>(p, part, splits);
+}
+
+static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
+  const int64_t rows = (int64_t)p.Tq * p.G;
+  const bool few = rows <= 64 * (int64_t)p.B;
+  const int per = few ? kRowsF : kRowsB, Hk = p.H / p.G, cus = cu_count(ctx);
+  // Keys of an average document's rows, and the blocks they make
+  int64_t keys = p.B ? p.Tk / p.B : 0;
+  if (p.half >= 0) keys = std::min<int64_t>(keys, 2 * (int64_t)p.half + per / p.G + 64);
+  const int64_t blocks = (rows + per - 1) / per > p.B ? (rows + per - 1) / per * Hk : (int64_t)p.B * Hk;
+  const int64_t want = 4 * (int64_t)cus, most = keys / (few ? 512 : 512);
+  int splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (want + blocks - 1) / std::max<int64_t>(blocks, 1), 32}));
+  CallScratch held(ctx);
+  Parts part{nullptr, nullptr};
+  const int64_t all = (int64_t)p.Tq * p.H;
+  if (splits > 1) {
+    if (held.take((size_t)(splits * all * (64 * 4 + 8)))) {
+      part.o = (float*)held.p;
+      part.ml = (float2*)(part.o + splits * all * 64);
+    } else {
+      splits = 1;  // no memory for the parts: unsplit
+    }
+  }
+  auto go = [&](auto bf, auto cap, auto bias) {
+    constexpr bool BF = decltype(bf)::value, CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
+    static std::atomic<uint64_t> attr{0};
+    if (few) packed_launch(ctx, packed_attn_few<BF, CAP, BIAS>, attr, kFewLds, kRowsF, p, splits, part);
+    else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, kRowsB, p, splits, part);
+  };
+  auto by_score = [&](auto bf) {
+    const std::true_type yes{};
+    const std::false_type no{};
+    if (p.cap > 0.f && p.slopes) go(bf, yes, yes);
+    else if (p.cap > 0.f) go(bf, yes, no);
+    else if (p.slopes) go(bf, no, yes);
+    else go(bf, no, no);
+  };
+  if (dt == HB_BF16) by_score(std::true_type{});
+  else by_score(std::false_type{});
+  if (splits > 1) {
+    check_launch("hb_sdpa_packed");
+    packed_attn_join<true><<<(unsigned)((all + 3) / 4), 256, 0, stream_of(ctx)>>>(dt, part, splits, all, p.O);
+  }
 }
 
 }  // namespace hb
@@ -162,7 +709,9 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   p.half = window < 0 ? -1 : (int)(window / 2 < (1ll << 30) ? window / 2 : (1ll << 30) - 1);
   p.scale = scale;
   p.cap = cap;
-  packed_attn_any<<<dim3((unsigned)Tq, (unsigned)H), 64, (size_t)(D + 128) * 4, stream_of(ctx)>>>(p, dt);
+  const bool mfma = (dt == HB_F16 || dt == HB_BF16) && packed_takes_mfma(p, 8);
+  if (mfma) packed_mfma(ctx, dt, p);
+  else packed_any(ctx, dt, p);
   check_launch("hb_sdpa_packed");
   HB_API_END
 }
