@@ -122,6 +122,9 @@ struct QW {  // quantized weight operand
   int group;  // values per group
 };
 
+// Dequantizes `rows` rows of a quantized weight into 16-bit weights (gemm.hip).
+void dequantize_rows(hipStream_t st, int cus, int dt, int bits, int mode, const QW& q, uint16_t* out, int64_t rows, int K);
+
 // The fused-projection epilogue (QKV): y = x . W^T with W the
 // stacked [3 * H * 64, K] q / k / v projection, written head-major as
 // [3][B][H][L][64] (B = M / L) with RoPE applied to the q and k parts.
@@ -442,13 +445,29 @@ __device__ __forceinline__ void ring_wait_stages(int later) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, int NST, bool BF16, bool GEGLU>
+// What a projection with adapters multiplies beyond K (EXT of gemm_ring): the
+// tile's rows have some distinct adapters (index[row] in [0, n)); number them as
+// they first occur, lay their ranks side by side, and columns [o R, (o + 1) R) of
+// this axis hold s of the rows whose adapter has number o, zeros in the others',
+// against B of that adapter.  So rows of several adapters go through the same
+// products, a stage of 64 ranks at a time, and ranks below 64 share one.
+struct NoExt {};
+struct LoraExt {
+  const uint16_t* s;     // [M, R], scaled; rows without an adapter are not read
+  const uint16_t* b;     // [n, N, R], below 2^31 bytes
+  const int32_t* index;  // [M]
+  int n, R;              // R % 8 == 0
+};
+
+template <int BM, int BN, int WM, int WN, int NST, bool BF16, bool GEGLU, class EXT = NoExt>
 __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restrict__ X, int64_t ldx,
                                                          const uint16_t* __restrict__ W,
                                                          const uint16_t* __restrict__ bias,
                                                          const uint16_t* __restrict__ R, int64_t ldr,
                                                          uint16_t* __restrict__ Y, int64_t ldy, int M, int N, int K,
-                                                         int tiles_n, int xpan, int ypan) {
+                                                         int tiles_n, int xpan, int ypan, EXT ext) {
+  constexpr bool LORA = std::is_same_v<EXT, LoraExt>;
+  static_assert(!LORA || !GEGLU, "adapters go beside a plain projection");
   constexpr int NW = WM * WN, NT = NW * 64;
   constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32;
   constexpr int PCS = (BM + BN) / 8, PW = PCS / NW;  // 1 KB pieces (8 rows x 64 k) per stage, per wave
@@ -504,7 +523,83 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
   }
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)smem);
+  const int KT0 = K >> 6;
+  int KT = KT0;
+  // The tile's adapters by number, and the number of each row's (-1: none)
+  __shared__ int adapter[LORA ? BM : 1];
+  __shared__ int number[LORA ? BM : 1];
+  int xnum[LORA ? PW : 1];  // of the rows of this lane's X pieces
+  if constexpr (LORA) {
+    constexpr int Q = (BM + 63) / 64;
+    int a[Q], num[Q];
+    uint64_t left[Q], any = 0;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+      const int r = q * 64 + lane;
+      a[q] = r < BM && m0 + r < M ? ext.index[m0 + r] : -1;
+      if (a[q] >= ext.n) a[q] = -1;
+      num[q] = -1;
+      left[q] = __ballot(a[q] >= 0);
+      any |= left[q];
+    }
+    int nd = 0;
+    while (any != 0) {  // (at most one round per row)
+      int cur = 0;
+#pragma unroll
+      for (int q = Q - 1; q >= 0; q--)
+        if (left[q] != 0) cur = __builtin_amdgcn_readlane(a[q], __builtin_ctzll(left[q]));
+      any = 0;
+#pragma unroll
+      for (int q = 0; q < Q; q++) {
+        if (a[q] == cur) num[q] = nd;
+        left[q] &= ~__ballot(a[q] == cur);
+        any |= left[q];
+      }
+      if (tid == 0) adapter[nd] = cur;
+      nd++;
+    }
+    if (wave == 0) {
+#pragma unroll
+      for (int q = 0; q < Q; q++)
+        if (q * 64 + lane < BM) number[q * 64 + lane] = num[q];
+    }
+    KT += (nd * ext.R + 63) >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PW; i++) {
+      const int r = (wave * PW + i) * 8 + (lane >> 3);
+      xnum[i] = r < BM ? number[r] : nd;  // W: the numbers there are
+    }
+  }
+  // stage kt - KT0 of the adapters' axis
+  auto issue_ext = [&](int kt, int slot, int i0, int i1) __attribute__((always_inline)) {
+    if constexpr (LORA) {
+      const int r8 = ext.R >> 3;  // chunks of an adapter
+#pragma unroll
+      for (int i = i0; i < i1; i++) {
+        const int p = wave * PW + i, r = p * 8 + (lane >> 3);
+        const int chunk = (kt - KT0) * 8 + ((lane & 7) ^ ((r >> 1) & 7)), o = chunk / r8, c = chunk - o * r8;
+        uint32_t at = 0xfffffff0u;  // past the records: zeros
+        uint64_t base;
+        if (p * 8 < BM) {
+          base = (uint64_t)(ext.s + (int64_t)m0 * ext.R);
+          if (xnum[i] == o) at = (uint32_t)(r * ext.R + c * 8) * 2u;
+        } else {
+          base = (uint64_t)ext.b;
+          const int n = n0 + r - BM, nc = n < N ? n : N - 1;
+          if (o < xnum[i]) at = (uint32_t)(((int64_t)adapter[o] * N + nc) * ext.R + c * 8) * 2u;
+        }
+        const uint4v rs = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base),
+                           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu), 0x80000000u,
+                           0x00020000u};
+        buffer_lds16(rs, at, lds0 + (uint32_t)(slot * STAGE * 2 + (wave * PW + i) * 1024));
+      }
+    }
+  };
   auto issue = [&](int kt, int slot, int i0, int i1) __attribute__((always_inline)) {
+    if constexpr (LORA) {
+      if (kt >= KT0) return issue_ext(kt, slot, i0, i1);
+    }
 #pragma unroll
     for (int i = i0; i < i1; i++)
       buffer_lds16(rsrc[i], off[i], (uint32_t)kt * step[i], lds0 + (uint32_t)(slot * STAGE * 2 + (wave * PW + i) * 1024));
@@ -548,7 +643,6 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
     }
   };
 
-  const int KT = K >> 6;
   // stages 0 .. NST - 2 in flight; stage 0 landed
 #pragma unroll
   for (int s = 0; s < NST - 1; s++)
@@ -594,6 +688,34 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
         }
         *(uint2v*)(Cs + orow * BN + tc + c) =
             uint2v{(uint32_t)o[0] | ((uint32_t)o[1] << 16), (uint32_t)o[2] | ((uint32_t)o[3] << 16)};
+      }
+    }
+  }
+  if constexpr (LORA) {
+    // The zeros of other rows do not keep a non-finite B out of a row's sums (0 *
+    // inf): an output that has come out non-finite is computed again with its own
+    // row's adapter alone.
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) z = fmaf(acc[i][j][r], 0.f, z);
+    if (__syncthreads_or(z != 0.f)) {
+#pragma unroll 1
+      for (int q = tid; q < BM * BN; q += NT) {
+        const int m = m0 + q / BN, n = n0 + q % BN;
+        const float v = to_f<BF16>(Cs[q]);
+        if (m >= M || n >= N || v * 0.f == 0.f) continue;
+        float sum = 0.f;
+        for (int k = 0; k < K; k++) sum = fmaf(to_f<BF16>(X[(int64_t)m * ldx + k]), to_f<BF16>(W[(int64_t)n * K + k]), sum);
+        const int a = ext.index[m];
+        if (a >= 0 && a < ext.n)
+          for (int r = 0; r < ext.R; r++)
+            sum = fmaf(to_f<BF16>(ext.s[(int64_t)m * ext.R + r]),
+                       to_f<BF16>(ext.b[((int64_t)a * N + n) * ext.R + r]), sum);
+        Cs[q] = from_f<BF16>(sum + (bias != nullptr ? to_f<BF16>(bias[n]) : 0.f));
       }
     }
   }
@@ -1430,13 +1552,13 @@ void launch_arow(hipStream_t st, int cus, unsigned pan, const uint16_t* x, int64
                                (pan & HB_Y_PANEL) ? 1 : 0, qk);
 }
 
-template <int BM, int BN, int WM, int WN, int NST, bool BF16, bool GEGLU>
+template <int BM, int BN, int WM, int WN, int NST, bool BF16, bool GEGLU, class EXT = NoExt>
 void launch_ring_t(hipStream_t st, unsigned pan, const uint16_t* x, int64_t ldx, const uint16_t* w, const uint16_t* bias,
-                   const uint16_t* r, int64_t ldr, uint16_t* y, int64_t ldy, int M, int N, int K) {
+                   const uint16_t* r, int64_t ldr, uint16_t* y, int64_t ldy, int M, int N, int K, EXT ext) {
   constexpr int BNO = GEGLU ? BN / 2 : BN;
   constexpr int lds = NST * (BM + BN) * 128;
   static_assert(lds >= BM * BN * 2 && lds <= 160 * 1024, "the C tile reuses the ring");
-  auto kern = gemm_ring<BM, BN, WM, WN, NST, BF16, GEGLU>;
+  auto kern = gemm_ring<BM, BN, WM, WN, NST, BF16, GEGLU, EXT>;
   static std::atomic<uint64_t> attr{0};
   once_per_device(attr, [&] {
     HB_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
@@ -1444,7 +1566,8 @@ void launch_ring_t(hipStream_t st, unsigned pan, const uint16_t* x, int64_t ldx,
   const int64_t tiles_m = (M + BM - 1) / BM, tiles_n = (N + BNO - 1) / BNO;
   HB_REQUIRE(tiles_m * tiles_n < (1ll << 31), "hb_linear: too many tiles");
   kern<<<(unsigned)(tiles_m * tiles_n), WM * WN * 64, lds, st>>>(x, ldx, w, bias, r, ldr, y, ldy, M, N, K, (int)tiles_n,
-                                                                  (pan & HB_X_PANEL) ? 1 : 0, (pan & HB_Y_PANEL) ? 1 : 0);
+                                                                  (pan & HB_X_PANEL) ? 1 : 0, (pan & HB_Y_PANEL) ? 1 : 0,
+                                                                  ext);
 }
 
 // Operands that the ring kernel's and the large-M kernel's 32-bit offsets reach
@@ -1617,7 +1740,7 @@ void mfma_dispatch(hipStream_t st, int cus, unsigned pan, const uint16_t* x, int
   const LinearKernel kern = QB == 0 ? linear_kernel(cus, M, N, K, (pan & HB_X_PANEL) ? K : ldx, GEGLU, pan != 0, qw.q != nullptr)
                                     : code_kernel(cus, M, N, GEGLU);
   if constexpr (QB == 0) {
-    auto args = [&](auto launch) { launch(st, pan, x, ldx, w, bias, r, ldr, y, ldy, M, N, K); };
+    auto args = [&](auto launch) { launch(st, pan, x, ldx, w, bias, r, ldr, y, ldy, M, N, K, NoExt{}); };
     auto arow = [&](auto launch) { launch(st, cus, pan, x, ldx, w, bias, r, ldr, y, ldy, M, N, K, QK{nullptr, 1, 1}); };
     switch (kern) {
       case LinearKernel::kRing32x64: return args(launch_ring_t<32, 64, 1, 2, 6, BF16, GEGLU>);

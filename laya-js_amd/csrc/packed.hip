@@ -158,6 +158,85 @@ __device__ __forceinline__ float2 rope_at_cs(const RopeAt& f, const int32_t* pos
   return float2{(float)c, (float)s};
 }
 
+// Rows of 16-byte aligned chunks (V values each, D / 2 a multiple of V): a block
+// takes TB tokens, computes the cosines and sines of their D / 2 angles once for
+// all heads, and rotates the chunk pairs (c, c + D / 2) of its heads, four loads
+// of a thread in flight.  Bound by reading and writing the heads; a sine and
+// cosine in f64 cost a block about as much as 16 KB of traffic, so TB tokens
+// share a block where there are enough of them.
+constexpr int kRopeTokens = 8;  // 256 threads: one angle each at D = 64
+template <class T, int V, bool BF16>
+__device__ __forceinline__ void rope_load(const T* p, float (&v)[V]) {
+  if constexpr (V == 4) {
+    const float4v x = *(const float4v*)p;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = x[e];
+  } else {
+    const uint4v x = *(const uint4v*)p;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const uint16_t h = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
+      v[e] = BF16 ? bf16_to_f32(h) : f16_bits_to_f32(h);
+    }
+  }
+}
+template <class T, int V, bool BF16>
+__device__ __forceinline__ void rope_store(T* p, const float (&v)[V]) {
+  if constexpr (V == 4) {
+    *(float4v*)p = float4v{v[0], v[1], v[2], v[3]};
+  } else {
+    uint4v x;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t a = BF16 ? f32_to_bf16(v[2 * e]) : f32_to_f16_bits(v[2 * e]);
+      const uint32_t c = BF16 ? f32_to_bf16(v[2 * e + 1]) : f32_to_f16_bits(v[2 * e + 1]);
+      x[e] = a | (c << 16);
+    }
+    *(uint4v*)p = x;
+  }
+}
+template <class T, int V, bool BF16>
+__global__ __launch_bounds__(256) void rope_at_vec_kernel(const T* __restrict__ x, int64_t s0, int64_t s1,
+                                                          T* __restrict__ y, int T_, int H, int D, int tb,
+                                                          const int32_t* __restrict__ positions, RopeAt f) {
+  extern __shared__ float2 cs[];  // [tb][D / 2]
+  const int half = D / 2, C = half / V, t0 = blockIdx.x * tb, nt = T_ - t0 < tb ? T_ - t0 : tb;
+  for (int i = threadIdx.x; i < nt * half; i += 256) cs[i] = rope_at_cs(f, positions, T_, t0 + i / half, i % half);
+  __syncthreads();
+  const int per = H * C, n = nt * per;
+  constexpr int U = 4;
+  for (int i0 = threadIdx.x; i0 < n; i0 += 256 * U) {
+    float a[U][V], b[U][V];
+    int at[U];  // angle of the chunk's first pair, or -1
+    int64_t to[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + 256 * u;
+      at[u] = -1;
+      if (i >= n) continue;
+      const int t = i / per, q = i - t * per, h = q / C, c = (q - h * C) * V;
+      const T* from = x + (int64_t)(t0 + t) * s0 + h * s1 + c;
+      rope_load<T, V, BF16>(from, a[u]);
+      rope_load<T, V, BF16>(from + half, b[u]);
+      at[u] = t * half + c;
+      to[u] = ((int64_t)(t0 + t) * H + h) * D + c;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (at[u] < 0) continue;
+      float lo[V], hi[V];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float2 w = cs[at[u] + e];
+        lo[e] = pin_f32(fmaf(-b[u][e], w.y, a[u][e] * w.x));
+        hi[e] = pin_f32(fmaf(a[u][e], w.y, b[u][e] * w.x));
+      }
+      rope_store<T, V, BF16>(y + to[u], lo);
+      rope_store<T, V, BF16>(y + to[u] + half, hi);
+    }
+  }
+}
+
 // Any type, head dimension and strides: one thread per rotation pair.
 __global__ __launch_bounds__(256) void rope_at_kernel(int dt, const void* __restrict__ x, int64_t s0, int64_t s1,
                                                       int64_t s2, void* __restrict__ y, int64_t T, int64_t H, int D,
@@ -243,8 +322,23 @@ int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t 
   }
   if (T * H == 0) return 0;
   HB_REQUIRE(x && y && positions, "hb_rope_at: null argument");
-  rope_at_kernel<<<grid_for(T * H * (D / 2), 256), 256, 0, stream_of(ctx)>>>(
-      dt, (const void*)x, xs[0], xs[1], xs[2], (void*)y, T, H, (int)D, (const int32_t*)positions, f);
+  const int per = dt == HB_F32 ? 4 : 8;  // values of a 16-byte chunk
+  if (D / 2 % per == 0 && xs[2] == 1 && xs[0] % per == 0 && xs[1] % per == 0 && x % 16 == 0 && y % 16 == 0) {
+    const int tb = T >= 2048 ? kRopeTokens : 1;
+    const unsigned grid = (unsigned)((T + tb - 1) / tb);
+    const size_t lds = (size_t)tb * (D / 2) * sizeof(float2);
+    auto go = [&](auto kern, auto v) {
+      using E = decltype(v);
+      kern<<<grid, 256, lds, stream_of(ctx)>>>((const E*)x, xs[0], xs[1], (E*)y, (int)T, (int)H, (int)D, tb,
+                                               (const int32_t*)positions, f);
+    };
+    if (dt == HB_F32) go(rope_at_vec_kernel<float, 4, false>, 0.f);
+    else if (dt == HB_F16) go(rope_at_vec_kernel<uint16_t, 8, false>, (uint16_t)0);
+    else go(rope_at_vec_kernel<uint16_t, 8, true>, (uint16_t)0);
+  } else {
+    rope_at_kernel<<<grid_for(T * H * (D / 2), 256), 256, 0, stream_of(ctx)>>>(
+        dt, (const void*)x, xs[0], xs[1], xs[2], (void*)y, T, H, (int)D, (const int32_t*)positions, f);
+  }
   check_launch("hb_rope_at");
   HB_API_END
 }

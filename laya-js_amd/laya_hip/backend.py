@@ -530,12 +530,13 @@ class PackedDocs:
 class LoraBank:
     """Low-rank adapters of one projection (HipBackend.loraBank): `count`
     adapters of rank `rank`, a [count, rank, in], b [count, out, rank] and f32
-    scales [count]."""
+    scales [count].  16-bit banks hold a whole number of 8 ranks, the last ones
+    zero."""
 
-    def __init__(self, be: "HipBackend", a, b, scales):
+    def __init__(self, be: "HipBackend", a, b, scales, rank: int):
         self._be = be
-        self.a, self.b, self.scales = a, b, scales
-        self.count, self.rank, self.inputs = a.shape
+        self.a, self.b, self.scales, self.rank = a, b, scales, rank
+        self.count, self.held_rank, self.inputs = a.shape
         self.outputs, self.dtype = b.shape[1], a.dtype
 
     def dispose(self) -> None:
@@ -1982,12 +1983,26 @@ class HipBackend:
             s = self.fromHost(HostTensor("f32", (a.shape[0],), np.ones(a.shape[0], np.float32)))
         else:
             s = self._held(scales if scales.dtype == "f32" else self.cast(scales, "f32"))
-        return LoraBank(self, self._held(a), self._held(b), s)
+        rank = a.shape[1]
+        if a.dtype != "f32" and rank % 8:
+            a, b = self._padded(a, 1, -rank % 8), self._padded(b, 2, -rank % 8)
+        return LoraBank(self, self._held(a), self._held(b), s, rank)
+
+    def _padded(self, t: HipTensor, axis: int, more: int) -> HipTensor:
+        """A contiguous copy of t with `more` zeros behind `axis`."""
+        shape = list(t.shape)
+        shape[axis] += more
+        out = self._new(shape, t.dtype)
+        if out.size:
+            self._call("loraBank", "hb_fill", self.ctx, out._st.ptr, 0, out.size * DT[t.dtype][1])
+        if t.size:
+            self._copy_into(t, out._st.ptr, _contig(shape))
+        return out
 
     def _held(self, t: HipTensor) -> HipTensor:
         """A contiguous tensor of t's values with a reference of its own."""
         c = self._contiguous(t)
-        return self._view(c, c.shape, _contig(c.shape), c._off) if c is t else c
+        return self._view(c, c.shape, _contig(c.shape), c._off)
 
     def _lora_operands(self, op: str, x: HipTensor, N: int, K: int, bank: LoraBank, index: HipTensor, bias, tmp: list):
         if not isinstance(bank, LoraBank):
@@ -2007,7 +2022,7 @@ class HipBackend:
             bias = self._plain(bias, x.dtype, tmp)
         _, xp, M, _, ldx = self._rows(x)
         out = self._new(x.shape[:-1] + (N,), x.dtype)
-        tail = (self._ptr(bank.a), self._ptr(bank.b), self._ptr(bank.scales), bank.count, bank.rank, self._ptr(idx))
+        tail = (self._ptr(bank.a), self._ptr(bank.b), self._ptr(bank.scales), bank.count, bank.held_rank, self._ptr(idx))
         return xp, M, ldx, self._ptr(bias) if bias is not None else 0, out, tail
 
     def loraLinear(self, x: HipTensor, w: HipTensor, bank: LoraBank, index: HipTensor,

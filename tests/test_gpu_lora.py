@@ -139,6 +139,26 @@ def test_lora_of_views(b, dtype):
     check(read32(b, b.loraLinear(odd, w, bank, index)), c, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_lora_adapters_do_not_reach_other_rows(b, dtype, what):
+    """A request's non-finite adapter, or input, stays with its own rows."""
+    rng = np.random.default_rng(11)
+    c = case(rng, dtype, 150, 128, 128, 4, 8, index=np.arange(150) // 20 % 5)
+    c["b"][1, 5:9], c["a"][2, 3] = what, what
+    c["x"][149, 0] = what
+    x, bank, index, _ = dev(b, c, dtype)
+    got = read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index))
+    c["b"][1], c["a"][2], c["x"][149] = 0, 0, 0
+    y, mass, delta = ref.lora_linear(c["x"], c["w"], None, c["a"], c["b"], c["scales"].astype(np.float64), c["index"])
+    clean = np.isin(c["index"], [0, 3, 4])
+    clean[149] = False
+    u = U[dtype]
+    tol = u * np.abs(y) + u * delta + u * (np.abs(y) + 2 * delta) + 144 * 2.0 ** -23 * (mass + delta)
+    assert (np.abs(got - y) <= tol)[clean].all()
+    assert not np.isfinite(got[c["index"] == 1][:, 5:9]).any() and not np.isfinite(got[149]).any()
+
+
 def test_lora_empty(b):
     """No rows, no adapters, rank 0, and weights of no inputs."""
     rng = np.random.default_rng(0)
