@@ -108,6 +108,7 @@ static void lora_ring(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, c
   auto go = [&](auto launch) { launch(st, 0u, x, ldx, w, bias, (const uint16_t*)nullptr, (int64_t)0, y, ldy, M, N, K, ext); };
   LinearKernel tile = LinearKernel::kRing64x64x3;
   ring_tile(cus, M, N, K, false, true, false, &tile);
+  if (M >= 4096) tile = LinearKernel::kRing128x256;
   switch (tile) {
     case LinearKernel::kRing32x64: return go(launch_ring_t<32, 64, 1, 2, 6, BF16, false, LoraExt>);
     case LinearKernel::kRing64x64: return go(launch_ring_t<64, 64, 2, 2, 4, BF16, false, LoraExt>);

@@ -514,6 +514,200 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void p
   }
 }
 
+// ------------------------------------------------------------------ f32 (D = 64)
+
+// 32 rows a block; its four waves take the 32-key tiles those rows can see in
+// turn, each with its own maximum, sum and output, and join them in LDS at the
+// end.  Bound by the f32 matrix rate: a tile is 64 MFMAs of 64 cycles.  K goes
+// through a wave-private LDS tile, V straight into operand registers, a whole
+// 128-byte line per 32 lanes.  S^T = K . Q^T leaves lane l with the scores of row
+// l % 32 for keys 8 (r / 4) + 4 (l / 32) + r % 4, which are the columns that the
+// B operand of O^T += V^T . P^T takes when MFMA step r multiplies keys 8 (r / 4) +
+// r % 4 and + 4: weights stay in registers, in f32.
+constexpr int kRows32 = 32, kKeys32 = 32;
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void packed_attn_f32(Packed p, Parts part,
+                                                                                               int splits) {
+  __shared__ __attribute__((aligned(16))) float buf[4][kKeys32 * 64];  // K tiles; the waves' outputs at the end
+  __shared__ float part_m[4][kRows32], part_l[4][kRows32];
+  const int tid = threadIdx.x, lane = tid & 63, lg = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Hk = p.H / p.G, hk = blockIdx.x % Hk;
+  const int64_t slot = blockIdx.x / Hk;
+  int64_t first;
+  const int b = slot_doc<kRows32>(p, slot, lane, &first);
+  const Doc d = packed_doc(p, b);
+  const int64_t at = (slot - first) * kRows32;
+  if (at >= (int64_t)d.nq * p.G) return;  // (the whole block)
+  const int rows = d.nq * p.G, r0 = (int)at, r = r0 + l32, rc = min(r, rows - 1);
+  const Row row = packed_row(p, d, rc, r0, rows, hk);
+  const int shift = d.nk - d.nq;
+  const Tiles ti = row_tiles<kKeys32>(p, d, r0 / p.G + shift, min(r0 + kRows32 - 1, rows - 1) / p.G + shift);
+  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits) + wave, i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const float* Kb = (const float*)p.K + d.k0 * p.ks[0] + hk * p.ks[1];
+  const float* Vb = (const float*)p.V + d.k0 * p.vs[0] + hk * p.vs[1];
+
+  // element e of qf[i] is column 8 i + 4 lg + e, the columns its half supplies to
+  // MFMA steps e of chunk pair i
+  float4v qf[8];
+  {
+    const float* qp = (const float*)p.Q + (d.q0 + rc / p.G) * p.qs[0] + (hk * p.G + rc % p.G) * p.qs[1] + 4 * lg;
+#pragma unroll
+    for (int i = 0; i < 8; i++) qf[i] = *(const float4v*)(qp + 8 * i);
+  }
+  // K tile: 8 lanes a row, chunk c of row r at c ^ (r & 15): a 16-lane pass of the
+  // fragment reads (16 rows, one chunk) covers all 64 banks.  Keys past the
+  // document repeat its last one: their scores are hidden.
+  const int kr = lane >> 3, c8 = lane & 7;
+  float4v klo[4], khi[4];
+  auto load_k = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float* kp = Kb + min(k0 + i * 8 + kr, d.nk - 1) * p.ks[0] + 4 * c8;
+      klo[i] = *(const float4v*)kp;
+      khi[i] = *(const float4v*)(kp + 32);
+    }
+  };
+  auto kslot = [](int r_, int c) { return r_ * 64 + ((c ^ (r_ & 15)) << 2); };
+  float* kb = buf[wave];
+  float16v o[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[e][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (i0 < i1) load_k(ti.at(i0) * kKeys32);
+  for (int i = i0; i < i1; i += 4) {
+    const int k0 = ti.at(i) * kKeys32, cl = tile_class<kKeys32>(d, row, k0);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      *(float4v*)(kb + kslot(q * 8 + kr, c8)) = klo[q];
+      *(float4v*)(kb + kslot(q * 8 + kr, c8 + 8)) = khi[q];
+    }
+    // the tile is this wave's own: its LDS stores and loads only need to stay in
+    // order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // V of the tile, the next tile's K
+    float v[2][16];
+#pragma unroll
+    for (int q = 0; q < 16; q++) {
+      const float* vp = Vb + min(k0 + 8 * (q >> 2) + 4 * lg + (q & 3), d.nk - 1) * p.vs[0] + l32;
+      v[0][q] = vp[0];
+      v[1][q] = vp[32];
+    }
+    if (i + 4 < i1) load_k(ti.at(i + 4) * kKeys32);
+    float16v st;
+#pragma unroll
+    for (int q = 0; q < 16; q++) st[q] = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+      const float4v kf = *(const float4v*)(kb + kslot(l32, 2 * q + lg));
+#pragma unroll
+      for (int e = 0; e < 4; e++) st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[q][e], st, 0, 0, 0);
+    }
+    // (the next tile's stores must not overtake these reads)
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float mx = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 16; q++) {
+      const int key = k0 + 8 * (q >> 2) + 4 * lg + (q & 3);
+      float x = st[q] * p.scale;
+      if constexpr (CAP) x = p.cap * tanhf(x / p.cap);
+      if constexpr (BIAS) x = fmaf(-row.slope, fabsf((float)(row.pos - key)), x);
+      if (cl != 1) x = key_seen(d, row, key) ? x : -INFINITY;
+      st[q] = x;
+      mx = fmaxf(mx, x);
+    }
+    mx = max_xor32(mx);
+    const float mnew = fmaxf(m, mx), mc = mnew == -INFINITY ? 0.f : mnew, alpha = expf(m - mc);
+    m = mnew;
+    float sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; q++) {
+      st[q] = expf(st[q] - mc);
+      sum += st[q];
+    }
+    l = l * alpha + sum;
+    if (!__all(alpha == 1.0f)) {
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int q = 0; q < 16; q++) o[e][q] *= alpha;
+    }
+    // A non-finite V must not reach a row whose weight for that key is 0, as 0 *
+    // inf in the product would: such a tile is added key by key, zero weights
+    // skipped.
+    float fin = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; q++) fin += v[0][q] * 0.f + v[1][q] * 0.f;
+    if (__any(fin != 0.f)) {  // 0 * finite = 0, 0 * (inf or NaN) = NaN
+#pragma unroll
+      for (int q = 0; q < 16; q++) kb[(8 * (q >> 2) + 4 * lg + (q & 3)) * 32 + l32] = st[q];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+      for (int j = 0; j < kKeys32; j++) {
+        const float w = kb[j * 32 + l32];
+        if (w == 0.f) continue;  // keys past the document among them
+        const float* vp = Vb + (k0 + j) * p.vs[0] + 4 * lg;
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int q = 0; q < 16; q++) o[e][q] = fmaf(w, vp[32 * e + 8 * (q >> 2) + (q & 3)], o[e][q]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      continue;
+    }
+#pragma unroll
+    for (int q = 0; q < 16; q++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) o[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e][q], st[q], o[e], 0, 0, 0);
+  }
+  // join the waves: weights exp(m_w - max); wave w finishes registers [8 w, 8 w + 8)
+  const float lw = sum_xor32(l);
+  if (lg == 0) {
+    part_m[wave][l32] = m;
+    part_l[wave][l32] = lw;
+  }
+  __syncthreads();  // every wave is done with its K tile
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int q = 0; q < 16; q++) buf[wave][(e * 16 + q) * 64 + lane] = o[e][q];
+  __syncthreads();
+  float mt = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; w++) mt = fmaxf(mt, part_m[w][l32]);
+  const float mc = mt == -INFINITY ? 0.f : mt;
+  float wt[4], lt = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    wt[w] = expf(part_m[w][l32] - mc);
+    lt += part_l[w][l32] * wt[w];
+  }
+  if (r >= rows) return;
+  const float inv = splits > 1 ? 1.f : lt == 0.f ? 0.f : 1.0f / lt;
+  const int64_t ri = row_index(p, d, r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
+  if (splits > 1 && wave == 0 && lg == 0) part.ml[pr] = float2{mt, lt};
+  float* op = splits > 1 ? part.o + pr * 64 : (float*)p.O + ri * 64;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int x = wave * 8 + h * 4;  // register x: column 32 (x / 16) + 8 (x % 16 / 4) + 4 lg
+    float4v ov;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) a += wt[w] == 0.f ? 0.f : buf[w][(x + e) * 64 + lane] * wt[w];
+      ov[e] = a * inv;
+    }
+    *(float4v*)(op + 32 * (x >> 4) + 8 * ((x & 15) >> 2) + 4 * lg) = ov;
+  }
+}
+
 // Joins the parts of split runs: one wave a row, a lane per column.  E2: maxima in
 // base 2 (the 16-bit kernels), else natural.
 template <bool E2>
@@ -625,13 +819,13 @@ static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, in
 
 static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
   const int64_t rows = (int64_t)p.Tq * p.G;
-  const bool few = rows <= 64 * (int64_t)p.B;
+  const bool f32 = dt == HB_F32, few = f32 || rows <= 64 * (int64_t)p.B;
   const int per = few ? kRowsF : kRowsB, Hk = p.H / p.G, cus = cu_count(ctx);
   // Keys of an average document's rows, and the blocks they make
   int64_t keys = p.B ? p.Tk / p.B : 0;
   if (p.half >= 0) keys = std::min<int64_t>(keys, 2 * (int64_t)p.half + per / p.G + 64);
-  const int64_t blocks = (rows + per - 1) / per > p.B ? (rows + per - 1) / per * Hk : (int64_t)p.B * Hk;
-  const int64_t want = 4 * (int64_t)cus, most = keys / (few ? 512 : 512);
+  const int64_t blocks = std::max<int64_t>((rows + per - 1) / per, p.B) * Hk;
+  const int64_t want = 4 * (int64_t)cus, most = keys / 512;
   int splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (want + blocks - 1) / std::max<int64_t>(blocks, 1), 32}));
   CallScratch held(ctx);
   Parts part{nullptr, nullptr};
@@ -644,25 +838,29 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
       splits = 1;  // no memory for the parts: unsplit
     }
   }
-  auto go = [&](auto bf, auto cap, auto bias) {
-    constexpr bool BF = decltype(bf)::value, CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
-    static std::atomic<uint64_t> attr{0};
-    if (few) packed_launch(ctx, packed_attn_few<BF, CAP, BIAS>, attr, kFewLds, kRowsF, p, splits, part);
-    else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, kRowsB, p, splits, part);
+  auto go = [&](auto cap, auto bias) {
+    constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
+    auto half = [&](auto bf) {
+      constexpr bool BF = decltype(bf)::value;
+      static std::atomic<uint64_t> attr{0};
+      if (few) packed_launch(ctx, packed_attn_few<BF, CAP, BIAS>, attr, kFewLds, kRowsF, p, splits, part);
+      else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, kRowsB, p, splits, part);
+    };
+    std::atomic<uint64_t> none{0};
+    if (f32) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, none, 0, kRows32, p, splits, part);
+    else if (dt == HB_BF16) half(std::true_type{});
+    else half(std::false_type{});
   };
-  auto by_score = [&](auto bf) {
-    const std::true_type yes{};
-    const std::false_type no{};
-    if (p.cap > 0.f && p.slopes) go(bf, yes, yes);
-    else if (p.cap > 0.f) go(bf, yes, no);
-    else if (p.slopes) go(bf, no, yes);
-    else go(bf, no, no);
-  };
-  if (dt == HB_BF16) by_score(std::true_type{});
-  else by_score(std::false_type{});
+  const std::true_type yes{};
+  const std::false_type no{};
+  if (p.cap > 0.f && p.slopes) go(yes, yes);
+  else if (p.cap > 0.f) go(yes, no);
+  else if (p.slopes) go(no, yes);
+  else go(no, no);
   if (splits > 1) {
     check_launch("hb_sdpa_packed");
-    packed_attn_join<true><<<(unsigned)((all + 3) / 4), 256, 0, stream_of(ctx)>>>(dt, part, splits, all, p.O);
+    auto join = f32 ? packed_attn_join<false> : packed_attn_join<true>;
+    join<<<(unsigned)((all + 3) / 4), 256, 0, stream_of(ctx)>>>(dt, part, splits, all, p.O);
   }
 }
 
@@ -709,8 +907,7 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   p.half = window < 0 ? -1 : (int)(window / 2 < (1ll << 30) ? window / 2 : (1ll << 30) - 1);
   p.scale = scale;
   p.cap = cap;
-  const bool mfma = (dt == HB_F16 || dt == HB_BF16) && packed_takes_mfma(p, 8);
-  if (mfma) packed_mfma(ctx, dt, p);
+  if (packed_takes_mfma(p, dt == HB_F32 ? 4 : 8)) packed_mfma(ctx, dt, p);
   else packed_any(ctx, dt, p);
   check_launch("hb_sdpa_packed");
   HB_API_END
