@@ -383,9 +383,12 @@ int hb_meanpool(uintptr_t ctx, int dt_x, uintptr_t x, uintptr_t mask, int64_t B,
  * the last), doc and pos i32 [T] (each row's document and position in it) and,
  * unless 0, slots i32 [T] (its row in the padded [B, L] batch).  A length below
  * 0 counts as 0 and, with L > 0, one above L as L; documents are cut off at T
- * rows.  Rows behind the last document get doc -1, pos 0 and slot -1. */
+ * rows.  Rows behind the last document get doc -1, pos 0 and slot -1.
+ * blocks i32 [T / 128 + B + 1, 2]: the documents in blocks of up to 128 rows, as
+ * (document, first row), then the rows behind the last one as document B, then
+ * (-1, 0): where hb_sdpa_packed's blocks work. */
 int hb_pack_plan(uintptr_t ctx, uintptr_t lengths, int64_t B, int64_t T, int64_t L, uintptr_t offsets, uintptr_t doc,
-                 uintptr_t pos, uintptr_t slots);
+                 uintptr_t pos, uintptr_t slots, uintptr_t blocks);
 /* Rows of the padded batch x [rows, row_bytes] into the packed out [T,
  * row_bytes]: row t is x's row slots[t], or zeros where that is outside x. */
 int hb_pack_rows(uintptr_t ctx, uintptr_t x, int64_t rows, int64_t row_bytes, uintptr_t slots, int64_t T,
@@ -407,8 +410,9 @@ int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t 
 
 /* Attention inside each document of a packed batch, softmax in f32.  q [Tq, H,
  * D], k and v [Tk, Hk, D] by element strides (3 each), o contiguous [Tq, H, D];
- * head h reads key head h / (H / Hk).  Documents are given by q_offsets and
- * k_offsets (i32 [B + 1], of hb_pack_plan); a document's queries are its last
+ * head h reads key head h / (H / Hk).  Documents are given by the plans of
+ * hb_pack_plan: doc, blocks and offsets of the queries' rows, offsets of the keys'
+ * (of B documents both); a document's queries are its last
  * tokens: query i of n_q is at position i + n_k - n_q among its n_k keys.
  * Query i sees key j if j < prefix[b] (i32 [B], or 0: none), or if (not causal,
  * or j <= pos) and (window -1, or |pos - j| <= window / 2).  Scores are scale *
@@ -417,8 +421,8 @@ int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t 
  * behind the last document, are zeros.  Values of hidden keys are not used,
  * whatever they hold. */
 int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t* qs, uintptr_t k, const int64_t* ks, uintptr_t v,
-                   const int64_t* vs, uintptr_t o, uintptr_t q_offsets, uintptr_t k_offsets, int64_t B, int64_t Tq,
-                   int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale, int causal, int64_t window,
+                   const int64_t* vs, uintptr_t o, uintptr_t q_doc, uintptr_t q_blocks, uintptr_t q_offsets,
+                   uintptr_t k_offsets, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale, int causal, int64_t window,
                    uintptr_t prefix, float cap, uintptr_t slopes);
 
 /* ---------------------------------------------------------------- adapters

@@ -40,6 +40,11 @@ inline void once_per_device(std::atomic<uint64_t>& done, Set&& set) {
   done.fetch_or(bit, std::memory_order_acq_rel);
 }
 
+// hb_pack_plan's table of blocks: a block is up to kBlockTokens rows of one document
+// (or of the rows behind the last one), and this many entries are enough.
+constexpr int kBlockTokens = 128;
+inline int64_t plan_blocks(int64_t B, int64_t T) { return T / kBlockTokens + B + 1; }
+
 struct Context;
 hipStream_t stream_of(uintptr_t ctx);
 int device_of(uintptr_t ctx);

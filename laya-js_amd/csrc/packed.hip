@@ -17,25 +17,51 @@ namespace hb {
 // and above L (if L > 0) as L; token t belongs to the last b with off_b <= t,
 // at position t - off_b.
 //
+// The table of blocks: document b has ceil(n_b / kBlockTokens) entries, in order,
+// then come those of the rows behind the last document (as document B), then -1.
+//
 // One launch: every block scans the lengths, 1024 at a time, as far as its own
 // 1024 tokens need, and finds their documents by bisection among the 1024
-// offsets in LDS; block 0 also writes the offsets.  Scanning B lengths again in
-// each block costs less than a second launch would (B / 1024 rounds of one 16-byte
-// read a thread); what bounds it is the launch itself, then the 12 bytes written a
-// token.
+// offsets in LDS; block 0 also writes the offsets, and the last block the end of the
+// table.  Scanning B lengths again in each block costs less than a second launch
+// would (B / 1024 rounds of one 16-byte read a thread); what bounds it is the
+// launch itself, then the 12 bytes written a token.
 constexpr int kPlanDocs = 1024, kPlanTokens = 1024;
 
+// Exclusive sums over the block's 256 threads, and their total.
+__device__ __forceinline__ int64_t scan256(int64_t v, int64_t* wsum, int64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t incl = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t up = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) wsum[wave] = incl;
+  __syncthreads();
+  int64_t base = incl - v;
+  *total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    if (w < wave) base += wsum[w];
+    *total += wsum[w];
+  }
+  return base;
+}
+
 __global__ __launch_bounds__(256) void pack_plan_kernel(const int32_t* __restrict__ lengths, int B, int T, int L,
-                                                        int32_t* __restrict__ offsets, int32_t* __restrict__ doc,
-                                                        int32_t* __restrict__ pos, int32_t* __restrict__ slots) {
-  __shared__ int off[kPlanDocs + 1];
-  __shared__ int64_t wsum[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+                                                        int nblocks, int32_t* __restrict__ offsets,
+                                                        int32_t* __restrict__ doc, int32_t* __restrict__ pos,
+                                                        int32_t* __restrict__ slots, int2* __restrict__ blocks) {
+  __shared__ int off[kPlanDocs + 1], boff[kPlanDocs];
+  __shared__ int64_t wsum[2][4];
+  const int tid = threadIdx.x;
   const int t0 = blockIdx.x * kPlanTokens, t1 = T - t0 < kPlanTokens ? T : t0 + kPlanTokens;
-  const bool first = blockIdx.x == 0;
+  const bool first = blockIdx.x == 0, last = blockIdx.x == gridDim.x - 1;
   int64_t carry = 0;  // sum of the lengths before this round
+  int bcarry = 0;     // and of their blocks
   for (int b0 = 0; b0 < B; b0 += kPlanDocs) {
-    int64_t n[4], sum = 0;
+    int64_t n[4], sum = 0, total;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int b = b0 + 4 * tid + e;
@@ -44,25 +70,21 @@ __global__ __launch_bounds__(256) void pack_plan_kernel(const int32_t* __restric
       n[e] = sum;
       sum += v;
     }
-    int64_t incl = sum;
+    const int64_t base = carry + scan256(sum, wsum[0], &total);
+    total += carry;
+    int nb = 0, bn[4];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t up = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += up;
+    for (int e = 0; e < 4; e++) {  // (cut off at T)
+      const int64_t o = base + n[e], x = base + (e < 3 ? n[e + 1] : sum);
+      const int a = o < T ? (int)o : T, c = x < T ? (int)x : T;
+      off[4 * tid + e] = a;
+      bn[e] = nb;
+      nb += (c - a + kBlockTokens - 1) / kBlockTokens;
     }
-    if (lane == 63) wsum[wave] = incl;
-    __syncthreads();
-    int64_t base = carry + incl - sum, total = carry;
+    int64_t btotal;
+    const int bbase = bcarry + (int)scan256(nb, wsum[1], &btotal);
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-      if (w < wave) base += wsum[w];
-      total += wsum[w];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int64_t o = base + n[e];
-      off[4 * tid + e] = o < T ? (int)o : T;
-    }
+    for (int e = 0; e < 4; e++) boff[4 * tid + e] = bbase + bn[e];
     const int end = total < T ? (int)total : T;  // of this round's documents
     if (tid == 0) off[kPlanDocs] = end;
     __syncthreads();
@@ -77,14 +99,16 @@ __global__ __launch_bounds__(256) void pack_plan_kernel(const int32_t* __restric
         if (off[m] <= t) a = m;
         else c = m;
       }
-      const int d = b0 + a, p = t - off[a];
+      const int d = b0 + a, q = t - off[a];
       doc[t] = d;
-      pos[t] = p;
-      if (slots != nullptr) slots[t] = d * L + p;
+      pos[t] = q;
+      if (slots != nullptr) slots[t] = d * L + q;
+      if (q % kBlockTokens == 0) blocks[boff[a] + q / kBlockTokens] = int2{d, t};
     }
     carry = total;
-    if (!first && end >= t1) break;  // (the same in every thread)
-    __syncthreads();  // off and wsum are written again
+    bcarry += (int)btotal;
+    if (!first && !last && end >= t1) break;  // (the same in every thread)
+    __syncthreads();  // off, boff and wsum are written again
   }
   const int end = carry < T ? (int)carry : T;
   if (first && tid == 0) offsets[B] = end;
@@ -92,7 +116,10 @@ __global__ __launch_bounds__(256) void pack_plan_kernel(const int32_t* __restric
     doc[t] = -1;
     pos[t] = 0;
     if (slots != nullptr) slots[t] = -1;
+    if ((t - end) % kBlockTokens == 0) blocks[bcarry + (t - end) / kBlockTokens] = int2{B, t};
   }
+  if (last)
+    for (int i = bcarry + (T - end + kBlockTokens - 1) / kBlockTokens + tid; i < nblocks; i += 256) blocks[i] = int2{-1, 0};
 }
 
 // ------------------------------------------------------------------ rows
@@ -261,16 +288,16 @@ using namespace hb;
 extern "C" {
 
 int hb_pack_plan(uintptr_t ctx, uintptr_t lengths, int64_t B, int64_t T, int64_t L, uintptr_t offsets, uintptr_t doc,
-                 uintptr_t pos, uintptr_t slots) {
+                 uintptr_t pos, uintptr_t slots, uintptr_t blocks) {
   HB_API_BEGIN
   HB_REQUIRE(B >= 0 && T >= 0 && L >= 0 && B < (1ll << 30) && T < (1ll << 30) && L < (1ll << 30),
              "hb_pack_plan: bad sizes");
-  HB_REQUIRE((B == 0 || lengths) && offsets && (T == 0 || (doc && pos)), "hb_pack_plan: null argument");
+  HB_REQUIRE((B == 0 || lengths) && offsets && blocks && (T == 0 || (doc && pos)), "hb_pack_plan: null argument");
   HB_REQUIRE(!slots || (L > 0 && B * L < (1ll << 31)), "hb_pack_plan: slots need L > 0 and B * L below 2^31");
   const unsigned grid = (unsigned)((T + kPlanTokens - 1) / kPlanTokens);
   pack_plan_kernel<<<grid < 1 ? 1 : grid, 256, 0, stream_of(ctx)>>>((const int32_t*)lengths, (int)B, (int)T, (int)L,
-                                                                    (int32_t*)offsets, (int32_t*)doc, (int32_t*)pos,
-                                                                    (int32_t*)slots);
+                                                                    (int)plan_blocks(B, T), (int32_t*)offsets, (int32_t*)doc,
+                                                                    (int32_t*)pos, (int32_t*)slots, (int2*)blocks);
   check_launch("hb_pack_plan");
   HB_API_END
 }

@@ -19,9 +19,8 @@
 // share what they read.  A block finds its document by its slot: document b has
 // slots from off_b G / R + b on (R rows a block, rounded down), which leaves every
 // document enough of them without a table, whatever the lengths.
-// Both go through the 64-key tiles that some row of the block can see: those of
-// the prefix, then the run from the first row's lowest key to the last row's
-// highest.  A long run may be split over `splits` blocks; packed_attn_join adds up
+// Both go through the 64-key tiles that some row of the block can see (tiles_of).
+// A long run may be split over `splits` blocks; packed_attn_join adds up
 // their parts.
 //
 // packed_attn_f32: f32, on v_mfma_f32_32x32x2_f32.
@@ -43,6 +42,9 @@ struct Packed {
   void* O;                 // [Tq, H, D]
   int64_t qs[3], ks[3], vs[3];  // element strides: token, head, column
   const int32_t *qoff, *koff;  // [B + 1]
+  const int32_t* doc;      // [Tq], outside [0, B) behind the last document
+  const int32_t* blocks;   // [nblocks, 2]: document (below 0: none) and first row of each block of tokens
+  int nblocks;
   const int32_t* prefix;   // [B], or null
   const float* slopes;     // [H], or null
   int B, Tq, Tk, H, G, D;  // G: query heads of a key head
@@ -57,12 +59,14 @@ struct Doc {
 };
 __device__ __forceinline__ Doc packed_doc(const Packed& p, int b) {
   Doc d;
-  d.q0 = min(max(p.qoff[b], 0), p.Tq);
   if (b >= p.B) {
+    d.q0 = min(max(p.qoff[p.B], 0), p.Tq);
     d.nq = p.Tq - d.q0;
-    d.k0 = d.nk = d.prefix = 0;
+    d.k0 = min(max(p.koff[p.B], 0), p.Tk);  // (behind the last key, so that nothing behind it is visited)
+    d.nk = d.prefix = 0;
     return d;
   }
+  d.q0 = min(max(p.qoff[b], 0), p.Tq);
   d.nq = min(max(p.qoff[b + 1], d.q0), p.Tq) - d.q0;
   d.k0 = min(max(p.koff[b], 0), p.Tk);
   d.nk = min(max(p.koff[b + 1], d.k0), p.Tk) - d.k0;
@@ -70,20 +74,62 @@ __device__ __forceinline__ Doc packed_doc(const Packed& p, int b) {
   return d;
 }
 
-// The keys that a query at `pos` sees besides the prefix: [lo, hi]
-__device__ __forceinline__ void packed_range(const Packed& p, int nk, int pos, int* lo, int* hi) {
-  *lo = p.half >= 0 ? max(pos - p.half, 0) : 0;
-  *hi = p.half >= 0 ? min(pos + p.half, nk - 1) : nk - 1;  // (both below 2^30)
-  if (p.causal) *hi = min(*hi, pos);
+// What query t of document d sees, as rows of the packed keys: [lo, end), and the
+// prefix [p0, pend).  All four grow with t, across documents too.
+struct Seen {
+  int pos, lo, end, p0, pend;
+};
+__device__ __forceinline__ Seen seen_by(const Packed& p, const Doc& d, int t) {
+  Seen s;
+  const int pos = t - d.q0 + d.nk - d.nq;
+  int hi = p.half >= 0 ? min(pos + p.half, d.nk - 1) : d.nk - 1;  // (both terms below 2^30)
+  if (p.causal) hi = min(hi, pos);
+  s.pos = d.k0 + pos;
+  s.lo = d.k0 + (p.half >= 0 ? max(pos - p.half, 0) : 0);
+  s.end = d.k0 + max(hi + 1, 0);
+  s.p0 = d.k0;
+  s.pend = d.k0 + d.prefix;
+  return s;
 }
+
+static_assert(kBlockTokens == 128, "a block of tokens is G blocks of rows");
 
 // ------------------------------------------------------------------ rows and tiles
 
-// The document of slot `slot`: the last b with off_b * G / R + b <= slot (the
-// documents' first slots; document B holds the rows behind the last one).  All
-// 64 lanes probe at once, so up to 63 documents take one round of loads.
+__device__ __forceinline__ int by_g(const Packed& p, int r) { return p.G == 1 ? r : r / p.G; }
+__device__ __forceinline__ int mod_g(const Packed& p, int r) { return p.G == 1 ? 0 : r % p.G; }
+
+// The document and the first row in it of block slot `slot`, of blocks that take R
+// rows of one document; false: none, the block has nothing to do.
+// Up to 63 documents: lane b counts document b's blocks, and the slots are dealt
+// out exactly (lane B stands for the rows behind the last document).  Else
+// document b has the slots from off_b G / R + b on, rounded down, which leaves each
+// enough of them; all 64 lanes probe at once for the last b that begins at or
+// before the slot.
 template <int R>
-__device__ __forceinline__ int slot_doc(const Packed& p, int64_t slot, int lane, int64_t* first) {
+__device__ __forceinline__ bool slot_doc(const Packed& p, int64_t slot, int lane, Doc* d, int* r0) {
+  if (p.B < 64) {
+    Doc x{0, 0, 0, 0, 0};
+    if (lane <= p.B) x = packed_doc(p, lane);
+    const int cnt = (x.nq * p.G + R - 1) / R;
+    int start = cnt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(start, o, 64);
+      if (lane >= o) start += up;
+    }
+    start -= cnt;
+    const uint64_t hit = __ballot(slot >= start && slot < (int64_t)start + cnt);
+    if (hit == 0) return false;
+    const int b = __builtin_ctzll(hit);
+    d->q0 = __builtin_amdgcn_readlane(x.q0, b);
+    d->nq = __builtin_amdgcn_readlane(x.nq, b);
+    d->k0 = __builtin_amdgcn_readlane(x.k0, b);
+    d->nk = __builtin_amdgcn_readlane(x.nk, b);
+    d->prefix = __builtin_amdgcn_readlane(x.prefix, b);
+    *r0 = ((int)slot - __builtin_amdgcn_readlane(start, b)) * R;
+    return true;
+  }
   auto base = [&](int b) { return (int64_t)min(max(p.qoff[b], 0), p.Tq) * p.G / R + b; };
   int lo = 0, n = p.B + 1;
   while (n > 1) {
@@ -92,57 +138,53 @@ __device__ __forceinline__ int slot_doc(const Packed& p, int64_t slot, int lane,
     lo += (cnt - 1) * step;
     n = min(step, n - (cnt - 1) * step);
   }
-  *first = base(lo);
-  return lo;
+  *d = packed_doc(p, lo);
+  const int64_t at = (slot - base(lo)) * R;
+  *r0 = (int)at;
+  return at < (int64_t)d->nq * p.G;
 }
 
-// The tiles of KT keys that rows at positions pb0 .. pb1 can see: `pre` tiles of
-// the prefix, then those from run0 on, `n` in all.
+// The tiles of KT keys that some of a document's rows can see, from what the first
+// and the last of them see: those of the prefix, then the run from the first row's
+// first key to the last row's last.  bound: the end of both.
 struct Tiles {
-  int pre, run0, n;
-  __device__ __forceinline__ int at(int i) const { return i < pre ? i : run0 + i - pre; }
+  int a0, na, b0, n, bound;
+  template <int KT>
+  __device__ __forceinline__ int at(int i) const { return i < na ? a0 + KT * i : b0 + KT * (i - na); }
 };
 template <int KT>
-__device__ __forceinline__ Tiles row_tiles(const Packed& p, const Doc& d, int pb0, int pb1) {
+__device__ __forceinline__ Tiles tiles_of(const Seen& f, const Seen& l) {
   Tiles t;
-  int lo, hi, x;
-  packed_range(p, d.nk, pb0, &lo, &x);
-  packed_range(p, d.nk, pb1, &x, &hi);
-  t.pre = (d.prefix + KT - 1) / KT;
-  t.run0 = max(lo / KT, t.pre);
-  t.n = t.pre + (hi >= lo ? max(hi / KT + 1 - t.run0, 0) : 0);
+  t.a0 = l.p0;
+  t.na = (l.pend - l.p0 + KT - 1) / KT;
+  t.b0 = max(f.lo, t.a0 + KT * t.na);
+  t.bound = max(l.end, l.pend);
+  t.n = t.na + (max(l.end - t.b0, 0) + KT - 1) / KT;
   return t;
 }
 
-// One lane's row, and the visibility of a tile for all rows of its wave
-struct Row {
-  int pos, lo, span;  // key j is visible if j < prefix or j - lo <= span, unsigned
-  int lo0, lo1, hi0, hi1;  // ranges of the wave's first and last rows' positions
+// One lane's row, and what its wave's first and last rows see
+struct Row : Seen {
+  Seen f, l;
   float slope;
 };
-__device__ __forceinline__ Row packed_row(const Packed& p, const Doc& d, int r, int rw0, int rows, int hk) {
-  // (a wave without rows, rw0 >= rows, repeats the last one: its caller skips it)
-  Row w;
-  const int shift = d.nk - d.nq, last = min(rw0 + 31, rows - 1);
-  int hi, x;
-  w.pos = r / p.G + shift;
-  packed_range(p, d.nk, w.pos, &w.lo, &hi);
-  if (hi < w.lo) w.lo = 1 << 30, hi = w.lo;  // sees nothing of the run: keys are below 2^30
-  w.span = hi - w.lo;
-  packed_range(p, d.nk, min(rw0, rows - 1) / p.G + shift, &w.lo0, &w.hi0);
-  packed_range(p, d.nk, last / p.G + shift, &w.lo1, &w.hi1);
-  w.slope = p.slopes == nullptr ? 0.f : p.slopes[hk * p.G + r % p.G];
-  return w;
-}
 // 0: no row sees a key of the tile, 1: every row sees every key, 2: neither
 template <int KT>
-__device__ __forceinline__ int tile_class(const Doc& d, const Row& w, int k0) {
-  if (k0 + KT <= d.prefix) return 1;
-  if (k0 >= d.prefix && (k0 > w.hi1 || k0 + KT - 1 < w.lo0)) return 0;
-  return k0 + KT <= d.nk && k0 >= w.lo1 && k0 + KT - 1 <= w.hi0 ? 1 : 2;
+__device__ __forceinline__ int tile_class(const Row& w, int k0) {
+  if ((k0 >= w.l.lo && k0 + KT <= w.f.end) || (k0 >= w.l.p0 && k0 + KT <= w.f.pend)) return 1;
+  return (k0 >= w.l.end || k0 + KT <= w.f.lo) && (k0 >= w.l.pend || k0 + KT <= w.f.p0) ? 0 : 2;
 }
-__device__ __forceinline__ bool key_seen(const Doc& d, const Row& w, int j) {
-  return j < d.prefix || (uint32_t)(j - w.lo) <= (uint32_t)w.span;
+// ones in the bits below n
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+// Bit i: the row sees key k0 + i
+__device__ __forceinline__ uint32_t seen_bits(const Seen& w, int k0) {
+  return (bits_below(w.pend - k0) & ~bits_below(w.p0 - k0)) | (bits_below(w.end - k0) & ~bits_below(w.lo - k0));
+}
+// x where the bit of `seen` is set, else -inf (the bit sign-extended to a word: one
+// extract and one bit-field insert a score)
+__device__ __forceinline__ float seen_or(uint32_t seen, int bit, float x) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)seen, bit, 1);
+  return __uint_as_float((__float_as_uint(x) & m) | (~m & 0xff800000u));
 }
 
 // Parts of a split run: per split and row (token * H + head) the unscaled output,
@@ -201,19 +243,34 @@ __device__ __forceinline__ void wave_init(Wave& w, const Score& sc, const uint16
   w.l = 0.f;
 }
 
+// sum + both halves of a packed pair, in f32
+template <bool BF16>
+__device__ __forceinline__ float add_pair(uint32_t p, float sum) {
+  if constexpr (BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum,
+                                           false);
+  } else {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, p), __builtin_bit_cast(half2v, 0x3c003c00u), sum, false);
+  }
+}
+
 // One tile of 64 keys in LDS: scores, mask (`mixed`), online softmax, O += P V.
 // Weights are rounded to the 16-bit type for the second product, as MFMA takes
-// them; their sum is of the unrounded ones.
+// them, and their sum is of the rounded ones (one dot product a pair).
 template <bool BF16, bool CAP, bool BIAS>
 __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16_t* Kc, const uint16_t* Vc, int k0,
-                                          const Doc& d, const Row& row, bool mixed, const Score& sc, int lg) {
+                                          const Row& row, bool mixed, const Score& sc, int lg) {
   float16v st[2];
 #pragma unroll
   for (int kb = 0; kb < 2; kb++) {
+    uint4v kf[4];
+#pragma unroll
+    for (int s = 0; s < 4; s++) kf[s] = *(const uint4v*)(Kc + f.ka[s] + kb * 2048);
 #pragma unroll
     for (int r = 0; r < 16; r++) st[kb][r] = 0.f;
 #pragma unroll
-    for (int s = 0; s < 4; s++) st[kb] = mfma32x16<BF16>(*(const uint4v*)(Kc + f.ka[s] + kb * 2048), w.qf[s], st[kb]);
+    for (int s = 0; s < 4; s++) st[kb] = mfma32x16<BF16>(kf[s], w.qf[s], st[kb]);
   }
   if constexpr (CAP || BIAS) {
 #pragma unroll
@@ -224,10 +281,11 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
   }
   if (mixed) {
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++)
+    for (int kb = 0; kb < 2; kb++) {
+      const uint32_t seen = seen_bits(row, k0 + 32 * kb) >> (4 * lg);
 #pragma unroll
-      for (int r = 0; r < 16; r++)
-        st[kb][r] = key_seen(d, row, k0 + 32 * kb + 8 * (r >> 2) + 4 * lg + (r & 3)) ? st[kb][r] : -INFINITY;
+      for (int r = 0; r < 16; r++) st[kb][r] = seen_or(seen, 8 * (r >> 2) + (r & 3), st[kb][r]);
+    }
   }
   float mx = -INFINITY;
 #pragma unroll
@@ -235,11 +293,20 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
 #pragma unroll
     for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[kb][r]);
   mx = max_xor32(mx);
-  const float mnew = fmaxf(w.m, mx);
-  const float mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
-  const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc);
-  w.m = mnew;
-  float psum = 0.f;
+  // Weights are relative to w.m, which follows the maximum once it is left behind by
+  // a factor of 2^8 for some row of the wave: up to there they fit the 16-bit types
+  // as well, and O and the sum need no rescaling.
+  if (!__all(mx * sc.mul <= fmaf(w.m, sc.mul, 8.f))) {
+    const float mnew = fmaxf(w.m, mx), mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
+    const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc);
+    w.m = mnew;
+    w.l *= alpha;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) w.o[e][r] *= alpha;
+  }
+  const float mc = w.m == -INFINITY ? 0.f : w.m * sc.mul;
   uint4v pf[4];
 #pragma unroll
   for (int t = 0; t < 4; t++) {
@@ -248,17 +315,10 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
     for (int e = 0; e < 8; e += 2) {
       const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t >> 1][8 * (t & 1) + e], sc.mul, -mc));
       const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t >> 1][8 * (t & 1) + e + 1], sc.mul, -mc));
-      psum += p0 + p1;
       pk[e >> 1] = pack2<BF16>(p0, p1);
+      w.l = add_pair<BF16>(pk[e >> 1], w.l);
     }
     pf[t] = uint4v{pk[0], pk[1], pk[2], pk[3]};
-  }
-  w.l = w.l * alpha + psum;
-  if (!__all(alpha == 1.0f)) {  // rescale O only when some row max of this wave moved
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) w.o[e][r] *= alpha;
   }
 #pragma unroll
   for (int t = 0; t < 4; t++)
@@ -275,8 +335,8 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
 // slow, and never run on finite data.  tiles [i0, i1) in steps of `step`.
 template <bool BF16, bool CAP, bool BIAS>
 __device__ __forceinline__ Wave wave_again(Wave w, const uint16_t* Kb, int64_t kst, const uint16_t* Vb, int64_t vst,
-                                        Doc d, Row row, Tiles ti, int i0, int i1, int step,
-                                        Score sc, int lg) {
+                                           const Row& row, const Tiles& ti, int i0, int i1, int step,
+                                           const Score& sc, int lg) {
 #pragma unroll
   for (int e = 0; e < 2; e++)
 #pragma unroll
@@ -285,7 +345,7 @@ __device__ __forceinline__ Wave wave_again(Wave w, const uint16_t* Kb, int64_t k
   w.l = 0.f;
 #pragma unroll 1
   for (int i = i0; i < i1; i += step) {
-    const int k0 = ti.at(i) * 64, k1 = min(k0 + 64, d.nk);
+    const int k0 = ti.at<64>(i), k1 = min(k0 + 64, ti.bound);
 #pragma unroll 1
     for (int j = k0; j < k1; j++) {
       const uint16_t* kr = Kb + j * kst + 8 * lg;
@@ -300,12 +360,12 @@ __device__ __forceinline__ Wave wave_again(Wave w, const uint16_t* Kb, int64_t k
         }
       }
       x = score<CAP, BIAS>(sc, row.slope, row.pos, j, sum_xor32(x));
-      x = key_seen(d, row, j) ? x : -INFINITY;
+      x = seen_bits(row, j) & 1u ? x : -INFINITY;
       const float mnew = fmaxf(w.m, x), mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
       const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc), pr = __builtin_amdgcn_exp2f(fmaf(x, sc.mul, -mc));
       w.m = mnew;
-      w.l = w.l * alpha + (lg == 0 ? pr : 0.f);  // (the halves' sums are added up later)
       const float p16 = tof<BF16>(fromf<BF16>(pr));
+      w.l = w.l * alpha + (lg == 0 ? p16 : 0.f);  // (the halves' sums are added up later)
 #pragma unroll
       for (int e = 0; e < 2; e++)
 #pragma unroll
@@ -331,12 +391,24 @@ __device__ __forceinline__ bool wave_finite(const Wave& w) {
   return !__any(z != 0.f);  // 0 * finite = 0, 0 * (inf or NaN) = NaN
 }
 
-__device__ __forceinline__ int64_t row_index(const Packed& p, const Doc& d, int r, int hk) {
-  return (int64_t)(d.q0 + r / p.G) * p.H + hk * p.G + r % p.G;
+// The output row of a row (a query and one of its G heads)
+__device__ __forceinline__ int64_t row_index(const Packed& p, int t, int r, int hk) {
+  return (int64_t)t * p.H + hk * p.G + mod_g(p, r);
+}
+// A lane's row among rows of one document, r of them from rw0 on.
+__device__ __forceinline__ Row doc_row(const Packed& p, const Doc& d, int r, int rw0, int rows, int hk) {
+  Row w;
+  static_cast<Seen&>(w) = seen_by(p, d, d.q0 + by_g(p, r));
+  w.f = seen_by(p, d, d.q0 + by_g(p, rw0));
+  w.l = seen_by(p, d, d.q0 + by_g(p, min(rw0 + 31, rows - 1)));
+  w.slope = p.slopes == nullptr ? 0.f : p.slopes[hk * p.G + mod_g(p, r)];
+  return w;
 }
 
 // 128 rows a block, four waves of 32, K and V tiles in a two-buffer LDS ring with
-// one barrier per tile.
+// one barrier per tile.  The plan's table of blocks of 128 tokens says where each
+// works, so that its set-up is two scalar loads deep (the entry, then its document's
+// offsets): a search among the documents took 2 us a block.
 constexpr int kRowsB = 128;
 template <bool BF16, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void packed_attn_rows(Packed p, Parts part,
@@ -345,50 +417,55 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void p
   __shared__ __attribute__((aligned(16))) uint16_t Vs[2][64 * 64];
   const int tid = threadIdx.x, lane = tid & 63, lg = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int Hk = p.H / p.G, hk = blockIdx.x % Hk;
-  const int64_t slot = blockIdx.x / Hk;
-  int64_t first;
-  const int b = slot_doc<kRowsB>(p, slot, lane, &first);
+  const int Hk = p.H / p.G;
+  int slot = blockIdx.x / Hk;
+  const int hk = blockIdx.x - slot * Hk;
+  if (p.causal) slot = (int)(gridDim.x / Hk) - 1 - slot;  // a document's last rows, which see the most, first
+  const int entry = by_g(p, slot), b = p.blocks[2 * entry];
+  if (b < 0) return;  // (the whole block, here and below)
   const Doc d = packed_doc(p, b);
-  const int64_t at = (slot - first) * kRowsB;
-  if (at >= (int64_t)d.nq * p.G) return;  // (the whole block)
-  const int rows = d.nq * p.G, r0 = (int)at, rw0 = r0 + 32 * wave;
-  const int r = rw0 + (lane & 31), rc = min(r, rows - 1);
+  const int t0 = min(max(p.blocks[2 * entry + 1], d.q0), d.q0 + d.nq), rows = min(d.q0 + d.nq - t0, kBlockTokens) * p.G;
+  const int r0 = mod_g(p, slot) * kRowsB, rw0 = r0 + 32 * wave;
+  if (r0 >= rows) return;
+  const int r = rw0 + (lane & 31), rc = min(r, rows - 1), t = t0 + by_g(p, rc);
   const Score sc = score_of(p, CAP, BIAS);
-  Row row = packed_row(p, d, rc, rw0, rows, hk);
-  row.slope *= kLog2e;
-  const int shift = d.nk - d.nq;
-  const Tiles ti = row_tiles<64>(p, d, r0 / p.G + shift, min(r0 + kRowsB - 1, rows - 1) / p.G + shift);
-  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits), i1 = (int)((int64_t)ti.n * (s + 1) / splits);
-  const uint16_t* Kb = (const uint16_t*)p.K + d.k0 * p.ks[0] + hk * p.ks[1];
-  const uint16_t* Vb = (const uint16_t*)p.V + d.k0 * p.vs[0] + hk * p.vs[1];
   Wave w;
-  wave_init(w, sc, (const uint16_t*)p.Q + (d.q0 + rc / p.G) * p.qs[0] + (hk * p.G + rc % p.G) * p.qs[1], lg);
+  wave_init(w, sc, (const uint16_t*)p.Q + t * p.qs[0] + (hk * p.G + mod_g(p, rc)) * p.qs[1], lg);
+  auto seen = [&](int q) { return seen_by(p, d, t0 + by_g(p, min(q, rows - 1))); };
+  const Tiles ti = tiles_of<64>(seen(r0), seen(r0 + kRowsB - 1));
+  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits), i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const uint16_t* Kb = (const uint16_t*)p.K + hk * p.ks[1];
+  const uint16_t* Vb = (const uint16_t*)p.V + hk * p.vs[1];
   auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
-    const int k0 = ti.at(i) * 64;
+    const int k0 = ti.at<64>(i);
 #pragma unroll
-    for (int q = 0; q < 2; q++) dma_piece(Vb, p.vs[0], k0, wave * 2 + q, d.nk, Vs[bf], lane);
+    for (int q = 0; q < 2; q++) dma_piece(Vb, p.vs[0], k0, wave * 2 + q, ti.bound, Vs[bf], lane);
 #pragma unroll
-    for (int q = 0; q < 2; q++) dma_piece(Kb, p.ks[0], k0, wave * 2 + q, d.nk, Ks[bf], lane);
+    for (int q = 0; q < 2; q++) dma_piece(Kb, p.ks[0], k0, wave * 2 + q, ti.bound, Ks[bf], lane);
   };
   if (i0 < i1) fetch(i0, 0);
+  Row row;
+  static_cast<Seen&>(row) = seen_by(p, d, t);
+  row.f = seen(rw0);
+  row.l = seen(rw0 + 31);
+  row.slope = p.slopes == nullptr ? 0.f : p.slopes[hk * p.G + mod_g(p, rc)] * kLog2e;
   const Frag32 f = frag32(lane);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  int bf = 0;
+  int at = 0;
   for (int i = i0; i < i1; i++) {
     // the next tile into the other buffer (free since the last barrier)
-    if (i + 1 < i1) fetch(i + 1, bf ^ 1);
-    const int k0 = ti.at(i) * 64, cl = rw0 < rows ? tile_class<64>(d, row, k0) : 0;
-    if (cl != 0) wave_tile<BF16, CAP, BIAS>(w, f, Ks[bf], Vs[bf], k0, d, row, cl == 2, sc, lg);
+    if (i + 1 < i1) fetch(i + 1, at ^ 1);
+    const int k0 = ti.at<64>(i), cl = rw0 < rows ? tile_class<64>(row, k0) : 0;
+    if (cl != 0) wave_tile<BF16, CAP, BIAS>(w, f, Ks[at], Vs[at], k0, row, cl == 2, sc, lg);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    bf ^= 1;
+    at ^= 1;
     __syncthreads();
   }
-  if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], d, row, ti, i0, i1, 1, sc, lg);
+  if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], row, ti, i0, i1, 1, sc, lg);
   const float lt = sum_xor32(w.l);
   if (r >= rows) return;
-  const int64_t ri = row_index(p, d, r, hk);
+  const int64_t ri = row_index(p, t, r, hk);
   if (splits > 1) {
     const int64_t pr = (int64_t)s * p.Tq * p.H + ri;
     if (lg == 0) part.ml[pr] = float2{w.m * sc.mul, lt};
@@ -424,32 +501,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void p
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hk = p.H / p.G, hk = blockIdx.x % Hk;
   const int64_t slot = blockIdx.x / Hk;
-  int64_t first;
-  const int b = slot_doc<kRowsF>(p, slot, lane, &first);
-  const Doc d = packed_doc(p, b);
-  const int64_t at = (slot - first) * kRowsF;
-  if (at >= (int64_t)d.nq * p.G) return;  // (the whole block)
-  const int rows = d.nq * p.G, r0 = (int)at, r = r0 + l32, rc = min(r, rows - 1);
+  Doc d;
+  int r0;
+  if (!slot_doc<kRowsF>(p, slot, lane, &d, &r0)) return;  // (the whole block)
+  const int rows = d.nq * p.G, r = r0 + l32, rc = min(r, rows - 1);
   const Score sc = score_of(p, CAP, BIAS);
-  Row row = packed_row(p, d, rc, r0, rows, hk);
+  Row row = doc_row(p, d, rc, r0, rows, hk);
   row.slope *= kLog2e;
-  const int shift = d.nk - d.nq;
-  const Tiles ti = row_tiles<64>(p, d, r0 / p.G + shift, min(r0 + kRowsF - 1, rows - 1) / p.G + shift);
+  const Tiles ti = tiles_of<64>(row.f, row.l);
   const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits) + wave, i1 = (int)((int64_t)ti.n * (s + 1) / splits);
-  const uint16_t* Kb = (const uint16_t*)p.K + d.k0 * p.ks[0] + hk * p.ks[1];
-  const uint16_t* Vb = (const uint16_t*)p.V + d.k0 * p.vs[0] + hk * p.vs[1];
+  const uint16_t* Kb = (const uint16_t*)p.K + hk * p.ks[1];
+  const uint16_t* Vb = (const uint16_t*)p.V + hk * p.vs[1];
   uint16_t* mine = ring + wave * (4 * 64 * 64);  // K, V, K, V
   auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
-    const int k0 = ti.at(i) * 64;
+    const int k0 = ti.at<64>(i);
     // this wave's reads of the tile that was there are done
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int q = 0; q < 8; q++) dma_piece(Kb, p.ks[0], k0, q, d.nk, mine + bf * 8192, lane);
+    for (int q = 0; q < 8; q++) dma_piece(Kb, p.ks[0], k0, q, ti.bound, mine + bf * 8192, lane);
 #pragma unroll
-    for (int q = 0; q < 8; q++) dma_piece(Vb, p.vs[0], k0, q, d.nk, mine + bf * 8192 + 4096, lane);
+    for (int q = 0; q < 8; q++) dma_piece(Vb, p.vs[0], k0, q, ti.bound, mine + bf * 8192 + 4096, lane);
   };
   Wave w;
-  wave_init(w, sc, (const uint16_t*)p.Q + (d.q0 + rc / p.G) * p.qs[0] + (hk * p.G + rc % p.G) * p.qs[1], lg);
+  wave_init(w, sc, (const uint16_t*)p.Q + (d.q0 + by_g(p, rc)) * p.qs[0] + (hk * p.G + mod_g(p, rc)) * p.qs[1], lg);
   const Frag32 f = frag32(lane);
   if (i0 < i1) fetch(i0, 0);
   int bf = 0;
@@ -460,12 +534,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void p
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    const int k0 = ti.at(i) * 64, cl = tile_class<64>(d, row, k0);
+    const int k0 = ti.at<64>(i), cl = tile_class<64>(row, k0);
     if (cl != 0)
-      wave_tile<BF16, CAP, BIAS>(w, f, mine + bf * 8192, mine + bf * 8192 + 4096, k0, d, row, cl == 2, sc, lg);
+      wave_tile<BF16, CAP, BIAS>(w, f, mine + bf * 8192, mine + bf * 8192 + 4096, k0, row, cl == 2, sc, lg);
     bf ^= 1;
   }
-  if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], d, row, ti, i0, i1, 4, sc, lg);
+  if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], row, ti, i0, i1, 4, sc, lg);
   // join the waves: weights 2^(m_w - max); wave w finishes registers [8 w, 8 w + 8)
   // of the 32
   const float lw = sum_xor32(w.l);
@@ -492,7 +566,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void p
   }
   if (r >= rows) return;
   const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-  const int64_t ri = row_index(p, d, r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
+  const int64_t ri = row_index(p, d.q0 + by_g(p, r), r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
   if (splits > 1 && wave == 0 && lg == 0) part.ml[pr] = float2{mt, lt};
 #pragma unroll
   for (int h = 0; h < 2; h++) {
@@ -534,36 +608,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hk = p.H / p.G, hk = blockIdx.x % Hk;
   const int64_t slot = blockIdx.x / Hk;
-  int64_t first;
-  const int b = slot_doc<kRows32>(p, slot, lane, &first);
-  const Doc d = packed_doc(p, b);
-  const int64_t at = (slot - first) * kRows32;
-  if (at >= (int64_t)d.nq * p.G) return;  // (the whole block)
-  const int rows = d.nq * p.G, r0 = (int)at, r = r0 + l32, rc = min(r, rows - 1);
-  const Row row = packed_row(p, d, rc, r0, rows, hk);
-  const int shift = d.nk - d.nq;
-  const Tiles ti = row_tiles<kKeys32>(p, d, r0 / p.G + shift, min(r0 + kRows32 - 1, rows - 1) / p.G + shift);
+  Doc d;
+  int r0;
+  if (!slot_doc<kRows32>(p, slot, lane, &d, &r0)) return;  // (the whole block)
+  const int rows = d.nq * p.G, r = r0 + l32, rc = min(r, rows - 1);
+  const Row row = doc_row(p, d, rc, r0, rows, hk);
+  const Tiles ti = tiles_of<kKeys32>(row.f, row.l);
   const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits) + wave, i1 = (int)((int64_t)ti.n * (s + 1) / splits);
-  const float* Kb = (const float*)p.K + d.k0 * p.ks[0] + hk * p.ks[1];
-  const float* Vb = (const float*)p.V + d.k0 * p.vs[0] + hk * p.vs[1];
+  const float* Kb = (const float*)p.K + hk * p.ks[1];
+  const float* Vb = (const float*)p.V + hk * p.vs[1];
 
   // element e of qf[i] is column 8 i + 4 lg + e, the columns its half supplies to
   // MFMA steps e of chunk pair i
   float4v qf[8];
   {
-    const float* qp = (const float*)p.Q + (d.q0 + rc / p.G) * p.qs[0] + (hk * p.G + rc % p.G) * p.qs[1] + 4 * lg;
+    const float* qp = (const float*)p.Q + (d.q0 + by_g(p, rc)) * p.qs[0] + (hk * p.G + mod_g(p, rc)) * p.qs[1] + 4 * lg;
 #pragma unroll
     for (int i = 0; i < 8; i++) qf[i] = *(const float4v*)(qp + 8 * i);
   }
   // K tile: 8 lanes a row, chunk c of row r at c ^ (r & 15): a 16-lane pass of the
   // fragment reads (16 rows, one chunk) covers all 64 banks.  Keys past the
-  // document repeat its last one: their scores are hidden.
+  // rows' last one repeat it: their scores are hidden.
   const int kr = lane >> 3, c8 = lane & 7;
   float4v klo[4], khi[4];
   auto load_k = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float* kp = Kb + min(k0 + i * 8 + kr, d.nk - 1) * p.ks[0] + 4 * c8;
+      const float* kp = Kb + min(k0 + i * 8 + kr, ti.bound - 1) * p.ks[0] + 4 * c8;
       klo[i] = *(const float4v*)kp;
       khi[i] = *(const float4v*)(kp + 32);
     }
@@ -576,9 +647,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
 #pragma unroll
     for (int i = 0; i < 16; i++) o[e][i] = 0.f;
   float m = -INFINITY, l = 0.f;
-  if (i0 < i1) load_k(ti.at(i0) * kKeys32);
+  if (i0 < i1) load_k(ti.at<kKeys32>(i0));
   for (int i = i0; i < i1; i += 4) {
-    const int k0 = ti.at(i) * kKeys32, cl = tile_class<kKeys32>(d, row, k0);
+    const int k0 = ti.at<kKeys32>(i), cl = tile_class<kKeys32>(row, k0);
 #pragma unroll
     for (int q = 0; q < 4; q++) {
       *(float4v*)(kb + kslot(q * 8 + kr, c8)) = klo[q];
@@ -592,11 +663,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     float v[2][16];
 #pragma unroll
     for (int q = 0; q < 16; q++) {
-      const float* vp = Vb + min(k0 + 8 * (q >> 2) + 4 * lg + (q & 3), d.nk - 1) * p.vs[0] + l32;
+      const float* vp = Vb + min(k0 + 8 * (q >> 2) + 4 * lg + (q & 3), ti.bound - 1) * p.vs[0] + l32;
       v[0][q] = vp[0];
       v[1][q] = vp[32];
     }
-    if (i + 4 < i1) load_k(ti.at(i + 4) * kKeys32);
+    if (i + 4 < i1) load_k(ti.at<kKeys32>(i + 4));
     float16v st;
 #pragma unroll
     for (int q = 0; q < 16; q++) st[q] = 0.f;
@@ -610,13 +681,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     float mx = -INFINITY;
+    const uint32_t seen = cl != 1 ? seen_bits(row, k0) >> (4 * lg) : ~0u;
 #pragma unroll
     for (int q = 0; q < 16; q++) {
       const int key = k0 + 8 * (q >> 2) + 4 * lg + (q & 3);
       float x = st[q] * p.scale;
       if constexpr (CAP) x = p.cap * tanhf(x / p.cap);
       if constexpr (BIAS) x = fmaf(-row.slope, fabsf((float)(row.pos - key)), x);
-      if (cl != 1) x = key_seen(d, row, key) ? x : -INFINITY;
+      if (cl != 1) x = seen_or(seen, 8 * (q >> 2) + (q & 3), x);
       st[q] = x;
       mx = fmaxf(mx, x);
     }
@@ -690,7 +762,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   }
   if (r >= rows) return;
   const float inv = splits > 1 ? 1.f : lt == 0.f ? 0.f : 1.0f / lt;
-  const int64_t ri = row_index(p, d, r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
+  const int64_t ri = row_index(p, d.q0 + by_g(p, r), r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
   if (splits > 1 && wave == 0 && lg == 0) part.ml[pr] = float2{mt, lt};
   float* op = splits > 1 ? part.o + pr * 64 : (float*)p.O + ri * 64;
 #pragma unroll
@@ -738,34 +810,27 @@ __global__ __launch_bounds__(64) void packed_attn_any(Packed p, int dt) {
   extern __shared__ float sh[];  // [D] query, [64] weights
   float* w = sh + p.D;
   const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, D = p.D;
-  int b = 0, e = p.B + 1;  // the last document that begins at or before t
-  while (e - b > 1) {
-    const int m = (b + e) >> 1;
-    if (p.qoff[m] <= t) b = m;
-    else e = m;
-  }
-  const Doc d = packed_doc(p, b);
-  const int pos = t - d.q0 + d.nk - d.nq;
-  int lo, hi;
-  packed_range(p, d.nk, pos, &lo, &hi);
+  const uint32_t b = (uint32_t)p.doc[t];
+  const Seen d = seen_by(p, packed_doc(p, b < (uint32_t)p.B ? (int)b : p.B), t);
   for (int c = lane; c < D; c += 64) sh[c] = load_f(p.Q, t * p.qs[0] + h * p.qs[1] + c * p.qs[2], dt);
   __syncthreads();
   const float slope = p.slopes == nullptr ? 0.f : p.slopes[h];
   float o[kAnyCols] = {}, m = -INFINITY, l = 0.f;
   const int64_t kh = (h / p.G) * p.ks[1], vh = (h / p.G) * p.vs[1];
-  for (int j0 = 0; j0 < d.nk; j0 += 64) {
+  const int bound = max(d.end, d.pend);
+  for (int j0 = d.p0; j0 < bound; j0 += 64) {
     // (the same in every lane: nothing of these keys is visible)
-    if (j0 >= d.prefix && (j0 > hi || j0 + 63 < lo)) continue;
+    if (j0 >= d.pend && (j0 >= d.end || j0 + 64 <= d.lo)) continue;
     const int j = j0 + lane;
-    const bool seen = j < d.nk && (j < d.prefix || (j >= lo && j <= hi));
+    const bool seen = j < d.pend || (j >= d.lo && j < d.end);
     float x = -INFINITY;
     if (seen) {
-      const int64_t row = (int64_t)(d.k0 + j) * p.ks[0] + kh;
+      const int64_t row = (int64_t)j * p.ks[0] + kh;
       float a = 0.f;
       for (int c = 0; c < D; c++) a = fmaf(sh[c], load_f(p.K, row + c * p.ks[2], dt), a);
       x = a * p.scale;
       if (p.cap > 0.f) x = p.cap * tanhf(x / p.cap);
-      x -= slope * fabsf((float)(pos - j));
+      x -= slope * fabsf((float)(d.pos - j));
     }
     const float mn = fmaxf(m, wave_max(x));
     const float mc = mn == -INFINITY ? 0.f : mn, alpha = expf(m - mc);
@@ -778,8 +843,8 @@ __global__ __launch_bounds__(64) void packed_attn_any(Packed p, int dt) {
     for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++) {
       float a = o[i] * alpha;
       const int64_t col = vh + (i * 64 + lane) * p.vs[2];
-      for (int k = 0; k < 64 && j0 + k < d.nk; k++)
-        if (w[k] != 0.f) a = fmaf(w[k], load_f(p.V, (int64_t)(d.k0 + j0 + k) * p.vs[0] + col, dt), a);
+      for (int k = 0; k < 64 && j0 + k < bound; k++)
+        if (w[k] != 0.f) a = fmaf(w[k], load_f(p.V, (int64_t)(j0 + k) * p.vs[0] + col, dt), a);
       o[i] = a;
     }
   }
@@ -806,13 +871,13 @@ static void packed_any(uintptr_t ctx, int dt, const Packed& p) {
 }
 
 template <class K>
-static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, int lds, int rows, const Packed& p, int splits,
-                          const Parts& part) {
+static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, int lds, int64_t blocks, const Packed& p,
+                          int splits, const Parts& part) {
   if (lds > 64 * 1024)
     once_per_device(attr, [&] {
       HB_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     });
-  const int64_t grid = ((int64_t)p.Tq * p.G / rows + p.B + 1) * (p.H / p.G);
+  const int64_t grid = blocks * (p.H / p.G);
   HB_REQUIRE(grid < (1ll << 31), "hb_sdpa_packed: too many rows and heads");
   kern<<<dim3((unsigned)grid, (unsigned)splits), 256, (size_t)lds, stream_of(ctx)>>>(p, part, splits);
 }
@@ -838,16 +903,18 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
       splits = 1;  // no memory for the parts: unsplit
     }
   }
+  static_assert(kRowsF == kRows32, "slots of both");
+  const int64_t slots = rows / kRowsF + p.B + 1;  // enough for every document's last, partly filled block
   auto go = [&](auto cap, auto bias) {
     constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
     auto half = [&](auto bf) {
       constexpr bool BF = decltype(bf)::value;
       static std::atomic<uint64_t> attr{0};
-      if (few) packed_launch(ctx, packed_attn_few<BF, CAP, BIAS>, attr, kFewLds, kRowsF, p, splits, part);
-      else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, kRowsB, p, splits, part);
+      if (few) packed_launch(ctx, packed_attn_few<BF, CAP, BIAS>, attr, kFewLds, slots, p, splits, part);
+      else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, (int64_t)p.nblocks * p.G, p, splits, part);
     };
     std::atomic<uint64_t> none{0};
-    if (f32) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, none, 0, kRows32, p, splits, part);
+    if (f32) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, none, 0, slots, p, splits, part);
     else if (dt == HB_BF16) half(std::true_type{});
     else half(std::false_type{});
   };
@@ -869,8 +936,8 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
 using namespace hb;
 
 extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t* qs, uintptr_t k, const int64_t* ks,
-                              uintptr_t v, const int64_t* vs, uintptr_t o, uintptr_t q_offsets, uintptr_t k_offsets,
-                              int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale,
+                              uintptr_t v, const int64_t* vs, uintptr_t o, uintptr_t q_doc, uintptr_t q_blocks,
+                              uintptr_t q_offsets, uintptr_t k_offsets, int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D, float scale,
                               int causal, int64_t window, uintptr_t prefix, float cap, uintptr_t slopes) {
   HB_API_BEGIN
   HB_REQUIRE(dt == HB_F32 || dt == HB_F16 || dt == HB_BF16, "hb_sdpa_packed: dtype must be f32, f16 or bf16");
@@ -882,7 +949,7 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   HB_REQUIRE(std::isfinite(scale) && std::isfinite(cap) && cap >= 0.f, "hb_sdpa_packed: scale and cap must be finite");
   HB_REQUIRE(window >= -1, "hb_sdpa_packed: a window is not negative (-1: none)");
   if (Tq == 0) return 0;
-  HB_REQUIRE(q && o && q_offsets && k_offsets && (Tk == 0 || (k && v)), "hb_sdpa_packed: null argument");
+  HB_REQUIRE(q && o && q_doc && q_blocks && q_offsets && k_offsets && (Tk == 0 || (k && v)), "hb_sdpa_packed: null argument");
   Packed p;
   p.Q = (const void*)q;
   p.K = (const void*)k;
@@ -893,6 +960,9 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
     p.ks[i] = ks[i];
     p.vs[i] = vs[i];
   }
+  p.doc = (const int32_t*)q_doc;
+  p.blocks = (const int32_t*)q_blocks;
+  p.nblocks = (int)plan_blocks(B, Tq);
   p.qoff = (const int32_t*)q_offsets;
   p.koff = (const int32_t*)k_offsets;
   p.prefix = (const int32_t*)prefix;

@@ -515,15 +515,16 @@ class PackedDocs:
     """The plan of a packed batch (HipBackend.packDocs): `offsets` i32 [count +
     1], `doc` and `pos` i32 [total] (each row's document, -1 behind the last one,
     and its position there) and, with a padded length, `slots` i32 [total] (its
-    row in the padded [count, padded] batch, -1 behind the last document)."""
+    row in the padded [count, padded] batch, -1 behind the last document).  `blocks`
+    i32 [total // 128 + count + 1, 2] is where sdpaPacked's blocks work."""
 
-    def __init__(self, be: "HipBackend", count: int, total: int, padded: int, offsets, doc, pos, slots):
+    def __init__(self, be: "HipBackend", count: int, total: int, padded: int, offsets, blocks, doc, pos, slots):
         self._be = be
         self.count, self.total, self.padded = count, total, padded
-        self.offsets, self.doc, self.pos, self.slots = offsets, doc, pos, slots
+        self.offsets, self.blocks, self.doc, self.pos, self.slots = offsets, blocks, doc, pos, slots
 
     def dispose(self) -> None:
-        for t in (self.offsets, self.doc, self.pos, self.slots):
+        for t in (self.offsets, self.blocks, self.doc, self.pos, self.slots):
             self._be.dispose(t)
 
 
@@ -1822,17 +1823,19 @@ class HipBackend:
             raise ValueError(f"packDocs: bad sizes (total {total}, padded {padded}, {count} documents)")
         tmp: list = []
         n = self._plain(lengths, "i32", tmp)
-        # one block: offsets, then the rows' arrays, each on a 256-byte boundary
-        at, step = (count + 64) // 64 * 64, (total + 63) // 64 * 64
+        # one block: offsets, the table, then the rows' arrays, each on a 256-byte boundary
+        nb = total // 128 + count + 1
+        tab, step = (count + 64) // 64 * 64, (total + 63) // 64 * 64
+        at = tab + (2 * nb + 63) // 64 * 64
         st = self._malloc(4 * (at + step * (3 if padded else 2)))
-        parts = [HipTensor((count + 1,), "i32", st)]
+        parts = [HipTensor((count + 1,), "i32", st), HipTensor((nb, 2), "i32", st.retain(), tab)]
         for i in range(3 if padded else 2):
             parts.append(HipTensor((total,), "i32", st.retain(), at + i * step))
         for t in parts:
             self._track(t)
         p = st.ptr + 4 * at
         self._call("packDocs", "hb_pack_plan", self.ctx, self._ptr(n), count, total, padded, st.ptr, p, p + 4 * step,
-                   p + 8 * step if padded else 0)
+                   p + 8 * step if padded else 0, st.ptr + 4 * tab)
         for t in tmp:
             self.dispose(t)
         return PackedDocs(self, count, total, padded, *parts, *([] if padded else [None]))
@@ -1920,7 +1923,7 @@ class HipBackend:
         keys = docs if keys is None else keys
         self._plan(docs, "sdpaPacked")
         self._plan(keys, "sdpaPacked")
-        self._live(q, k, v, prefix, slopes, docs.offsets, keys.offsets, op="sdpaPacked")
+        self._live(q, k, v, prefix, slopes, docs.doc, docs.blocks, docs.offsets, keys.offsets, op="sdpaPacked")
         if len(q.shape) != 3 or len(k.shape) != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
             raise ValueError(f"sdpaPacked: q {list(q.shape)} k {list(k.shape)} v {list(v.shape)}")
         (T, H, D), (Tk, Hk, _) = q.shape, k.shape
@@ -1958,7 +1961,8 @@ class HipBackend:
             self.stats["sdpa"] += 1
             self._call("sdpaPacked", "hb_sdpa_packed", self.ctx, DT[dt][0], self._ptr(q), F.i64s(q._strides),
                        self._ptr(k), F.i64s(k._strides), self._ptr(v), F.i64s(v._strides), out._st.ptr,
-                       self._ptr(docs.offsets), self._ptr(keys.offsets), docs.count, T, Tk, H, Hk, D, float(scale),
+                       self._ptr(docs.doc), self._ptr(docs.blocks), self._ptr(docs.offsets), self._ptr(keys.offsets),
+                       docs.count, T, Tk, H, Hk, D, float(scale),
                        1 if causal else 0, -1 if window is None else int(window),
                        0 if prefix is None else self._ptr(prefix), float(cap or 0.0),
                        0 if slopes is None else self._ptr(slopes))

@@ -80,11 +80,11 @@ SYMBOLS: dict[str, tuple] = {
     "hb_reduce": (I, [U, I, I, U, I64, I64, I64, I, U]),
     "hb_scan": (I, [U, I, I, U, I64, I64, I64, I, U]),
     "hb_meanpool": (I, [U, I, U, U, I64, I64, I64, U]),
-    "hb_pack_plan": (I, [U, U, I64, I64, I64, U, U, U, U]),
+    "hb_pack_plan": (I, [U, U, I64, I64, I64, U, U, U, U, U]),
     "hb_pack_rows": (I, [U, U, I64, I64, U, I64, U]),
     "hb_unpack_rows": (I, [U, U, I64, I64, U, I64, I64, U]),
     "hb_rope_at": (I, [U, I, U, PI64, U, I64, I64, I64, U, I64, PI64, D]),
-    "hb_sdpa_packed": (I, [U, I, U, PI64, U, PI64, U, PI64, U, U, U, I64, I64, I64, I64, I64, I64, F, I, I64, U, F, U]),
+    "hb_sdpa_packed": (I, [U, I, U, PI64, U, PI64, U, PI64, U, U, U, U, U, I64, I64, I64, I64, I64, I64, F, I, I64, U, F, U]),
     "hb_lora_linear": (I, [U, I, U, I64, U, U, U, I64, I64, I64, I64, U, U, U, I64, I64, U]),
     "hb_lora_qlinear": (I, [U, I, U, I64, U, U, U, U, U, I64, I64, I64, I64, I, I, I, U, U, U, I64, I64, U]),
 }

@@ -19,6 +19,14 @@ def plan(lengths, total, padded=0):
     return off, doc, pos, np.where(doc < 0, -1, doc * padded + pos)
 
 
+def blocks(off, total):
+    """Blocks of up to 128 rows: (document, first row), rows behind the last as
+    document B, (-1, 0) to the end of the table."""
+    B, end = len(off) - 1, off[-1]
+    got = [(b, t) for b in range(B) for t in range(off[b], off[b + 1], 128)] + [(B, t) for t in range(end, total, 128)]
+    return np.array(got + [(-1, 0)] * (total // 128 + B + 1 - len(got)))
+
+
 def angles(positions, D, base, sections):
     """cos and sin [T, D / 2] by the contract's f32 angle rule."""
     half = D // 2

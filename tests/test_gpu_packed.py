@@ -53,6 +53,7 @@ def test_plan(b, lengths, total, padded):
     np.testing.assert_array_equal(ints(b, p.offsets), off)
     np.testing.assert_array_equal(ints(b, p.doc), doc)
     np.testing.assert_array_equal(ints(b, p.pos), pos)
+    np.testing.assert_array_equal(ints(b, p.blocks), ref.blocks(off, total))
     if padded:
         np.testing.assert_array_equal(ints(b, p.slots), slots)
     else:

@@ -135,11 +135,12 @@ def test_entry_points_refuse_before_they_touch_a_context():
             n.call("op", name, 0, *args)
     three, two = F.i64s([64, 64, 1]), F.i64s([16, 16])
     P = 1 << 20
-    refuses("hb_pack_plan", "bad sizes", P, -1, 4, 0, P, P, P, 0)
-    refuses("hb_pack_plan", "bad sizes", P, 1, 1 << 30, 0, P, P, P, 0)
-    refuses("hb_pack_plan", "null argument", 0, 1, 4, 0, P, P, P, 0)
-    refuses("hb_pack_plan", "null argument", P, 1, 4, 0, P, 0, P, 0)
-    refuses("hb_pack_plan", "slots need", P, 1, 4, 0, P, P, P, P)
+    refuses("hb_pack_plan", "bad sizes", P, -1, 4, 0, P, P, P, 0, P)
+    refuses("hb_pack_plan", "bad sizes", P, 1, 1 << 30, 0, P, P, P, 0, P)
+    refuses("hb_pack_plan", "null argument", 0, 1, 4, 0, P, P, P, 0, P)
+    refuses("hb_pack_plan", "null argument", P, 1, 4, 0, P, 0, P, 0, P)
+    refuses("hb_pack_plan", "null argument", P, 1, 4, 0, P, P, P, 0, 0)
+    refuses("hb_pack_plan", "slots need", P, 1, 4, 0, P, P, P, P, P)
     refuses("hb_pack_rows", "bad sizes", P, -1, 4, P, 3, P)
     refuses("hb_pack_rows", "null argument", P, 1, 4, 0, 3, P)
     refuses("hb_unpack_rows", "bad sizes", P, 3, 4, P, 1 << 20, 1 << 20, P)
@@ -155,7 +156,7 @@ def test_entry_points_refuse_before_they_touch_a_context():
     refuses("hb_rope_at", "base", *rope(base=0.0))
 
     def attn(dt=F.HB_F16, q=P, B=1, Tq=4, Tk=4, H=2, Hk=1, D=64, scale=1.0, window=-1, cap=0.0):
-        return (dt, q, three, P, three, P, three, P, P, P, B, Tq, Tk, H, Hk, D, scale, 0, window, 0, cap, 0)
+        return (dt, q, three, P, three, P, three, P, P, P, P, P, B, Tq, Tk, H, Hk, D, scale, 0, window, 0, cap, 0)
     for match, bad in (("dtype", dict(dt=F.HB_U8)), ("bad sizes", dict(B=-1)), ("bad sizes", dict(Tk=1 << 30)),
                        ("multiple", dict(H=3, Hk=2)), ("multiple", dict(Hk=0)), ("head dimension", dict(D=513)),
                        ("finite", dict(scale=float("nan"))), ("finite", dict(cap=-1.0)), ("window", dict(window=-2)),
@@ -187,4 +188,4 @@ def test_bank_from_a_scope_outlives_it():
     bank = b.scope(lambda: b.loraBank(b.t(2, 4, 8), b.t(2, 6, 4)))
     assert not (bank.a._dead or bank.b._dead or bank.scales._dead)
     docs = b.scope(lambda: b.packDocs(b.fromHost(HostTensor("i32", (2,), np.zeros(2, np.int32))), 4, 2))
-    assert not any(t._dead for t in (docs.offsets, docs.doc, docs.pos, docs.slots))
+    assert not any(t._dead for t in (docs.offsets, docs.blocks, docs.doc, docs.pos, docs.slots))
