@@ -37,6 +37,15 @@
 
 namespace hb {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Scores to base 2 (the 16-bit kernels).
+struct Score {
+  float mul, c1, c2;  // mul: the factor left once a cap or slope has been applied (1), else of the products
+  float poly[5], near;  // coefficients of the capped score, and the products they hold for
+  uint32_t flip;      // a negative scale turns the query round instead
+};
+
 struct Packed {
   const void *Q, *K, *V;
   void* O;                 // [Tq, H, D]
@@ -50,6 +59,7 @@ struct Packed {
   int B, Tq, Tk, H, G, D;  // G: query heads of a key head
   int causal, half;        // half < 0: no window
   float scale, cap;        // cap <= 0: none
+  Score sc;
 };
 
 // A document's queries [q0, q0 + nq) and keys [k0, k0 + nk); document B stands
@@ -188,15 +198,14 @@ __device__ __forceinline__ float seen_or(uint32_t seen, int bit, float x) {
 }
 
 // Parts of a split run: per split and row (token * H + head) the unscaled output,
-// its maximum score and its sum of weights.
+// the score its weights are relative to and their sum.
 struct Parts {
   float* o;    // [splits][rows][64]
   float2* ml;  // [splits][rows]
+  int tiles;   // of a split; the last one takes what is left
 };
 
 // ------------------------------------------------------------------ f16 / bf16 (D = 64)
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 // A wave's 32 rows (lane l holds row l % 32; the halves split its columns and its
 // keys).  Scores are in base 2 once `mul` is applied: mul is 1 where a cap or a
@@ -206,26 +215,41 @@ struct Wave {
   float16v o[2];  // columns 32 d + 8 (r / 4) + 4 lg + r % 4
   float m, l;     // running maximum (before mul), the lane's sum of weights
 };
-struct Score {
-  float mul, c1, c2;  // capped: c2 tanh, computed as c2 - 2 c2 / (1 + 2^(c1 score))
-  uint32_t flip;      // a negative scale turns the query round instead
-};
-__device__ __forceinline__ Score score_of(const Packed& p, bool cap, bool bias) {
-  Score s;
-  // (scale 0: any tiny factor; 0 * -inf would not be a maximum)
-  const float sl = fmaxf(fabsf(p.scale), 1e-30f) * kLog2e;
-  s.mul = cap || bias ? 1.f : sl;
-  s.c1 = cap ? 2.f * sl / p.cap : sl;
-  s.c2 = p.cap * kLog2e;
-  s.flip = p.scale < 0.f ? 0x80008000u : 0u;
-  return s;
-}
+// A capped score c2 tanh(c1 x / 2) is c2 - 2 c2 / (1 + 2^(c1 x)) anywhere (c1 in base
+// 2), and where every score of a tile is within 0.75 cap, the odd polynomial of
+// degree 9 through tanh's Chebyshev points there, off by 3.6e-7 at most: 6
+// instructions instead of an exponential and a reciprocal at a quarter of the rate
+// (chunks of 1000 queries over up to 8192 keys: 164 -> POLY us).
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ float score(const Score& s, float slope, int pos, int key, float x) {
   if constexpr (CAP) x = fmaf(-2.f * s.c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * s.c1)), s.c2);
   else if constexpr (BIAS) x *= s.c1;
   if constexpr (BIAS) x = fmaf(-slope, fabsf((float)(pos - key)), x);
   return x;
+}
+__device__ __forceinline__ float capped_near(const Score& s, float x) {
+  const float u = x * x;
+  float r = fmaf(u, s.poly[4], s.poly[3]);
+#pragma unroll
+  for (int i = 2; i >= 0; i--) r = fmaf(u, r, s.poly[i]);
+  return x * r;
+}
+static Score score_of(float scale, float cap, bool bias) {
+  Score s{};
+  // (scale 0: any tiny factor; 0 * -inf would not be a maximum)
+  const float sl = fmaxf(fabsf(scale), 1e-30f);
+  const bool capped = cap > 0.f;
+  s.mul = capped || bias ? 1.f : sl * kLog2e;
+  s.c1 = capped ? 2.f * sl / cap * kLog2e : sl * kLog2e;
+  s.c2 = cap * kLog2e;
+  s.flip = scale < 0.f ? 0x80008000u : 0u;
+  // tanh(y) / y in y^2 on [0, 0.75^2]
+  const double c[5] = {0.99999942, -0.33328192, 0.13258462, -0.05004161, 0.01291665};
+  const double g = capped ? (double)sl / cap : 0.0;
+  double f = (double)s.c2 * g;
+  for (int i = 0; i < 5; i++, f *= g * g) s.poly[i] = (float)(f * c[i]);
+  s.near = capped ? (float)(0.75 / g) : 0.f;
+  return s;
 }
 
 __device__ __forceinline__ void wave_init(Wave& w, const Score& sc, const uint16_t* qrow, int lg) {
@@ -255,13 +279,9 @@ __device__ __forceinline__ float add_pair(uint32_t p, float sum) {
   }
 }
 
-// One tile of 64 keys in LDS: scores, mask (`mixed`), online softmax, O += P V.
-// Weights are rounded to the 16-bit type for the second product, as MFMA takes
-// them, and their sum is of the rounded ones (one dot product a pair).
-template <bool BF16, bool CAP, bool BIAS>
-__device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16_t* Kc, const uint16_t* Vc, int k0,
-                                          const Row& row, bool mixed, const Score& sc, int lg) {
-  float16v st[2];
+// One tile of 64 keys in LDS, in three parts: the products of queries and keys,
+template <bool BF16>
+__device__ __forceinline__ void wave_products(const Wave& w, const Frag32& f, const uint16_t* Kc, float16v (&st)[2]) {
 #pragma unroll
   for (int kb = 0; kb < 2; kb++) {
     uint4v kf[4];
@@ -272,12 +292,52 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
 #pragma unroll
     for (int s = 0; s < 4; s++) st[kb] = mfma32x16<BF16>(kf[s], w.qf[s], st[kb]);
   }
-  if constexpr (CAP || BIAS) {
+}
+__device__ __forceinline__ float max_of(const float16v (&st)[2]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[kb][r]);
+  return mx;
+}
+// their weights (cap, slope, mask if `mixed`, online softmax).  Weights are rounded
+// to the 16-bit type for the second product, as MFMA takes them, and their sum is of
+// the rounded ones (one dot product a pair),
+template <bool BF16, bool CAP, bool BIAS>
+__device__ __forceinline__ void wave_weights(Wave& w, float16v (&st)[2], int k0, const Row& row, bool mixed,
+                                             const Score& sc, int lg, uint4v (&pf)[4]) {
+  float mx = -INFINITY;
+  if constexpr (CAP) {
+    mx = max_of(st);
+    float mn = INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-      for (int r = 0; r < 16; r++)
-        st[kb][r] = score<CAP, BIAS>(sc, row.slope, row.pos, k0 + 32 * kb + 8 * (r >> 2) + 4 * lg + (r & 3), st[kb][r]);
+      for (int r = 0; r < 16; r++) mn = fminf(mn, st[kb][r]);
+    if (__all(mx <= sc.near && mn >= -sc.near)) {
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) st[kb][r] = capped_near(sc, st[kb][r]);
+      mx = capped_near(sc, mx);  // (the maximum's own value: the cap keeps the order)
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) st[kb][r] = score<true, false>(sc, 0.f, 0, 0, st[kb][r]);
+      mx = score<true, false>(sc, 0.f, 0, 0, mx);
+    }
+  }
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * lg + (r & 3);
+        const float x = CAP ? st[kb][r] : st[kb][r] * sc.c1;
+        st[kb][r] = fmaf(-row.slope, fabsf((float)(row.pos - key)), x);
+      }
   }
   if (mixed) {
 #pragma unroll
@@ -287,11 +347,7 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
       for (int r = 0; r < 16; r++) st[kb][r] = seen_or(seen, 8 * (r >> 2) + (r & 3), st[kb][r]);
     }
   }
-  float mx = -INFINITY;
-#pragma unroll
-  for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[kb][r]);
+  if (!CAP || BIAS || mixed) mx = max_of(st);
   mx = max_xor32(mx);
   // Weights are relative to w.m, which follows the maximum once it is left behind by
   // a factor of 2^8 for some row of the wave: up to there they fit the 16-bit types
@@ -307,7 +363,6 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
       for (int r = 0; r < 16; r++) w.o[e][r] *= alpha;
   }
   const float mc = w.m == -INFINITY ? 0.f : w.m * sc.mul;
-  uint4v pf[4];
 #pragma unroll
   for (int t = 0; t < 4; t++) {
     uint32_t pk[4];
@@ -320,6 +375,10 @@ __device__ __forceinline__ void wave_tile(Wave& w, const Frag32& f, const uint16
     }
     pf[t] = uint4v{pk[0], pk[1], pk[2], pk[3]};
   }
+}
+// and O += weights . V.
+template <bool BF16>
+__device__ __forceinline__ void wave_values(Wave& w, const Frag32& f, const uint16_t* Vc, const uint4v (&pf)[4]) {
 #pragma unroll
   for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -428,12 +487,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void p
   const int r0 = mod_g(p, slot) * kRowsB, rw0 = r0 + 32 * wave;
   if (r0 >= rows) return;
   const int r = rw0 + (lane & 31), rc = min(r, rows - 1), t = t0 + by_g(p, rc);
-  const Score sc = score_of(p, CAP, BIAS);
+  const Score& sc = p.sc;
   Wave w;
   wave_init(w, sc, (const uint16_t*)p.Q + t * p.qs[0] + (hk * p.G + mod_g(p, rc)) * p.qs[1], lg);
   auto seen = [&](int q) { return seen_by(p, d, t0 + by_g(p, min(q, rows - 1))); };
   const Tiles ti = tiles_of<64>(seen(r0), seen(r0 + kRowsB - 1));
-  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits), i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const int s = blockIdx.y, i0 = min(s * part.tiles, ti.n), i1 = s + 1 < splits ? min(i0 + part.tiles, ti.n) : ti.n;
+  if (splits > 1 && i0 >= i1) {  // nothing left for this split
+    if (r < rows && lg == 0) part.ml[(int64_t)s * p.Tq * p.H + row_index(p, t, r, hk)] = float2{-INFINITY, 0.f};
+    return;
+  }
   const uint16_t* Kb = (const uint16_t*)p.K + hk * p.ks[1];
   const uint16_t* Vb = (const uint16_t*)p.V + hk * p.vs[1];
   auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
@@ -457,7 +520,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void p
     // the next tile into the other buffer (free since the last barrier)
     if (i + 1 < i1) fetch(i + 1, at ^ 1);
     const int k0 = ti.at<64>(i), cl = rw0 < rows ? tile_class<64>(row, k0) : 0;
-    if (cl != 0) wave_tile<BF16, CAP, BIAS>(w, f, Ks[at], Vs[at], k0, row, cl == 2, sc, lg);
+    if (cl != 0) {
+      float16v st[2];
+      uint4v pf[4];
+      wave_products<BF16>(w, f, Ks[at], st);
+      wave_weights<BF16, CAP, BIAS>(w, st, k0, row, cl == 2, sc, lg, pf);
+      wave_values<BF16>(w, f, Vs[at], pf);
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     at ^= 1;
     __syncthreads();
@@ -488,12 +557,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void p
 }
 
 // 32 rows a block, for few queries a document: the block's four waves hold the
-// same rows and take its tiles in turn, each through an LDS ring of its own with
-// no barrier, so the block has 64 KB of keys and values on their way; then the
-// waves' parts are joined.  Bound by reading K and V once.
-constexpr int kRowsF = 32, kFewLds = 4 * 2 * 2 * 64 * 64 * 2;  // four rings of two K and V tiles
+// same rows and take its tiles in turn, each through a K and a V tile of its own in
+// LDS with no barrier; a tile's K is requested once the last one's products are
+// made, its V once that one's values are, so a wave has 8 to 16 KB on their way
+// whatever it does, and two blocks share a CU.  Then the waves' parts are joined.
+// Bound by reading K and V once.
+constexpr int kRowsF = 32, kFewLds = 4 * 2 * 64 * 64 * 2;
 template <bool BF16, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void packed_attn_few(Packed p, Parts part,
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void packed_attn_few(Packed p, Parts part,
                                                                                                int splits) {
   extern __shared__ __attribute__((aligned(16))) uint16_t ring[];
   __shared__ float part_m[4][kRowsF], part_l[4][kRowsF];
@@ -505,39 +576,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void p
   int r0;
   if (!slot_doc<kRowsF>(p, slot, lane, &d, &r0)) return;  // (the whole block)
   const int rows = d.nq * p.G, r = r0 + l32, rc = min(r, rows - 1);
-  const Score sc = score_of(p, CAP, BIAS);
+  const Score& sc = p.sc;
   Row row = doc_row(p, d, rc, r0, rows, hk);
   row.slope *= kLog2e;
   const Tiles ti = tiles_of<64>(row.f, row.l);
-  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits) + wave, i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const int s = blockIdx.y, s0 = min(s * part.tiles, ti.n), i1 = s + 1 < splits ? min(s0 + part.tiles, ti.n) : ti.n;
+  const int i0 = s0 + wave;
+  if (splits > 1 && s0 >= i1) {  // nothing left for this split
+    if (wave == 0 && r < rows && lg == 0)
+      part.ml[(int64_t)s * p.Tq * p.H + row_index(p, d.q0 + by_g(p, r), r, hk)] = float2{-INFINITY, 0.f};
+    return;
+  }
   const uint16_t* Kb = (const uint16_t*)p.K + hk * p.ks[1];
   const uint16_t* Vb = (const uint16_t*)p.V + hk * p.vs[1];
-  uint16_t* mine = ring + wave * (4 * 64 * 64);  // K, V, K, V
-  auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
-    const int k0 = ti.at<64>(i);
+  uint16_t *Kt = ring + wave * (2 * 64 * 64), *Vt = Kt + 64 * 64;
+  auto fetch = [&](const uint16_t* base, int64_t stride, int i, uint16_t* tile) __attribute__((always_inline)) {
     // this wave's reads of the tile that was there are done
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int q = 0; q < 8; q++) dma_piece(Kb, p.ks[0], k0, q, ti.bound, mine + bf * 8192, lane);
-#pragma unroll
-    for (int q = 0; q < 8; q++) dma_piece(Vb, p.vs[0], k0, q, ti.bound, mine + bf * 8192 + 4096, lane);
+    for (int q = 0; q < 8; q++) dma_piece(base, stride, ti.at<64>(i), q, ti.bound, tile, lane);
   };
   Wave w;
   wave_init(w, sc, (const uint16_t*)p.Q + (d.q0 + by_g(p, rc)) * p.qs[0] + (hk * p.G + mod_g(p, rc)) * p.qs[1], lg);
   const Frag32 f = frag32(lane);
-  if (i0 < i1) fetch(i0, 0);
-  int bf = 0;
+  if (i0 < i1) {
+    fetch(Kb, p.ks[0], i0, Kt);
+    fetch(Vb, p.vs[0], i0, Vt);
+  }
   for (int i = i0; i < i1; i += 4) {
-    if (i + 4 < i1) {
-      fetch(i + 4, bf ^ 1);
-      asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // all but the 16 loads just requested
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    const int k0 = ti.at<64>(i), cl = tile_class<64>(row, k0);
-    if (cl != 0)
-      wave_tile<BF16, CAP, BIAS>(w, f, mine + bf * 8192, mine + bf * 8192 + 4096, k0, row, cl == 2, sc, lg);
-    bf ^= 1;
+    const int k0 = ti.at<64>(i);
+    const bool more = i + 4 < i1;
+    float16v st[2];
+    uint4v pf[4];
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // all but the 8 loads of V
+    wave_products<BF16>(w, f, Kt, st);
+    if (more) fetch(Kb, p.ks[0], i + 4, Kt);
+    wave_weights<BF16, CAP, BIAS>(w, st, k0, row, tile_class<64>(row, k0) != 1, sc, lg, pf);
+    if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // all but the next K
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wave_values<BF16>(w, f, Vt, pf);
+    if (more) fetch(Vb, p.vs[0], i + 4, Vt);
   }
   if (!wave_finite(w)) w = wave_again<BF16, CAP, BIAS>(w, Kb, p.ks[0], Vb, p.vs[0], row, ti, i0, i1, 4, sc, lg);
   // join the waves: weights 2^(m_w - max); wave w finishes registers [8 w, 8 w + 8)
@@ -614,7 +692,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   const int rows = d.nq * p.G, r = r0 + l32, rc = min(r, rows - 1);
   const Row row = doc_row(p, d, rc, r0, rows, hk);
   const Tiles ti = tiles_of<kKeys32>(row.f, row.l);
-  const int s = blockIdx.y, i0 = (int)((int64_t)ti.n * s / splits) + wave, i1 = (int)((int64_t)ti.n * (s + 1) / splits);
+  const int s = blockIdx.y, s0 = min(s * part.tiles, ti.n), i1 = s + 1 < splits ? min(s0 + part.tiles, ti.n) : ti.n;
+  const int i0 = s0 + wave;
+  if (splits > 1 && s0 >= i1) {  // nothing left for this split
+    if (wave == 0 && r < rows && lg == 0)
+      part.ml[(int64_t)s * p.Tq * p.H + row_index(p, d.q0 + by_g(p, r), r, hk)] = float2{-INFINITY, 0.f};
+    return;
+  }
   const float* Kb = (const float*)p.K + hk * p.ks[1];
   const float* Vb = (const float*)p.V + hk * p.vs[1];
 
@@ -780,25 +864,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   }
 }
 
-// Joins the parts of split runs: one wave a row, a lane per column.  E2: maxima in
+// Joins the parts of split runs: 16 lanes a row, four columns a lane.  E2: scores in
 // base 2 (the 16-bit kernels), else natural.
 template <bool E2>
 __global__ __launch_bounds__(256) void packed_attn_join(int dt, Parts part, int splits, int64_t rows,
                                                         void* __restrict__ O) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = (threadIdx.x & 15) * 4;
+  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   if (r >= rows) return;
   float m = -INFINITY;
   for (int s = 0; s < splits; s++) m = fmaxf(m, part.ml[s * rows + r].x);
   const float mc = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
+  float l = 0.f;
+  float4v o = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < splits; s++) {
     const float2 ml = part.ml[s * rows + r];
     const float w = E2 ? __builtin_amdgcn_exp2f(ml.x - mc) : expf(ml.x - mc);
     l = fmaf(ml.y, w, l);
-    if (w != 0.f) o = fmaf(part.o[(s * rows + r) * 64 + lane], w, o);
+    if (w == 0.f) continue;  // (a split without tiles has written no output)
+    const float4v v = *(const float4v*)(part.o + (s * rows + r) * 64 + c);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = fmaf(v[e], w, o[e]);
   }
-  store_f(O, r * 64 + lane, dt, l == 0.f ? 0.f : o / l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (dt == HB_F32) {
+    *(float4v*)((float*)O + r * 64 + c) = float4v{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  } else {
+    uint2v x;
+    if (dt == HB_BF16) x = uint2v{pack2<true>(o[0] * inv, o[1] * inv), pack2<true>(o[2] * inv, o[3] * inv)};
+    else x = uint2v{pack2<false>(o[0] * inv, o[1] * inv), pack2<false>(o[2] * inv, o[3] * inv)};
+    *(uint2v*)((uint16_t*)O + r * 64 + c) = x;
+  }
 }
 
 // ------------------------------------------------------------------ any type
@@ -886,14 +982,19 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
   const int64_t rows = (int64_t)p.Tq * p.G;
   const bool f32 = dt == HB_F32, few = f32 || rows <= 64 * (int64_t)p.B;
   const int per = few ? kRowsF : kRowsB, Hk = p.H / p.G, cus = cu_count(ctx);
-  // Keys of an average document's rows, and the blocks they make
+  // An average document's tiles, and the blocks there are
+  const int tile = f32 ? kKeys32 : 64;
   int64_t keys = p.B ? p.Tk / p.B : 0;
-  if (p.half >= 0) keys = std::min<int64_t>(keys, 2 * (int64_t)p.half + per / p.G + 64);
-  const int64_t blocks = std::max<int64_t>((rows + per - 1) / per, p.B) * Hk;
-  const int64_t want = 4 * (int64_t)cus, most = keys / 512;
-  int splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (want + blocks - 1) / std::max<int64_t>(blocks, 1), 32}));
+  if (p.half >= 0) keys = std::min<int64_t>(keys, 2 * (int64_t)p.half + per / p.G + tile);
+  const int64_t tiles = keys / tile, blocks = std::max<int64_t>((rows + per - 1) / per, p.B) * Hk;
+  // A run is split where the blocks would leave the GPU short of work: into pieces
+  // of so many tiles that there are `want` of them, at least 8 each, and twice as many
+  // as an average document has (the last piece takes what is left of a longer one).
+  const int64_t want = (few ? 2 : 4) * (int64_t)cus;
+  Parts part{nullptr, nullptr, (int)std::max<int64_t>(8, blocks * tiles / want)};
+  int splits = (int)std::min<int64_t>(32, (2 * tiles + part.tiles - 1) / part.tiles);
+  if (blocks >= want || part.tiles >= tiles) splits = 1;
   CallScratch held(ctx);
-  Parts part{nullptr, nullptr};
   const int64_t all = (int64_t)p.Tq * p.H;
   if (splits > 1) {
     if (held.take((size_t)(splits * all * (64 * 4 + 8)))) {
@@ -927,7 +1028,7 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
   if (splits > 1) {
     check_launch("hb_sdpa_packed");
     auto join = f32 ? packed_attn_join<false> : packed_attn_join<true>;
-    join<<<(unsigned)((all + 3) / 4), 256, 0, stream_of(ctx)>>>(dt, part, splits, all, p.O);
+    join<<<(unsigned)((all + 15) / 16), 256, 0, stream_of(ctx)>>>(dt, part, splits, all, p.O);
   }
 }
 
@@ -977,6 +1078,7 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   p.half = window < 0 ? -1 : (int)(window / 2 < (1ll << 30) ? window / 2 : (1ll << 30) - 1);
   p.scale = scale;
   p.cap = cap;
+  p.sc = score_of(scale, cap, slopes != 0);
   if (packed_takes_mfma(p, dt == HB_F32 ? 4 : 8)) packed_mfma(ctx, dt, p);
   else packed_any(ctx, dt, p);
   check_launch("hb_sdpa_packed");
