@@ -31,6 +31,7 @@ Design (MI355X-first, not a port of any reference backend):
 """
 from __future__ import annotations
 
+import functools
 import json
 import math
 from typing import Any, Callable, Optional, Sequence
@@ -52,7 +53,8 @@ WIDEN = {"f64": "f32", "i64": "i32", "u64": "i32"}
 FLOAT_DT = ("f32", "f16", "bf16")
 
 
-def _contig(shape) -> tuple:
+@functools.lru_cache(maxsize=4096)
+def _contig_strides(shape: tuple) -> tuple:
     st = []
     acc = 1
     for d in reversed(shape):
@@ -61,11 +63,11 @@ def _contig(shape) -> tuple:
     return tuple(reversed(st))
 
 
-def _numel(shape) -> int:
-    n = 1
-    for d in shape:
-        n *= d
-    return n
+def _contig(shape) -> tuple:
+    return _contig_strides(tuple(shape))
+
+
+_numel = math.prod
 
 
 def _promote(a: str, b: str) -> str:
@@ -515,16 +517,17 @@ class PackedDocs:
     """The plan of a packed batch (HipBackend.packDocs): `offsets` i32 [count +
     1], `doc` and `pos` i32 [total] (each row's document, -1 behind the last one,
     and its position there) and, with a padded length, `slots` i32 [total] (its
-    row in the padded [count, padded] batch, -1 behind the last document).  `blocks`
-    i32 [total // 128 + count + 1, 2] is where sdpaPacked's blocks work."""
+    row in the padded [count, padded] batch, -1 behind the last document).  The table
+    of sdpaPacked's blocks, i32 [total // 128 + count + 1, 2], lies `table` elements
+    behind the offsets in their storage."""
 
-    def __init__(self, be: "HipBackend", count: int, total: int, padded: int, offsets, blocks, doc, pos, slots):
+    def __init__(self, be: "HipBackend", count: int, total: int, padded: int, table: int, offsets, doc, pos, slots):
         self._be = be
-        self.count, self.total, self.padded = count, total, padded
-        self.offsets, self.blocks, self.doc, self.pos, self.slots = offsets, blocks, doc, pos, slots
+        self.count, self.total, self.padded, self.table = count, total, padded, table
+        self.offsets, self.doc, self.pos, self.slots = offsets, doc, pos, slots
 
     def dispose(self) -> None:
-        for t in (self.offsets, self.blocks, self.doc, self.pos, self.slots):
+        for t in (self.offsets, self.doc, self.pos, self.slots):
             self._be.dispose(t)
 
 
@@ -797,7 +800,7 @@ class HipBackend:
 
     def _is_contig(self, t: HipTensor) -> bool:
         exp = _contig(t.shape)
-        return all(s == e or d == 1 for s, e, d in zip(t._strides, exp, t.shape))
+        return t._strides == exp or all(s == e or d == 1 for s, e, d in zip(t._strides, exp, t.shape))
 
     def _contiguous(self, t: HipTensor) -> HipTensor:
         """t itself when contiguous, else a contiguous copy (tracked)."""
@@ -1796,6 +1799,8 @@ class HipBackend:
     # ---------------------------------------------------------------- packed batches
     def _plain(self, t: HipTensor, dtype: str, tmp: list) -> HipTensor:
         """t contiguous and of `dtype`: t itself, or a copy added to `tmp`."""
+        if t._lazy is None and t.dtype == dtype and t._strides == _contig(t.shape):
+            return t
         for c in ((lambda x: x if x.dtype == dtype else self.cast(x, dtype)), self._contiguous):
             n = c(t)
             if n is not t:
@@ -1828,17 +1833,18 @@ class HipBackend:
         tab, step = (count + 64) // 64 * 64, (total + 63) // 64 * 64
         at = tab + (2 * nb + 63) // 64 * 64
         st = self._malloc(4 * (at + step * (3 if padded else 2)))
-        parts = [HipTensor((count + 1,), "i32", st), HipTensor((nb, 2), "i32", st.retain(), tab)]
+        parts = [HipTensor((count + 1,), "i32", st)]
         for i in range(3 if padded else 2):
-            parts.append(HipTensor((total,), "i32", st.retain(), at + i * step))
-        for t in parts:
-            self._track(t)
+            parts.append(HipTensor((total,), "i32", st, at + i * step))
+        st.refs = len(parts)
+        if self._scopes:
+            self._scopes[-1].extend(parts)
         p = st.ptr + 4 * at
         self._call("packDocs", "hb_pack_plan", self.ctx, self._ptr(n), count, total, padded, st.ptr, p, p + 4 * step,
                    p + 8 * step if padded else 0, st.ptr + 4 * tab)
         for t in tmp:
             self.dispose(t)
-        return PackedDocs(self, count, total, padded, *parts, *([] if padded else [None]))
+        return PackedDocs(self, count, total, padded, tab, *parts, *([] if padded else [None]))
 
     def packRows(self, x: HipTensor, docs: PackedDocs) -> HipTensor:
         """Rows of the padded batch x [count, padded, ...] in the packed layout
@@ -1923,7 +1929,7 @@ class HipBackend:
         keys = docs if keys is None else keys
         self._plan(docs, "sdpaPacked")
         self._plan(keys, "sdpaPacked")
-        self._live(q, k, v, prefix, slopes, docs.doc, docs.blocks, docs.offsets, keys.offsets, op="sdpaPacked")
+        self._live(q, k, v, prefix, slopes, docs.doc, docs.offsets, keys.offsets, op="sdpaPacked")
         if len(q.shape) != 3 or len(k.shape) != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
             raise ValueError(f"sdpaPacked: q {list(q.shape)} k {list(k.shape)} v {list(v.shape)}")
         (T, H, D), (Tk, Hk, _) = q.shape, k.shape
@@ -1961,7 +1967,7 @@ class HipBackend:
             self.stats["sdpa"] += 1
             self._call("sdpaPacked", "hb_sdpa_packed", self.ctx, DT[dt][0], self._ptr(q), F.i64s(q._strides),
                        self._ptr(k), F.i64s(k._strides), self._ptr(v), F.i64s(v._strides), out._st.ptr,
-                       self._ptr(docs.doc), self._ptr(docs.blocks), self._ptr(docs.offsets), self._ptr(keys.offsets),
+                       self._ptr(docs.doc), self._ptr(docs.offsets) + 4 * docs.table, self._ptr(docs.offsets), self._ptr(keys.offsets),
                        docs.count, T, Tk, H, Hk, D, float(scale),
                        1 if causal else 0, -1 if window is None else int(window),
                        0 if prefix is None else self._ptr(prefix), float(cap or 0.0),

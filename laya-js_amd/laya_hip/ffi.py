@@ -9,6 +9,7 @@ exits the process (ffi.ts:15-16,190-201).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 from .lib import resolve_lib
 
@@ -117,10 +118,15 @@ class Native:
             raise HipError(f"{op}: {self.last_error()}")
 
 
-def i64s(vals) -> C.Array:
-    """A C int64 array (strides / shapes) from a Python sequence."""
-    vals = list(vals)
+@functools.lru_cache(maxsize=4096)
+def _i64s(vals: tuple) -> C.Array:
     return (C.c_int64 * max(1, len(vals)))(*vals)
+
+
+def i64s(vals) -> C.Array:
+    """A C int64 array (strides / shapes) from a Python sequence: arguments that
+    the library only reads, so equal ones are one array."""
+    return _i64s(tuple(vals))
 
 
 _native: Native | None = None

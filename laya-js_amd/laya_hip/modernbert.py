@@ -265,7 +265,7 @@ class ModernBert:
 
         def f():
             docs = b.packDocs(b.fromHost(HostTensor("i32", lengths.shape, lengths)), total, padded)
-            out = [b.fromHost(HostTensor("i32", (total,), ids)), docs.offsets, docs.blocks, docs.doc, docs.pos]
+            out = [b.fromHost(HostTensor("i32", (total,), ids)), docs.offsets, docs.doc, docs.pos]
             out += [docs.slots] if docs.slots is not None else []
             idx = None
             if adapters is not None:

@@ -53,7 +53,9 @@ def test_plan(b, lengths, total, padded):
     np.testing.assert_array_equal(ints(b, p.offsets), off)
     np.testing.assert_array_equal(ints(b, p.doc), doc)
     np.testing.assert_array_equal(ints(b, p.pos), pos)
-    np.testing.assert_array_equal(ints(b, p.blocks), ref.blocks(off, total))
+    want = ref.blocks(off, total)
+    table = b._view(p.offsets, want.shape, (2, 1), p.offsets._off + p.table)
+    np.testing.assert_array_equal(ints(b, table), want)
     if padded:
         np.testing.assert_array_equal(ints(b, p.slots), slots)
     else:

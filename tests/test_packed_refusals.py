@@ -188,4 +188,4 @@ def test_bank_from_a_scope_outlives_it():
     bank = b.scope(lambda: b.loraBank(b.t(2, 4, 8), b.t(2, 6, 4)))
     assert not (bank.a._dead or bank.b._dead or bank.scales._dead)
     docs = b.scope(lambda: b.packDocs(b.fromHost(HostTensor("i32", (2,), np.zeros(2, np.int32))), 4, 2))
-    assert not any(t._dead for t in (docs.offsets, docs.blocks, docs.doc, docs.pos, docs.slots))
+    assert not any(t._dead for t in (docs.offsets, docs.doc, docs.pos, docs.slots))
