@@ -459,6 +459,33 @@ struct LoraExt {
   int n, R;              // R % 8 == 0
 };
 
+// Whether an adapter of the tile other than row m's own holds a non-finite element of
+// column n's B: only then do the zeros of other rows change an output (0 * inf).
+template <bool BF16>
+__device__ __forceinline__ bool lora_mixed(const LoraExt& ext, const int* adapters, int nd, int N, int m, int n) {
+  const int own = ext.index[m];
+  for (int o = 0; o < nd; o++) {
+    const int a = adapters[o];
+    if (a == own) continue;
+    for (int r = 0; r < ext.R; r++)
+      if (to_f<BF16>(ext.b[((int64_t)a * N + n) * ext.R + r]) * 0.f != 0.f) return true;
+  }
+  return false;
+}
+
+// One output of a projection with adapters, on its own (slow: see its callers).
+template <bool BF16>
+__device__ __forceinline__ uint16_t lora_output(const uint16_t* X, int64_t ldx, const uint16_t* W, const uint16_t* bias,
+                                                int N, int K, const LoraExt& ext, int m, int n) {
+  float sum = 0.f;
+  for (int k = 0; k < K; k++) sum = fmaf(to_f<BF16>(X[(int64_t)m * ldx + k]), to_f<BF16>(W[(int64_t)n * K + k]), sum);
+  const int a = ext.index[m];
+  if (a >= 0 && a < ext.n)
+    for (int r = 0; r < ext.R; r++)
+      sum = fmaf(to_f<BF16>(ext.s[(int64_t)m * ext.R + r]), to_f<BF16>(ext.b[((int64_t)a * N + n) * ext.R + r]), sum);
+  return from_f<BF16>(sum + (bias != nullptr ? to_f<BF16>(bias[n]) : 0.f));
+}
+
 template <int BM, int BN, int WM, int WN, int NST, bool BF16, bool GEGLU, class EXT = NoExt>
 __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restrict__ X, int64_t ldx,
                                                          const uint16_t* __restrict__ W,
@@ -524,11 +551,12 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)smem);
   const int KT0 = K >> 6;
-  int KT = KT0;
+  int KT = KT0, nd = 0;
   // The tile's adapters by number, and the number of each row's (-1: none)
   __shared__ int adapter[LORA ? BM : 1];
   __shared__ int number[LORA ? BM : 1];
   int xnum[LORA ? PW : 1];  // of the rows of this lane's X pieces
+  float inv8 = 0.f;         // of the chunks of an adapter
   if constexpr (LORA) {
     constexpr int Q = (BM + 63) / 64;
     int a[Q], num[Q];
@@ -542,7 +570,6 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
       left[q] = __ballot(a[q] >= 0);
       any |= left[q];
     }
-    int nd = 0;
     while (any != 0) {  // (at most one round per row)
       int cur = 0;
 #pragma unroll
@@ -564,6 +591,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
         if (q * 64 + lane < BM) number[q * 64 + lane] = num[q];
     }
     KT += (nd * ext.R + 63) >> 6;
+    inv8 = 8.f / (float)ext.R;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PW; i++) {
@@ -578,7 +606,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
 #pragma unroll
       for (int i = i0; i < i1; i++) {
         const int p = wave * PW + i, r = p * 8 + (lane >> 3);
-        const int chunk = (kt - KT0) * 8 + ((lane & 7) ^ ((r >> 1) & 7)), o = chunk / r8, c = chunk - o * r8;
+        const int chunk = (kt - KT0) * 8 + ((lane & 7) ^ ((r >> 1) & 7)), o = (int)(((float)chunk + 0.5f) * inv8);
+        const int c = chunk - o * r8;  // (below 2^16 chunks: the quotient by the reciprocal is exact half a unit away)
         uint32_t at = 0xfffffff0u;  // past the records: zeros
         uint64_t base;
         if (p * 8 < BM) {
@@ -587,7 +616,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
         } else {
           base = (uint64_t)ext.b;
           const int n = n0 + r - BM, nc = n < N ? n : N - 1;
-          if (o < xnum[i]) at = (uint32_t)(((int64_t)adapter[o] * N + nc) * ext.R + c * 8) * 2u;
+          if (o < xnum[i]) at = (((uint32_t)adapter[o] * (uint32_t)N + (uint32_t)nc) * (uint32_t)ext.R + c * 8) * 2u;
         }
         const uint4v rs = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base),
                            (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu), 0x80000000u,
@@ -707,15 +736,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
       for (int q = tid; q < BM * BN; q += NT) {
         const int m = m0 + q / BN, n = n0 + q % BN;
         const float v = to_f<BF16>(Cs[q]);
-        if (m >= M || n >= N || v * 0.f == 0.f) continue;
-        float sum = 0.f;
-        for (int k = 0; k < K; k++) sum = fmaf(to_f<BF16>(X[(int64_t)m * ldx + k]), to_f<BF16>(W[(int64_t)n * K + k]), sum);
-        const int a = ext.index[m];
-        if (a >= 0 && a < ext.n)
-          for (int r = 0; r < ext.R; r++)
-            sum = fmaf(to_f<BF16>(ext.s[(int64_t)m * ext.R + r]),
-                       to_f<BF16>(ext.b[((int64_t)a * N + n) * ext.R + r]), sum);
-        Cs[q] = from_f<BF16>(sum + (bias != nullptr ? to_f<BF16>(bias[n]) : 0.f));
+        if (m >= M || n >= N || v * 0.f == 0.f || !lora_mixed<BF16>(ext, adapter, nd, N, m, n)) continue;
+        Cs[q] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, n);
       }
     }
   }

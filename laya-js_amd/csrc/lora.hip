@@ -6,9 +6,10 @@
 // with a bank of n adapters A [n, R, K], B [n, N, R]; a row whose index is
 // outside [0, n) has none.
 //
-// lora_shrink: s = scale_i x_m . A_i^T of f16 / bf16 rows on v_mfma_f32_16x16x32,
+// lora_prepare: s = scale_i x_m . A_i^T of f16 / bf16 rows on v_mfma_f32_16x16x32,
 // rounded to the 16-bit type for the second product, which the projection's own
-// GEMM takes as ranks beyond K (gemm_ring with LoraExt): y is rounded once.
+// GEMM takes as ranks beyond K (gemm_ring with LoraExt, or lora_stream for large
+// M): y is rounded once.
 //
 // lora_shrink_any, lora_expand_any: the inner products s = scale_i x_m . A_i^T
 // in f32, then y = round(y + s . B_i^T) on top of the projection, any type and
@@ -22,63 +23,102 @@ namespace hb {
 
 // ------------------------------------------------------------------ f16 / bf16
 
-// A block takes 16 MT rows and 64 ranks; its four waves share out K by 64 and
-// their sums meet in LDS.  The rows' distinct adapters are gone through one after
-// another, for all rows of the block, and a row keeps its own adapter's sums;
-// with few row blocks those are shared out over gridDim.z.  Bound by reading x
-// once (and A from the caches); at few rows by the chain of loads.
+// lora_stream: rows and columns of a tile, stages of its ring, their width, waves
+constexpr int kStTile = 256, kStStages = 4, kStBK = 32, kStWaves = 8;
+constexpr int kStStage = 2 * kStTile * kStBK;  // u16 of a stage
+constexpr int kStLds = kStStages * kStStage * 2;
+
+// The adapters of lora_stream's tiles of rows, as LoraExt describes them.
+struct Numbers {
+  int16_t* number;        // [tiles * 256]: each row's adapter's number in its tile of 256 rows, or -1
+  int32_t *list, *count;  // [tiles * 256]: the adapters by number; [tiles]
+  int tiles;              // 0: gemm_ring numbers them itself (48 rows of 24 adapters: 17 us, with numbers from here 19)
+};
+
+// What the projection's GEMM needs beforehand, in one launch (two runs of blocks): the
+// numbers, and the rows' inner products with their adapters.
+struct Prepare {
+  const uint16_t* x;
+  int64_t ldx;
+  const uint16_t* a;
+  const float* scales;
+  const int32_t* index;
+  int n, M, R, K;
+  uint16_t* s;               // [M, R]
+  Numbers num;
+  int gx, gy, gz;            // inner products: row blocks, rank blocks, turns
+};
+
+// Inner products.  A block takes 16 MT rows and 64 ranks; its four waves share out K
+// by 64 and their sums meet in LDS.  The rows' distinct adapters are gone through one
+// after another, for all rows of the block, and a row keeps its own adapter's sums;
+// with few row blocks those are shared out over gz blocks.  Bound by reading x once
+// (and A from the caches); at few rows by the chain of loads, so that a chunk's loads
+// are requested before the last one's products.  (16k x 1024, rank 64: 24 us of which
+// reading x is 7.)
 template <bool BF16, int MT>
-__global__ __launch_bounds__(256) void lora_shrink(const uint16_t* __restrict__ X, int64_t ldx,
-                                                   const uint16_t* __restrict__ A, const float* __restrict__ scales,
-                                                   const int32_t* __restrict__ index, int n, int M, int R, int K,
-                                                   uint16_t* __restrict__ S) {
-  __shared__ __attribute__((aligned(16))) float red[4][MT * 16][68];  // 64 ranks, padded against bank conflicts
+__device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int bz, float (*red)[MT * 16][68]) {
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int m0 = blockIdx.x * 16 * MT, r0 = blockIdx.y * 64;
-  int a = lane < 16 * MT && m0 + lane < M ? index[m0 + lane] : -1;
-  if (a >= n) a = -1;
+  const int m0 = bx * 16 * MT, r0 = by * 64, R = p.R, K = p.K;
+  int a = lane < 16 * MT && m0 + lane < p.M ? p.index[m0 + lane] : -1;
+  if (a >= p.n) a = -1;
   uint64_t left = __ballot(a >= 0);
   const uint16_t* xr[MT];
 #pragma unroll
-  for (int i = 0; i < MT; i++) xr[i] = X + (int64_t)min(m0 + 16 * i + l16, M - 1) * ldx + 8 * g;
+  for (int i = 0; i < MT; i++) xr[i] = p.x + (int64_t)min(m0 + 16 * i + l16, p.M - 1) * p.ldx + 8 * g;
+  const int nt = min((R - r0 + 15) >> 4, 4);  // rank blocks there are
   for (int turn = 0; left != 0; turn++) {
     const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
     const uint64_t same = __ballot(a == cur);
     left &= ~same;
-    if (turn % gridDim.z != blockIdx.z) continue;  // (the same in every wave)
+    if (turn % p.gz != bz) continue;  // (the same in every wave)
     const uint16_t* ar[4];
 #pragma unroll
-    for (int t = 0; t < 4; t++) ar[t] = A + ((int64_t)cur * R + min(r0 + 16 * t + l16, R - 1)) * K + 8 * g;
+    for (int t = 0; t < 4; t++) ar[t] = p.a + ((int64_t)cur * R + min(r0 + 16 * t + l16, R - 1)) * K + 8 * g;
     float4v acc[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
       for (int t = 0; t < 4; t++) acc[i][t] = float4v{0.f, 0.f, 0.f, 0.f};
-    const int nt = min((R - r0 + 15) >> 4, 4);  // rank blocks there are
-    for (int k = wave * 64; k < K; k += 256) {
-      uint4v xf[MT][2];
+    struct Chunk {
+      uint4v x[MT][2], a[4][2];
+    } c0, c1;
+    auto load = [&](Chunk& c, int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < MT; i++)
+      for (int s = 0; s < 2; s++) {
 #pragma unroll
-        for (int s = 0; s < 2; s++) xf[i][s] = *(const uint4v*)(xr[i] + k + 32 * s);
+        for (int i = 0; i < MT; i++) c.x[i][s] = *(const uint4v*)(xr[i] + k + 32 * s);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+          if (t < nt) c.a[t][s] = *(const uint4v*)(ar[t] + k + 32 * s);
+      }
+    };
+    auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         if (t >= nt) break;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-          const uint4v af = *(const uint4v*)(ar[t] + k + 32 * s);
+        for (int s = 0; s < 2; s++)
 #pragma unroll
           for (int i = 0; i < MT; i++) {
             if constexpr (BF16)
-              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, af),
-                                                                  __builtin_bit_cast(bf16x8, xf[i][s]), acc[i][t], 0, 0, 0);
+              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c.a[t][s]),
+                                                                  __builtin_bit_cast(bf16x8, c.x[i][s]), acc[i][t], 0, 0, 0);
             else
-              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, af),
-                                                                 __builtin_bit_cast(half8, xf[i][s]), acc[i][t], 0, 0, 0);
+              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c.a[t][s]),
+                                                                 __builtin_bit_cast(half8, c.x[i][s]), acc[i][t], 0, 0, 0);
           }
-        }
       }
+    };
+    int k = wave * 64;
+    if (k < K) load(c0, k);
+    for (; k < K; k += 512) {
+      if (k + 256 < K) load(c1, k + 256);
+      multiply(c0);
+      if (k + 256 >= K) break;
+      if (k + 512 < K) load(c0, k + 512);
+      multiply(c1);
     }
     // lane: row l16 of its block, ranks 16 t + 4 g ..
 #pragma unroll
@@ -86,7 +126,7 @@ __global__ __launch_bounds__(256) void lora_shrink(const uint16_t* __restrict__ 
 #pragma unroll
       for (int t = 0; t < 4; t++) *(float4v*)&red[wave][16 * i + l16][16 * t + 4 * g] = acc[i][t];
     __syncthreads();
-    const float sc = scales[cur];
+    const float sc = p.scales[cur];
     for (int q = tid; q < 16 * MT * 16; q += 256) {  // four ranks of a row
       const int row = q >> 4, r = (q & 15) * 4;
       if (!((same >> row) & 1) || r0 + r >= R) continue;  // (R % 8 == 0)
@@ -95,20 +135,360 @@ __global__ __launch_bounds__(256) void lora_shrink(const uint16_t* __restrict__ 
       for (int w = 1; w < 4; w++) v += *(const float4v*)&red[w][row][r];
       const uint32_t h[4] = {from_f<BF16>(v[0] * sc), from_f<BF16>(v[1] * sc), from_f<BF16>(v[2] * sc),
                              from_f<BF16>(v[3] * sc)};
-      *(uint2v*)(S + (int64_t)(m0 + row) * R + r0 + r) = uint2v{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+      *(uint2v*)(p.s + (int64_t)(m0 + row) * R + r0 + r) = uint2v{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
     }
     __syncthreads();  // the sums are written again
   }
 }
 
-// The ring's tile for the projection with adapters.
+// Numbers a tile's adapters as they first occur (one wave, up to 256 rows).
+__device__ __forceinline__ void lora_number(const Prepare& p, int tile) {
+  const int lane = threadIdx.x;
+  if (lane >= 64) return;
+  const int64_t m0 = (int64_t)tile * kStTile;
+  int a[4], num[4];
+  uint64_t left[4], any = 0;
+#pragma unroll
+  for (int q = 0; q < 4; q++) {
+    const int r = q * 64 + lane;
+    a[q] = r < kStTile && m0 + r < p.M ? p.index[m0 + r] : -1;
+    if (a[q] >= p.n) a[q] = -1;
+    num[q] = -1;
+    left[q] = __ballot(a[q] >= 0);
+    any |= left[q];
+  }
+  int nd = 0;
+  while (any != 0) {  // (at most one round per row)
+    int cur = 0;
+#pragma unroll
+    for (int q = 3; q >= 0; q--)
+      if (left[q] != 0) cur = __builtin_amdgcn_readlane(a[q], __builtin_ctzll(left[q]));
+    any = 0;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      if (a[q] == cur) num[q] = nd;
+      left[q] &= ~__ballot(a[q] == cur);
+      any |= left[q];
+    }
+    if (lane == 0) p.num.list[m0 + nd] = cur;
+    nd++;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; q++)
+    if (q * 64 + lane < kStTile) p.num.number[m0 + q * 64 + lane] = (int16_t)num[q];
+  if (lane == 0) p.num.count[tile] = nd;
+}
+
+template <bool BF16, int MT>
+__global__ __launch_bounds__(256) void lora_prepare(Prepare p) {
+  __shared__ __attribute__((aligned(16))) float red[4][MT * 16][68];  // 64 ranks, padded against bank conflicts
+  int b = blockIdx.x;
+  if (b < p.num.tiles) return lora_number(p, b);
+  b -= p.num.tiles;
+  const int bx = b % p.gx, q = b / p.gx;
+  lora_inner<BF16, MT>(p, bx, q % p.gy, q / p.gy, red);
+}
+
+// The projection with adapters for large M: 256 x 256 tiles, 8 waves of 128 x 64 (6
+// fragment reads per 8 products; 16 waves of 64 x 64 read 8, 16k x 5248 x 1024 rank 64
+// 257 -> 273 us; 4 of 128 x 128 do not fit the registers, 305), a ring of four 32-wide
+// stages as gemm_ring's, and one block per CU that streams its tiles without a pause:
+// the ring is filled with the next tile's first stages during a tile's last ones, and
+// the outputs go from registers to memory (the lane halves exchange 4 columns, so that
+// a lane stores 8 of a row) while those loads are on their way.  On gemm_ring's blocks
+// of one tile each the same tiles took 269 us, its tiles of 128 x 256 338.
+// What bounds it: 242 us with lora_prepare's 24; without the loads into LDS 197, without
+// the fragment reads too 187: the products alone, at the clock that the card holds under
+// them, and behind them the 32 KB per stage from the L2.
+// Of its numbering only whole-wave scalars are read, by scalar loads (kept in their
+// address space), which the waits for the ring do not count.
+using ScalarInts = const __attribute__((address_space(4))) int32_t*;
+__device__ __forceinline__ ScalarInts scalar_ints(const void* p) {
+  const uint64_t a = (uint64_t)p;
+  return (ScalarInts)(((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32) |
+                      (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a));
+}
+
+__device__ __forceinline__ int stream_f(int r) { return (r >> 2) & 3; }  // swizzle of a row's 4 chunks
+
 template <bool BF16>
-static void lora_ring(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, const uint16_t* w, const uint16_t* bias,
-                      uint16_t* y, int64_t ldy, int M, int N, int K, const LoraExt& ext) {
+__global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __restrict__ X, int64_t ldx,
+                                                             const uint16_t* __restrict__ W,
+                                                             const uint16_t* __restrict__ bias, uint16_t* __restrict__ Y,
+                                                             int64_t ldy, int M, int N, int K, int tiles_m, int tiles_n,
+                                                             LoraExt ext, Numbers num) {
+  constexpr int NST = kStStages, NW = kStWaves, WM = 2, WN = NW / WM, TM = kStTile / WM / 32, TN = kStTile / WN / 32;
+  constexpr int PW = 2 * kStTile / 16 / NW;  // 1 KB pieces (16 rows) of a stage per wave
+  constexpr int ST = TM * TN * 2;            // stores of a tile per lane
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, lg = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const bool xwave = wave < NW / 2;  // requests pieces of X, else of W
+  const int KT0 = K / kStBK;
+  const float inv8 = 8.f / (float)ext.R;
+
+  // An XCD has one contiguous run of tiles, its blocks take them in turn; tiles are
+  // numbered down 4 row tiles, then along N, so that the XCD's 32 share 4 x 8 operands
+  // in its L2.
+  const int ntiles = tiles_m * tiles_n, xcd = blockIdx.x & 7, nb = (int)((gridDim.x - xcd + 7) >> 3);
+  const int run0 = (int)((int64_t)ntiles * xcd >> 3), run1 = (int)((int64_t)ntiles * (xcd + 1) >> 3);
+  auto place = [&](int t, int* tm, int* tn) {
+    constexpr int G = 4;
+    const int grp = t / (G * tiles_n), rem = t - grp * G * tiles_n, gm = min(G, tiles_m - grp * G);
+    *tn = rem / gm;
+    *tm = grp * G + rem - *tn * gm;
+  };
+
+  // ---- requests: the tile they are at, its stage, and this wave's pieces of it
+  int rt = run0 + (int)(blockIdx.x >> 3), rk = 0, rKT = 0, rn0 = 0;
+  uint4v rsrc{};
+  uint32_t off[PW];
+  int xnum[PW];
+  const int slot4 = (lane & 3), prow = lane >> 2;  // slot and row within a piece
+  auto enter = [&]() __attribute__((always_inline)) {
+    int tm, tn;
+    place(rt, &tm, &tn);
+    const int nd = scalar_ints(num.count)[tm];
+    rKT = KT0 + (nd * ext.R + kStBK - 1) / kStBK;
+    rk = 0;
+    rn0 = tn * kStTile;
+    const uint64_t base = xwave ? (uint64_t)(X + (int64_t)tm * kStTile * ldx) : (uint64_t)(W + (int64_t)rn0 * K);
+    rsrc = uint4v{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base),
+                  (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu), 0x80000000u, 0x00020000u};
+#pragma unroll
+    for (int i = 0; i < PW; i++) {
+      const int r = (wave % (NW / 2) * PW + i) * 16 + prow;  // of X or of W
+      const uint32_t c = (slot4 ^ stream_f(r)) * 16;
+      // (rows past the operand are clamped: their outputs are never stored)
+      off[i] = xwave ? (uint32_t)min(r, M - 1 - tm * kStTile) * (uint32_t)ldx * 2u + c
+                     : (uint32_t)min(r, N - 1 - rn0) * (uint32_t)K * 2u + c;
+      xnum[i] = nd;
+      if (xwave) {  // the piece's 16 rows' numbers, two to a word: scalar loads, which no wait for the ring counts
+        const ScalarInts nums = scalar_ints(num.number + (int64_t)tm * kStTile + (wave % (NW / 2) * PW + i) * 16);
+        int v = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          int w = nums[e];
+          asm("" : "+s"(w));  // (or the compiler loads a chosen address per lane)
+          v = (lane >> 3) == e ? w : v;
+        }
+        xnum[i] = (int)(int16_t)(v >> (16 * ((lane >> 2) & 1)));
+      }
+    }
+  };
+  const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)smem);
+  // the next stage into ring slot `slot`; the last one of a tile moves on to the next
+  auto request = [&](int slot) __attribute__((always_inline)) {
+    const uint32_t to = lds0 + (uint32_t)(slot * kStStage * 2 + wave * PW * 1024);
+    if (rk < KT0) {
+#pragma unroll
+      for (int i = 0; i < PW; i++) buffer_lds16(rsrc, off[i], (uint32_t)rk * 64u, to + 1024u * i);
+    } else {
+      // 4 chunks of 8 ranks of the adapters' axis (LoraExt)
+      const int ch0 = (rk - KT0) * 4, r8 = ext.R >> 3;
+      const uint64_t base = xwave ? (uint64_t)ext.s : (uint64_t)ext.b;
+      const uint4v rs = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base),
+                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu), 0x80000000u,
+                         0x00020000u};
+      int tm, tn;
+      place(rt, &tm, &tn);
+      const ScalarInts list = scalar_ints(num.list + (int64_t)tm * kStTile);
+      int who[4];  // the chunks' adapters
+      if (!xwave) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          who[j] = list[min(__builtin_amdgcn_readfirstlane((int)(((float)(ch0 + j) + 0.5f) * inv8)), kStTile - 1)];
+      }
+#pragma unroll
+      for (int i = 0; i < PW; i++) {
+        const int r = (wave % (NW / 2) * PW + i) * 16 + prow, j = slot4 ^ stream_f(r);
+        const int o = (int)(((float)(ch0 + j) + 0.5f) * inv8), c = ch0 + j - o * r8;
+        uint32_t at = 0xfffffff0u;  // past the records: zeros
+        if (xwave) {
+          if (o == xnum[i]) at = ((uint32_t)(tm * kStTile + r) * (uint32_t)ext.R + (uint32_t)c * 8u) * 2u;
+        } else if (o < xnum[i]) {
+          const int a = j == 0 ? who[0] : j == 1 ? who[1] : j == 2 ? who[2] : who[3];
+          const int n = min(rn0 + r, N - 1);
+          at = (((uint32_t)a * (uint32_t)N + (uint32_t)n) * (uint32_t)ext.R + (uint32_t)c * 8u) * 2u;
+        }
+        buffer_lds16(rs, at, to + 1024u * i);
+      }
+    }
+    if (++rk == rKT) {
+      rt += nb;
+      if (rt < run1) enter();
+    }
+  };
+
+  // ---- products
+  float16v acc[TM][TN];
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+  };
+  int fo[2];
+#pragma unroll
+  for (int s = 0; s < 2; s++) fo[s] = l32 * kStBK + (((2 * s + lg) ^ stream_f(l32)) << 3);
+  uint4v xf[2][TM], wf[2][TN];
+  auto read = [&](int slot, int s, int d) __attribute__((always_inline)) {
+    const uint16_t* b = smem + slot * kStStage;
+#pragma unroll
+    for (int i = 0; i < TM; i++) xf[d][i] = *(const uint4v*)(b + fo[s] + (wm * TM + i) * 32 * kStBK);
+#pragma unroll
+    for (int j = 0; j < TN; j++) wf[d][j] = *(const uint4v*)(b + fo[s] + (kStTile + (wn * TN + j) * 32) * kStBK);
+  };
+  auto multiply = [&](int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = mfma32<BF16>(wf[d][j], xf[d][i], acc[i][j]);
+  };
+
+  if (rt >= run1) return;  // (the whole block: more blocks than tiles)
+  int ct = rt;             // the tile whose products are made
+  enter();
+  // total stages of this block's tiles are at least 2 (K >= 64)
+  int ahead = 0;  // stages requested and not yet multiplied
+#pragma unroll
+  for (int s = 0; s < NST - 1; s++)
+    if (rt < run1) {
+      request(s);
+      ahead++;
+    }
+  ring_wait_stages<PW, NST - 2>(ahead - 1);
+  read(0, 0, 0);
+  clear();
+  int slot = 0;
+  bool stored = false;  // the stores lie between the requests of this tile's stages 2 and 3
+  while (true) {
+    int tm, tn;
+    place(ct, &tm, &tn);
+    const int KT = KT0 + (scalar_ints(num.count)[tm] * ext.R + kStBK - 1) / kStBK;
+    for (int kt = 0; kt < KT; kt++) {
+      // the stage after this one has landed (if there is one) and everybody is done
+      // with the one before, whose slot takes the third from here
+      if (ahead >= NST - 1) {
+        if (stored && kt < NST - 2) ring_wait_barrier<(NST - 3) * PW + ST>();
+        else ring_wait_barrier<(NST - 3) * PW>();
+      } else {
+        ring_wait_barrier<0>();
+      }
+      read(slot, 1, 1);
+      multiply(0);
+      if (rt < run1) request(slot == 0 ? NST - 1 : slot - 1);
+      else ahead--;
+      slot = slot == NST - 1 ? 0 : slot + 1;
+      if (ahead > 0) read(slot, 0, 0);
+      multiply(1);
+    }
+    // ---- write-out: lane l32 holds row l32 of a 32 x 32 block, columns 8 g + 4 lg ..
+    const int m0 = tm * kStTile + wm * TM * 32, n0 = tn * kStTile + wn * TN * 32;
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) z = fmaf(acc[i][j][r], 0.f, z);
+    const bool odd = __any(z != 0.f);  // (a non-finite output: below)
+    float bv[TN][4][4];
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        uint2v b = {0u, 0u};
+        if (bias != nullptr) b = *(const uint2v*)(bias + min(n0 + 32 * j + 8 * g + 4 * lg, N - 4));
+#pragma unroll
+        for (int e = 0; e < 4; e++) bv[j][g][e] = to_f<BF16>((uint16_t)(b[e >> 1] >> (16 * (e & 1))));
+      }
+    const auto ys = __builtin_amdgcn_make_buffer_rsrc((void*)(Y + (int64_t)(tm * kStTile) * ldy + tn * kStTile), 0,
+                                                      0x80000000u, 0x00020000u);
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int m = m0 + 32 * i + l32;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          uint32_t lo[2], hi[2];
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const int x = 8 * h + 4 * g;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = acc[i][j][x + e] + bv[j][2 * h + g][e];
+            lo[g] = (uint32_t)from_f<BF16>(v[0]) | ((uint32_t)from_f<BF16>(v[1]) << 16);
+            hi[g] = (uint32_t)from_f<BF16>(v[2]) | ((uint32_t)from_f<BF16>(v[3]) << 16);
+          }
+          // lane half lg now takes all 8 columns of group 2 h + lg
+          const auto a = __builtin_amdgcn_permlane32_swap(lo[0], lo[1], false, false);
+          const auto c = __builtin_amdgcn_permlane32_swap(hi[0], hi[1], false, false);
+          const uint4v o = {(uint32_t)a[0], (uint32_t)c[0], (uint32_t)a[1], (uint32_t)c[1]};
+          const int n = n0 + 32 * j + 16 * h + 8 * lg;
+          // as many stores whatever the edges: those past them fall outside the records
+          const uint32_t at = m < M && n < N
+                                  ? (uint32_t)(m - tm * kStTile) * (uint32_t)ldy * 2u + (uint32_t)(n - tn * kStTile) * 2u
+                                  : 0xfffffff0u;
+          __builtin_amdgcn_raw_buffer_store_b128(o, ys, at, 0, 0);
+        }
+    }
+    stored = !odd;
+    if (odd) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      // the zeros of other rows do not keep a non-finite B out of a row's sums (0 *
+      // inf): an output that has come out non-finite is computed again with its own
+      // row's adapter alone
+      const int* list = num.list + (int64_t)tm * kStTile;
+      const int nd = num.count[tm];
+#pragma unroll 1
+      for (int q = lane; q < TM * TN * 1024; q += 64) {
+        const int m = m0 + q / (TN * 32), n = n0 + q % (TN * 32);
+        if (m >= M || n >= N) continue;
+        const float v = to_f<BF16>(__builtin_nontemporal_load(Y + (int64_t)m * ldy + n));
+        if (v * 0.f == 0.f || !lora_mixed<BF16>(ext, list, nd, N, m, n)) continue;
+        Y[(int64_t)m * ldy + n] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, n);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    ct += nb;
+    if (ct >= run1) return;
+    clear();
+  }
+}
+
+// The GEMM's tile, by the rules of the plain projection (ring_tile); on the streaming
+// kernel, which stores 16 bytes at a time, once its tiles occupy half of the CUs
+// (f16, 4 adapters in runs of 512 rows, streaming and by ring_tile: 4096 x 2304 x 768, 144 tiles, 36 and 45 us; 3000 x
+// 5248 x 1024 47 and 102; 16384 x 768 x 1152 51 and 81; 16k x 5248 x 1024 262 and 502).
+// Its tiles of 256 rows suit rows that come in runs of one request: a tile of all
+// different adapters multiplies 256 R ranks, gemm_ring's tile of 64 rows 64 R.
+static bool lora_streams(int cus, int64_t M, int64_t N, const uint16_t* bias, const uint16_t* y, int64_t ldy) {
+  if (M <= kStTile || N % 8 != 0 || ldy % 8 != 0 || (uintptr_t)y % 16 != 0 || (uintptr_t)bias % 8 != 0) return false;
+  return 2 * ((M + kStTile - 1) / kStTile) * ((N + kStTile - 1) / kStTile) >= cus;
+}
+template <bool BF16>
+static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, const uint16_t* w, const uint16_t* bias,
+                      uint16_t* y, int64_t ldy, int M, int N, int K, const LoraExt& ext, const Numbers& num) {
+  if (num.tiles > 0) {
+    auto kernel = lora_stream<BF16>;
+    static std::atomic<uint64_t> attr{0};
+    once_per_device(attr, [&] {
+      HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kStLds));
+    });
+    const int tm = (M + kStTile - 1) / kStTile, tn = (N + kStTile - 1) / kStTile;
+    kernel<<<(unsigned)std::min<int64_t>(cus, (int64_t)tm * tn), kStWaves * 64, kStLds, st>>>(x, ldx, w, bias, y, ldy, M, N,
+                                                                                       K, tm, tn, ext, num);
+    return;
+  }
   auto go = [&](auto launch) { launch(st, 0u, x, ldx, w, bias, (const uint16_t*)nullptr, (int64_t)0, y, ldy, M, N, K, ext); };
   LinearKernel tile = LinearKernel::kRing64x64x3;
   ring_tile(cus, M, N, K, false, true, false, &tile);
-  if (M >= 4096) tile = LinearKernel::kRing128x256;
   switch (tile) {
     case LinearKernel::kRing32x64: return go(launch_ring_t<32, 64, 1, 2, 6, BF16, false, LoraExt>);
     case LinearKernel::kRing64x64: return go(launch_ring_t<64, 64, 2, 2, 4, BF16, false, LoraExt>);
@@ -177,32 +557,39 @@ static bool lora_takes_ring(int dt, uintptr_t x, int64_t ldx, uintptr_t w, uintp
                             int64_t K, const LoraArgs& l) {
   return (dt == HB_F16 || dt == HB_BF16) && M > 0 && N > 0 && K > 0 && l.n > 0 && l.R > 0 && ring_ok(ldx, K) &&
          l.R % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && (x | w | y | l.a | l.b) % 16 == 0 &&
-         l.n * l.R * N * 2 < (1ll << 31);
+         l.n * l.R * N * 2 < (1ll << 31) && M * l.R * 2 < (1ll << 31) && ldy < (1 << 22);
 }
 
 // The projection with adapters on 16-bit weights; false: no memory for the inner
 // products.
 static bool lora_fused(uintptr_t ctx, int dt, const uint16_t* x, int64_t ldx, const uint16_t* w, const uint16_t* bias,
                        uint16_t* y, int64_t ldy, int M, int N, int K, const LoraArgs& l) {
-  CallScratch held(ctx);
-  if (!held.take((size_t)M * l.R * 2)) return false;
-  uint16_t* S = (uint16_t*)held.p;
-  hipStream_t st = stream_of(ctx);
   const int cus = cu_count(ctx);
-  auto shrink = [&](auto kern, int rows) {
-    const unsigned gx = (unsigned)((M + rows - 1) / rows), gy = (unsigned)((l.R + 63) / 64);
-    const int64_t blocks = (int64_t)gx * gy;
-    const unsigned gz = (unsigned)std::max<int64_t>(1, std::min<int64_t>({l.n, rows, cus / blocks}));
-    kern<<<dim3(gx, gy, gz), 256, 0, st>>>(x, ldx, (const uint16_t*)l.a, (const float*)l.scales, (const int32_t*)l.index,
-                                           (int)l.n, M, (int)l.R, K, S);
-  };
+  const int tiles = lora_streams(cus, M, N, bias, y, ldy) ? (M + kStTile - 1) / kStTile : 0;
+  const int64_t rows = (int64_t)tiles * kStTile, s_bytes = ((int64_t)M * l.R * 2 + 255) / 256 * 256;
+  CallScratch held(ctx);
+  if (!held.take((size_t)(s_bytes + rows * 6 + tiles * 4))) return false;
+  Prepare p{x, ldx, (const uint16_t*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, M, (int)l.R, K};
+  p.s = (uint16_t*)held.p;
+  p.num.list = (int32_t*)((char*)held.p + s_bytes);
+  p.num.count = p.num.list + rows;
+  p.num.number = (int16_t*)(p.num.count + tiles);
+  p.num.tiles = tiles;
+  const int br = M >= 8192 ? 32 : 16;
+  p.gx = (M + br - 1) / br;
+  p.gy = ((int)l.R + 63) / 64;
+  p.gz = (int)std::max<int64_t>(2, std::min<int64_t>({l.n, br, cus / ((int64_t)p.gx * p.gy)}));
+  const int64_t blocks = tiles + (int64_t)p.gx * p.gy * p.gz;
+  if (blocks >= (1ll << 31)) return false;
+  hipStream_t st = stream_of(ctx);
   const bool bf = dt == HB_BF16;
-  if (M >= 8192) shrink(bf ? lora_shrink<true, 2> : lora_shrink<false, 2>, 32);
-  else shrink(bf ? lora_shrink<true, 1> : lora_shrink<false, 1>, 16);
+  auto prepare = br == 32 ? (bf ? lora_prepare<true, 2> : lora_prepare<false, 2>)
+                            : (bf ? lora_prepare<true, 1> : lora_prepare<false, 1>);
+  prepare<<<(unsigned)blocks, 256, 0, st>>>(p);
   check_launch("hb_lora_linear");
-  const LoraExt ext{S, (const uint16_t*)l.b, (const int32_t*)l.index, (int)l.n, (int)l.R};
-  if (bf) lora_ring<true>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext);
-  else lora_ring<false>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext);
+  const LoraExt ext{p.s, (const uint16_t*)l.b, p.index, p.n, p.R};
+  if (bf) lora_gemm<true>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
+  else lora_gemm<false>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
   check_launch("hb_lora_linear");
   return true;
 }

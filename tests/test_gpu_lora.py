@@ -159,6 +159,53 @@ def test_lora_adapters_do_not_reach_other_rows(b, dtype, what):
     assert not np.isfinite(got[c["index"] == 1][:, 5:9]).any() and not np.isfinite(got[149]).any()
 
 
+# sizes whose tiles of 256 x 256 go round the CUs: K of two stages, edges in both
+# directions, tiles without and of many adapters, ranks that end inside a stage
+LARGE = [(8200, 1032, 64, 5, 8), (4099, 2056, 128, 40, 72), (520, 16392, 64, 2, 16), (4096, 2304, 192, 3, 64),
+         (33000, 256, 64, 90, 24), (1, 65544, 64, 2, 8)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,n,R", LARGE)
+def test_lora_large(b, dtype, M, N, K, n, R):
+    """Rows in runs of their requests, some without an adapter."""
+    rng = np.random.default_rng(M + N)
+    runs = rng.integers(1, 700, M)
+    c = case(rng, dtype, M, N, K, n, R, index=np.repeat(rng.integers(-1, n, M), runs)[:M], bias=M % 2 == 0)
+    x, bank, index, bias = dev(b, c, dtype)
+    w = b.fromHost(to_host(c["w"], dtype))
+    check(read32(b, b.loraLinear(x, w, bank, index, bias)), c, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_lora_large_shuffled(b, dtype):
+    rng = np.random.default_rng(3)
+    c = case(rng, dtype, 4100, 2056, 64, 300, 8, index=rng.integers(-1, 301, 4100))
+    x, bank, index, _ = dev(b, c, dtype)
+    check(read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index)), c, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_lora_large_adapters_do_not_reach_other_rows(b, dtype, what):
+    rng = np.random.default_rng(12)
+    M, N = 4100, 2064
+    c = case(rng, dtype, M, N, 64, 4, 8, index=np.arange(M) // 20 % 5)
+    c["b"][1, 5:9], c["a"][2, 3] = what, what
+    c["x"][M - 1, 0] = what
+    x, bank, index, _ = dev(b, c, dtype)
+    got = read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index))
+    bad = (c["index"] == 1)[:, None] & ((np.arange(N) >= 5) & (np.arange(N) < 9))[None]
+    bad[c["index"] == 2] = True
+    bad[M - 1] = True
+    c["b"][1, 5:9], c["a"][2, 3], c["x"][M - 1, 0] = 0, 0, 0
+    y, mass, delta = ref.lora_linear(c["x"], c["w"], None, c["a"], c["b"], c["scales"].astype(np.float64), c["index"])
+    u = U[dtype]
+    tol = u * np.abs(y) + u * delta + u * (np.abs(y) + 2 * delta) + 80 * 2.0 ** -23 * (mass + delta)
+    assert (np.abs(got - y) <= tol)[~bad].all()
+    assert not np.isfinite(got[(c["index"] == 1)][:, 5:9]).any() and not np.isfinite(got[M - 1]).any()
+
+
 def test_lora_empty(b):
     """No rows, no adapters, rank 0, and weights of no inputs."""
     rng = np.random.default_rng(0)
@@ -170,7 +217,7 @@ def test_lora_empty(b):
         np.testing.assert_array_equal(got, read32(b, b.linear(x, w)))
 
 
-@pytest.mark.parametrize("M", [48, 600])
+@pytest.mark.parametrize("M", [48, 600, 17000])
 def test_lora_recorded(b, M):
     """Two layers recorded into a graph share scratch; replays with other rows
     and adapter numbers, eager calls in between, give the eager bits."""
