@@ -385,16 +385,6 @@ static void launch_dequant_rows(hipStream_t st, int cus, int dt, const QW& q, ui
   else dequant_rows_kernel<QB, AFF, false><<<grid, 256, 0, st>>>(q, out, rows, K);
 }
 
-namespace hb {
-// The copy above for any of the formats (K % 8 == 0, group % 8 == 0).
-void dequantize_rows(hipStream_t st, int cus, int dt, int bits, int mode, const QW& q, uint16_t* out, int64_t rows, int K) {
-  if (bits == 8 && mode == 0) launch_dequant_rows<8, false>(st, cus, dt, q, out, rows, K);
-  else if (bits == 8) launch_dequant_rows<8, true>(st, cus, dt, q, out, rows, K);
-  else if (mode == 0) launch_dequant_rows<4, false>(st, cus, dt, q, out, rows, K);
-  else launch_dequant_rows<4, true>(st, cus, dt, q, out, rows, K);
-}
-}  // namespace hb
-
 extern "C" int hb_qlinear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t qw, uintptr_t scales,
                           uintptr_t zeros, uintptr_t bias, uintptr_t resid, int64_t ldr, uintptr_t y, int64_t ldy,
                           int64_t M, int64_t N, int64_t K, int bits, int group, int mode, unsigned flags) {
@@ -439,7 +429,10 @@ extern "C" int hb_qlinear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintp
     }
     if (dequant) {
       uint16_t* wd = (uint16_t*)held.p;
-      dequantize_rows(st, cus, dt, bits, mode, q, wd, rows, k);
+      if (bits == 8 && mode == 0) launch_dequant_rows<8, false>(st, cus, dt, q, wd, rows, k);
+      else if (bits == 8) launch_dequant_rows<8, true>(st, cus, dt, q, wd, rows, k);
+      else if (mode == 0) launch_dequant_rows<4, false>(st, cus, dt, q, wd, rows, k);
+      else launch_dequant_rows<4, true>(st, cus, dt, q, wd, rows, k);
       check_launch("hb_qlinear (dequantize)");
       mfma_dtype<0, false, false>(dt, geglu, st, cus, pan, X, ldx, wd, q, Bp, Rp, ldr, Yp, ldy, m, n, k);
     } else if (bits == 8 && mode == 0) mfma_dtype<8, false, false>(dt, geglu, st, cus, pan, X, ldx, nullptr, q, Bp, Rp, ldr, Yp, ldy, m, n, k);

@@ -122,9 +122,6 @@ struct QW {  // quantized weight operand
   int group;  // values per group
 };
 
-// Dequantizes `rows` rows of a quantized weight into 16-bit weights (gemm.hip).
-void dequantize_rows(hipStream_t st, int cus, int dt, int bits, int mode, const QW& q, uint16_t* out, int64_t rows, int K);
-
 // The fused-projection epilogue (QKV): y = x . W^T with W the
 // stacked [3 * H * 64, K] q / k / v projection, written head-major as
 // [3][B][H][L][64] (B = M / L) with RoPE applied to the q and k parts.

@@ -35,63 +35,78 @@ struct Numbers {
   int tiles;              // 0: gemm_ring numbers them itself (48 rows of 24 adapters: 17 us, with numbers from here 19)
 };
 
-// What the projection's GEMM needs beforehand, in one launch (two runs of blocks): the
-// numbers, and the rows' inner products with their adapters.
+// A quantized weight [N, K] and its 16-bit copy.
+struct Codes {
+  QW q;
+  uint16_t* copy;
+  int bits, mode;    // 8 or 4, 1: affine
+  int N, K, blocks;  // 0 blocks: none
+};
+
+// What the projection's GEMM needs beforehand, in one launch (runs of blocks): the
+// rows' inner products with their adapters, the numbers, and the weight's copy, as
+// hb_qlinear makes it.  (With a launch of its own for the copy: 54
+// rows x 1024 x 2624 35 -> 30 us.)
 struct Prepare {
-  const uint16_t* x;
+  const char* x;
   int64_t ldx;
-  const uint16_t* a;
+  const char* a;
   const float* scales;
   const int32_t* index;
   int n, M, R, K;
-  uint16_t* s;               // [M, R]
+  void* s;                   // [M, R], of x's type
   Numbers num;
-  int gx, gy, gz;            // inner products: row blocks, rank blocks, turns
+  Codes codes;
+  int br, gx, gy, gz;        // inner products: ranks of a block, row blocks, rank blocks, turns
 };
 
-// Inner products.  A block takes 16 MT rows and 64 ranks; its four waves share out K
+// Inner products.  A block takes 16 MT rows and br ranks; its four waves share out K
 // by 64 and their sums meet in LDS.  The rows' distinct adapters are gone through one
 // after another, for all rows of the block, and a row keeps its own adapter's sums;
-// with few row blocks those are shared out over gz blocks.  Bound by reading x once
-// (and A from the caches); at few rows by the chain of loads, so that a chunk's loads
-// are requested before the last one's products.  (16k x 1024, rank 64: 24 us of which
+// with few row blocks those are shared out over gz blocks.  f32 rows go through
+// v_mfma_f32_16x16x4: of four k in a lane's registers each product takes one.  Bound by
+// reading x once (and A from the caches); at few rows by the chain of loads, so that a
+// chunk's loads are requested before the last one's products, and by one CU's reading of
+// A, so that blocks take 16 ranks then (48 x 2624, 29 adapters
+// of rank 64: 14.9 -> 8.3 us).  (16k x 1024, rank 64: 24 us of which
 // reading x is 7.)
-template <bool BF16, int MT>
+template <int DT, int MT>
 __device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int bz, float (*red)[MT * 16][68]) {
+  constexpr int ES = DT == HB_F32 ? 4 : 2, S = ES;  // bytes; 16-byte loads of a lane per 64 k
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int m0 = bx * 16 * MT, r0 = by * 64, R = p.R, K = p.K;
+  const int m0 = bx * 16 * MT, r0 = by * p.br, R = p.R, K = p.K;
   int a = lane < 16 * MT && m0 + lane < p.M ? p.index[m0 + lane] : -1;
   if (a >= p.n) a = -1;
   uint64_t left = __ballot(a >= 0);
-  const uint16_t* xr[MT];
+  const char* xr[MT];
 #pragma unroll
-  for (int i = 0; i < MT; i++) xr[i] = p.x + (int64_t)min(m0 + 16 * i + l16, p.M - 1) * p.ldx + 8 * g;
-  const int nt = min((R - r0 + 15) >> 4, 4);  // rank blocks there are
+  for (int i = 0; i < MT; i++) xr[i] = p.x + (int64_t)min(m0 + 16 * i + l16, p.M - 1) * p.ldx * ES + 16 * g;
+  const int nt = min((min(R - r0, p.br) + 15) >> 4, 4);  // rank blocks there are
   for (int turn = 0; left != 0; turn++) {
     const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
     const uint64_t same = __ballot(a == cur);
     left &= ~same;
     if (turn % p.gz != bz) continue;  // (the same in every wave)
-    const uint16_t* ar[4];
+    const char* ar[4];
 #pragma unroll
-    for (int t = 0; t < 4; t++) ar[t] = p.a + ((int64_t)cur * R + min(r0 + 16 * t + l16, R - 1)) * K + 8 * g;
+    for (int t = 0; t < 4; t++) ar[t] = p.a + ((int64_t)cur * R + min(r0 + 16 * t + l16, R - 1)) * K * ES + 16 * g;
     float4v acc[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
       for (int t = 0; t < 4; t++) acc[i][t] = float4v{0.f, 0.f, 0.f, 0.f};
     struct Chunk {
-      uint4v x[MT][2], a[4][2];
+      uint4v x[MT][S], a[4][S];
     } c0, c1;
     auto load = [&](Chunk& c, int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int s = 0; s < 2; s++) {
+      for (int s = 0; s < S; s++) {
 #pragma unroll
-        for (int i = 0; i < MT; i++) c.x[i][s] = *(const uint4v*)(xr[i] + k + 32 * s);
+        for (int i = 0; i < MT; i++) c.x[i][s] = *(const uint4v*)(xr[i] + (int64_t)k * ES + 64 * s);
 #pragma unroll
         for (int t = 0; t < 4; t++)
-          if (t < nt) c.a[t][s] = *(const uint4v*)(ar[t] + k + 32 * s);
+          if (t < nt) c.a[t][s] = *(const uint4v*)(ar[t] + (int64_t)k * ES + 64 * s);
       }
     };
     auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
@@ -99,15 +114,20 @@ __device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int
       for (int t = 0; t < 4; t++) {
         if (t >= nt) break;
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int s = 0; s < S; s++)
 #pragma unroll
           for (int i = 0; i < MT; i++) {
-            if constexpr (BF16)
+            if constexpr (DT == HB_F32) {
+              const float4v av = __builtin_bit_cast(float4v, c.a[t][s]), xv = __builtin_bit_cast(float4v, c.x[i][s]);
+#pragma unroll
+              for (int e = 0; e < 4; e++) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], xv[e], acc[i][t], 0, 0, 0);
+            } else if constexpr (DT == HB_BF16) {
               acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c.a[t][s]),
                                                                   __builtin_bit_cast(bf16x8, c.x[i][s]), acc[i][t], 0, 0, 0);
-            else
+            } else {
               acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c.a[t][s]),
                                                                  __builtin_bit_cast(half8, c.x[i][s]), acc[i][t], 0, 0, 0);
+            }
           }
       }
     };
@@ -129,13 +149,19 @@ __device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int
     const float sc = p.scales[cur];
     for (int q = tid; q < 16 * MT * 16; q += 256) {  // four ranks of a row
       const int row = q >> 4, r = (q & 15) * 4;
-      if (!((same >> row) & 1) || r0 + r >= R) continue;  // (R % 8 == 0)
+      if (!((same >> row) & 1) || r >= 16 * nt || r0 + r >= R) continue;  // (R % 4 == 0)
       float4v v = *(const float4v*)&red[0][row][r];
 #pragma unroll
       for (int w = 1; w < 4; w++) v += *(const float4v*)&red[w][row][r];
-      const uint32_t h[4] = {from_f<BF16>(v[0] * sc), from_f<BF16>(v[1] * sc), from_f<BF16>(v[2] * sc),
-                             from_f<BF16>(v[3] * sc)};
-      *(uint2v*)(p.s + (int64_t)(m0 + row) * R + r0 + r) = uint2v{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+      v *= sc;
+      const int64_t at = (int64_t)(m0 + row) * R + r0 + r;
+      if constexpr (DT == HB_F32) {
+        *(float4v*)((float*)p.s + at) = v;
+      } else {
+        constexpr bool BF16 = DT == HB_BF16;
+        const uint32_t h[4] = {from_f<BF16>(v[0]), from_f<BF16>(v[1]), from_f<BF16>(v[2]), from_f<BF16>(v[3])};
+        *(uint2v*)((uint16_t*)p.s + at) = uint2v{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+      }
     }
     __syncthreads();  // the sums are written again
   }
@@ -179,14 +205,222 @@ __device__ __forceinline__ void lora_number(const Prepare& p, int tile) {
   if (lane == 0) p.num.count[tile] = nd;
 }
 
-template <bool BF16, int MT>
+// 8 codes at a time, four of them requested together.
+template <int QB, bool AFF, bool BF16>
+__device__ __forceinline__ void lora_dequantize(const Codes& c, int block) {
+  const int cpr = c.K >> 3, n = c.N * cpr, step = c.blocks * 256;
+  for (int i0 = block * 256 + (int)threadIdx.x; i0 < n; i0 += 4 * step) {
+    uint32_t w0[4], w1[4], sb[4], zb[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int i = min(i0 + u * step, n - 1), r = i / cpr, k = 8 * (i - r * cpr);
+      if constexpr (QB == 8) {
+        const uint2v w = *(const uint2v*)(c.q.q + (int64_t)i * 8);
+        w0[u] = w.x;
+        w1[u] = w.y;
+      } else {
+        w0[u] = *(const uint32_t*)(c.q.q + (int64_t)i * 4);
+        w1[u] = 0;
+      }
+      const int64_t gi = (int64_t)r * c.q.G + k / c.q.group;
+      sb[u] = ((const uint16_t*)c.q.scales)[gi];
+      zb[u] = AFF ? ((const uint16_t*)c.q.zeros)[gi] : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (i0 + u * step < n)
+        *(uint4v*)(c.copy + (int64_t)(i0 + u * step) * 8) = dequant8<QB, AFF, false, BF16>(w0[u], w1[u], sb[u], zb[u], 0.f, 0.f);
+  }
+}
+
+template <int DT, int MT>
 __global__ __launch_bounds__(256) void lora_prepare(Prepare p) {
   __shared__ __attribute__((aligned(16))) float red[4][MT * 16][68];  // 64 ranks, padded against bank conflicts
-  int b = blockIdx.x;
-  if (b < p.num.tiles) return lora_number(p, b);
-  b -= p.num.tiles;
-  const int bx = b % p.gx, q = b / p.gx;
-  lora_inner<BF16, MT>(p, bx, q % p.gy, q / p.gy, red);
+  const int b = blockIdx.x, inner = p.gx * p.gy * p.gz;
+  if (b < inner) {
+    const int bx = b % p.gx, q = b / p.gx;
+    return lora_inner<DT, MT>(p, bx, q % p.gy, q / p.gy, red);
+  }
+  if constexpr (DT != HB_F32) {
+    constexpr bool BF16 = DT == HB_BF16;
+    const Codes& c = p.codes;
+    const int e = b - inner - p.num.tiles;
+    if (e < 0) lora_number(p, b - inner);
+    else if (c.bits == 8 && c.mode == 0) lora_dequantize<8, false, BF16>(c, e);
+    else if (c.bits == 8) lora_dequantize<8, true, BF16>(c, e);
+    else if (c.mode == 0) lora_dequantize<4, false, BF16>(c, e);
+    else lora_dequantize<4, true, BF16>(c, e);
+  }
+}
+
+static void launch_prepare(hipStream_t st, int cus, int dt, Prepare& p) {
+  const int rows = p.M >= 8192 ? 32 : 16;
+  p.gx = (p.M + rows - 1) / rows;
+  p.br = 64;
+  p.gy = (p.R + 63) / 64;
+  p.gz = std::max(2, std::min({p.n, rows, cus / (int)std::min<int64_t>((int64_t)p.gx * p.gy, cus)}));
+  if ((int64_t)p.gx * p.gy * p.gz < cus) {
+    p.br = 16;
+    p.gy = (p.R + 15) / 16;
+  }
+  const int64_t blocks = (int64_t)p.gx * p.gy * p.gz + p.num.tiles + p.codes.blocks;
+  HB_REQUIRE(blocks < (1ll << 31), "hb_lora_linear: too many rows and ranks");
+  auto kernel = rows == 32 ? (dt == HB_F32 ? lora_prepare<HB_F32, 2> : dt == HB_F16 ? lora_prepare<HB_F16, 2> : lora_prepare<HB_BF16, 2>)
+                           : (dt == HB_F32 ? lora_prepare<HB_F32, 1> : dt == HB_F16 ? lora_prepare<HB_F16, 1> : lora_prepare<HB_BF16, 1>);
+  kernel<<<(unsigned)blocks, 256, 0, st>>>(p);
+}
+
+// The projection with adapters for few rows: tiles of up to 32 x 32, whose 8 waves share out
+// K, then the adapters' axis (LoraExt), fragments straight from memory into registers,
+// and meet in LDS.  Bound by the chain of loads (the tile's adapters, operands, s and
+// B): a wave's are requested kFewDeep chunks ahead, nothing waits for a barrier
+// before the sums.  K's sum has another order than the other kernels' (a wave per tile
+// in theirs: 12.5 us at the first of these sizes).  Taken up to 5 tiles to 4 CUs (f16;
+// here and on gemm_ring's tiles, with lora_prepare: 48 x 2304 x 768, 24 adapters of rank
+// 16, 10.4 and 15.6 us; 128 x 2304 x 768, 288 tiles, 11.8 and 12.4; 512 x 768 x 1152, 384
+// tiles, 15.0 and 14.6; 128 x 5248 x 1024, 656 tiles, 22 and 18).  The tiles are of 16
+// columns while they leave CUs idle, so that a CU reads less (48 x 1024 x 2624, 24
+// adapters of rank 64: 22.5 -> 19.2 us; 100 x 768 x 1152: 13.4 -> 11.9), and of 16 rows
+// where there are no more.
+constexpr int kFewDeep = 2;
+
+template <bool BF16, int TM, int TN>
+__global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W,
+                                                const uint16_t* __restrict__ bias, uint16_t* __restrict__ Y, int64_t ldy,
+                                                int M, int N, int K, int tiles_m, LoraExt ext) {
+  __shared__ __attribute__((aligned(16))) float red[8][TM * 16][TN * 16 + 4];  // padded against bank conflicts
+  __shared__ int adapter[32];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile = xcd_tile(blockIdx.x, gridDim.x), tn = tile / tiles_m;
+  const int m0 = (tile - tn * tiles_m) * TM * 16, n0 = tn * TN * 16, R = ext.R;
+  int a = lane < TM * 16 && m0 + lane < M ? ext.index[m0 + lane] : -1;
+  const uint16_t *xr[TM], *wr[TN];
+  int mr[TM], nr[TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++) {
+    mr[i] = min(m0 + 16 * i + l16, M - 1);
+    xr[i] = X + (int64_t)mr[i] * ldx + 8 * g;
+  }
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+    nr[j] = min(n0 + 16 * j + l16, N - 1);
+    wr[j] = W + (int64_t)nr[j] * K + 8 * g;
+  }
+  float4v acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
+  struct Chunk {  // of 64 k, or of 64 ranks
+    uint4v x[TM][2], w[TN][2];
+  } c[kFewDeep];
+  auto load = [&](Chunk& c, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+#pragma unroll
+      for (int i = 0; i < TM; i++) c.x[i][s] = *(const uint4v*)(xr[i] + k + 32 * s);
+#pragma unroll
+      for (int j = 0; j < TN; j++) c.w[j][s] = *(const uint4v*)(wr[j] + k + 32 * s);
+    }
+  };
+  auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+          if constexpr (BF16)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c.w[j][s]),
+                                                                __builtin_bit_cast(bf16x8, c.x[i][s]), acc[i][j], 0, 0, 0);
+          else
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c.w[j][s]),
+                                                               __builtin_bit_cast(half8, c.x[i][s]), acc[i][j], 0, 0, 0);
+        }
+  };
+  const int k0 = wave * 64;
+#pragma unroll
+  for (int b = 0; b < kFewDeep; b++)
+    if (k0 + 512 * b < K) load(c[b], k0 + 512 * b);
+  // the tile's adapters by number, as they first occur: lane o has number o's
+  if (a >= ext.n) a = -1;
+  int num = -1, mine = 0, nd = 0;
+  for (uint64_t left = __ballot(a >= 0); left != 0; nd++) {  // (at most one round per row)
+    const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+    const uint64_t same = __ballot(a == cur);
+    left &= ~same;
+    num = a == cur ? nd : num;
+    mine = lane == nd ? cur : mine;
+  }
+  if (tid < 32) adapter[tid] = mine;
+  int xnum[TM];
+#pragma unroll
+  for (int i = 0; i < TM; i++) xnum[i] = __shfl(num, 16 * i + l16);
+  const int r8 = R >> 3, chunks = (nd * r8 + 7) >> 3;  // chunks of 8 ranks of an adapter; chunks of 64 ranks
+  const float inv8 = 8.f / (float)R;
+  auto load_ranks = [&](Chunk& c, int e) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const int ch = e * 8 + s * 4 + g, o = (int)(((float)ch + 0.5f) * inv8), r = (ch - o * r8) * 8;
+      const int who = __shfl(mine, o & 31);
+#pragma unroll
+      for (int i = 0; i < TM; i++) {
+        c.x[i][s] = uint4v{0u, 0u, 0u, 0u};
+        if (o == xnum[i]) c.x[i][s] = *(const uint4v*)(ext.s + (int64_t)mr[i] * R + r);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        c.w[j][s] = uint4v{0u, 0u, 0u, 0u};
+        if (o < nd) c.w[j][s] = *(const uint4v*)(ext.b + ((int64_t)who * N + nr[j]) * R + r);
+      }
+    }
+  };
+  for (int k = k0; k < K; k += 512 * kFewDeep) {
+#pragma unroll
+    for (int b = 0; b < kFewDeep; b++) {
+      if (k + 512 * b >= K) break;
+      multiply(c[b]);
+      if (k + 512 * (b + kFewDeep) < K) load(c[b], k + 512 * (b + kFewDeep));
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < kFewDeep; b++)
+    if (wave + 8 * b < chunks) load_ranks(c[b], wave + 8 * b);
+  for (int e = wave; e < chunks; e += 8 * kFewDeep) {
+#pragma unroll
+    for (int b = 0; b < kFewDeep; b++) {
+      if (e + 8 * b >= chunks) break;
+      multiply(c[b]);
+      if (e + 8 * (b + kFewDeep) < chunks) load_ranks(c[b], e + 8 * (b + kFewDeep));
+    }
+  }
+  // lane: row 16 i + l16, columns 16 j + 4 g ..
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++) *(float4v*)&red[wave][16 * i + l16][16 * j + 4 * g] = acc[i][j];
+  __syncthreads();
+  constexpr int CW = TN * 8;  // threads of a row
+  const int row = tid / CW, col = tid % CW * 2, m = m0 + row, n = n0 + col;
+  if (row >= TM * 16 || m >= M || n >= N) return;
+  float v[2] = {0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < 8; w++)
+#pragma unroll
+    for (int q = 0; q < 2; q++) v[q] += red[w][row][col + q];
+  uint16_t o[2];
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const int nq = min(n + q, N - 1);
+    o[q] = from_f<BF16>(v[q] + (bias != nullptr ? to_f<BF16>(bias[nq]) : 0.f));
+    // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf)
+    if (v[q] * 0.f != 0.f && lora_mixed<BF16>(ext, adapter, nd, N, m, nq))
+      o[q] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, nq);
+  }
+  uint16_t* y = Y + (int64_t)m * ldy + n;
+  if (n + 1 < N) *(uint32_t*)y = (uint32_t)o[0] | ((uint32_t)o[1] << 16);
+  else y[0] = o[0];
 }
 
 // The projection with adapters for large M: 256 x 256 tiles, 8 waves of 128 x 64 (6
@@ -486,6 +720,17 @@ static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, c
                                                                                        K, tm, tn, ext, num);
     return;
   }
+  const int64_t few = (int64_t)((M + 31) / 32) * ((N + 31) / 32);
+  if (4 * few <= 5 * cus) {
+    auto run = [&](auto kernel, int bm, int bn) {
+      const int tm = (M + bm - 1) / bm;
+      kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), 512, 0, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, ext);
+    };
+    const bool half = 2 * few <= cus;
+    if (M <= 16) half ? run(lora_few<BF16, 1, 1>, 16, 16) : run(lora_few<BF16, 1, 2>, 16, 32);
+    else half ? run(lora_few<BF16, 2, 1>, 32, 16) : run(lora_few<BF16, 2, 2>, 32, 32);
+    return;
+  }
   auto go = [&](auto launch) { launch(st, 0u, x, ldx, w, bias, (const uint16_t*)nullptr, (int64_t)0, y, ldy, M, N, K, ext); };
   LinearKernel tile = LinearKernel::kRing64x64x3;
   ring_tile(cus, M, N, K, false, true, false, &tile);
@@ -496,6 +741,67 @@ static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, c
     case LinearKernel::kRing128x64: return go(launch_ring_t<128, 64, 4, 2, 4, BF16, false, LoraExt>);
     case LinearKernel::kRing128x256: return go(launch_ring_t<128, 256, 4, 4, 3, BF16, false, LoraExt>);
     default: return go(launch_ring_t<64, 64, 2, 2, 3, BF16, false, LoraExt>);
+  }
+}
+
+// ------------------------------------------------------------------ f32
+
+// y += s . B^T of f32 rows on v_mfma_f32_16x16x4, onto the projection: 4 waves of 32
+// rows and 64 columns, the rows' distinct adapters one after another (of few tiles shared
+// out over blocks), each row's columns read and written in its own adapter's turn.  Bound by that, 8 bytes an output.
+__global__ __launch_bounds__(256) void lora_expand_f32(const float* __restrict__ S, const float* __restrict__ Bk,
+                                                       const int32_t* __restrict__ index, int n, int M, int N, int R,
+                                                       float* __restrict__ Y, int64_t ldy) {
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m0 = blockIdx.y * 32, n0 = (blockIdx.x * 4 + wave) * 64;
+  int a = lane < 32 && m0 + lane < M ? index[m0 + lane] : -1;
+  if (a >= n) a = -1;
+  if (n0 >= N) return;
+  const float* sr[2];
+  int own[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    sr[i] = S + (int64_t)min(m0 + 16 * i + l16, M - 1) * R + 4 * g;
+    own[i] = __shfl(a, 16 * i + l16);
+  }
+  int turn = 0;
+  for (uint64_t left = __ballot(a >= 0); left != 0; turn++) {
+    const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+    left &= ~__ballot(a == cur);
+    if (turn % (int)gridDim.z != (int)blockIdx.z) continue;  // (a row is in one turn)
+    const float* br[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) br[t] = Bk + ((int64_t)cur * N + min(n0 + 16 * t + l16, N - 1)) * R + 4 * g;
+    float4v acc[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) acc[i][t] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int r = 0; r < R; r += 16) {
+      const bool in = r + 4 * g < R;
+      float4v x[2], b[4];
+#pragma unroll
+      for (int i = 0; i < 2; i++) x[i] = in ? *(const float4v*)(sr[i] + r) : float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < 4; t++) b[t] = in ? *(const float4v*)(br[t] + r) : float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int t = 0; t < 4; t++) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[t][e], x[i][e], acc[i][t], 0, 0, 0);
+    }
+    // lane: row 16 i + l16, columns 16 t + 4 g ..
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      if (own[i] != cur) continue;  // (cur >= 0: no row behind M)
+      float* y = Y + (int64_t)(m0 + 16 * i + l16) * ldy + n0 + 4 * g;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+        if (n0 + 16 * t + 4 * g < N) *(float4v*)(y + 16 * t) += acc[i][t];  // (N % 4 == 0)
+    }
   }
 }
 
@@ -560,35 +866,34 @@ static bool lora_takes_ring(int dt, uintptr_t x, int64_t ldx, uintptr_t w, uintp
          l.n * l.R * N * 2 < (1ll << 31) && M * l.R * 2 < (1ll << 31) && ldy < (1 << 22);
 }
 
-// The projection with adapters on 16-bit weights; false: no memory for the inner
-// products.
-static bool lora_fused(uintptr_t ctx, int dt, const uint16_t* x, int64_t ldx, const uint16_t* w, const uint16_t* bias,
-                       uint16_t* y, int64_t ldy, int M, int N, int K, const LoraArgs& l) {
+// The projection with adapters on 16-bit weights w, or on quantized ones (`codes`);
+// false: no memory for the inner products, or for the weights' copy.
+static bool lora_fused(uintptr_t ctx, int dt, const uint16_t* x, int64_t ldx, const uint16_t* w, Codes codes,
+                       const uint16_t* bias, uint16_t* y, int64_t ldy, int M, int N, int K, const LoraArgs& l) {
   const int cus = cu_count(ctx);
   const int tiles = lora_streams(cus, M, N, bias, y, ldy) ? (M + kStTile - 1) / kStTile : 0;
   const int64_t rows = (int64_t)tiles * kStTile, s_bytes = ((int64_t)M * l.R * 2 + 255) / 256 * 256;
   CallScratch held(ctx);
-  if (!held.take((size_t)(s_bytes + rows * 6 + tiles * 4))) return false;
-  Prepare p{x, ldx, (const uint16_t*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, M, (int)l.R, K};
-  p.s = (uint16_t*)held.p;
-  p.num.list = (int32_t*)((char*)held.p + s_bytes);
+  const int64_t w_bytes = codes.bits ? (int64_t)N * K * 2 : 0;  // (K % 64 == 0)
+  if (!held.take((size_t)(w_bytes + s_bytes + rows * 6 + tiles * 4))) return false;
+  Prepare p{(const char*)x, ldx, (const char*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, M, (int)l.R, K};
+  if (codes.bits) {
+    codes.blocks = (int)std::min<int64_t>(((int64_t)N * K / 8 + 1023) / 1024, (int64_t)cus * 16);
+    codes.N = N;
+    codes.K = K;
+    w = codes.copy = (uint16_t*)held.p;
+  }
+  p.codes = codes;
+  p.s = (char*)held.p + w_bytes;
+  p.num.list = (int32_t*)((char*)p.s + s_bytes);
   p.num.count = p.num.list + rows;
   p.num.number = (int16_t*)(p.num.count + tiles);
   p.num.tiles = tiles;
-  const int br = M >= 8192 ? 32 : 16;
-  p.gx = (M + br - 1) / br;
-  p.gy = ((int)l.R + 63) / 64;
-  p.gz = (int)std::max<int64_t>(2, std::min<int64_t>({l.n, br, cus / ((int64_t)p.gx * p.gy)}));
-  const int64_t blocks = tiles + (int64_t)p.gx * p.gy * p.gz;
-  if (blocks >= (1ll << 31)) return false;
   hipStream_t st = stream_of(ctx);
-  const bool bf = dt == HB_BF16;
-  auto prepare = br == 32 ? (bf ? lora_prepare<true, 2> : lora_prepare<false, 2>)
-                            : (bf ? lora_prepare<true, 1> : lora_prepare<false, 1>);
-  prepare<<<(unsigned)blocks, 256, 0, st>>>(p);
+  launch_prepare(st, cus, dt, p);
   check_launch("hb_lora_linear");
-  const LoraExt ext{p.s, (const uint16_t*)l.b, p.index, p.n, p.R};
-  if (bf) lora_gemm<true>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
+  const LoraExt ext{(const uint16_t*)p.s, (const uint16_t*)l.b, p.index, p.n, p.R};
+  if (dt == HB_BF16) lora_gemm<true>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
   else lora_gemm<false>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
   check_launch("hb_lora_linear");
   return true;
@@ -601,6 +906,19 @@ static void add_adapters(uintptr_t ctx, const char* op, int dt, uintptr_t x, int
   if (!s.take((size_t)(M * l.R * 4)))
     throw std::runtime_error(std::string(op) + ": out of device memory for the adapters' inner products");
   hipStream_t st = stream_of(ctx);
+  if (dt == HB_F32 && K % 64 == 0 && N % 4 == 0 && l.R % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 &&
+      (x | y | l.a | l.b) % 16 == 0 && (M + 31) / 32 < 65536) {
+    Prepare p{(const char*)x, ldx, (const char*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, (int)M,
+              (int)l.R, (int)K};
+    p.s = s.p;
+    launch_prepare(st, cu_count(ctx), dt, p);
+    const int64_t tiles = (N + 255) / 256 * ((M + 31) / 32);
+    const dim3 blocks((unsigned)((N + 255) / 256), (unsigned)((M + 31) / 32),
+                      (unsigned)std::max<int64_t>(1, std::min<int64_t>({l.n, 32, 2 * cu_count(ctx) / std::max<int64_t>(tiles, 1)})));
+    lora_expand_f32<<<blocks, 256, 0, st>>>((const float*)s.p, (const float*)l.b, (const int32_t*)l.index, (int)l.n, (int)M,
+                                            (int)N, (int)l.R, (float*)y, ldy);
+    return check_launch(op);
+  }
   HB_REQUIRE((M * l.R + 3) / 4 < (1ll << 31), "hb_lora_linear: too many rows and ranks");
   lora_shrink_any<<<(unsigned)((M * l.R + 3) / 4), 256, 0, st>>>(dt, (const void*)x, ldx, (const void*)l.a,
                                                                  (const float*)l.scales, (const int32_t*)l.index,
@@ -625,8 +943,8 @@ int hb_lora_linear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t w,
   check_lora("hb_lora_linear", dt, M, N, K, l);
   HB_REQUIRE(ldx >= K && ldy >= N, "hb_lora_linear: leading dimension smaller than the row");
   if (lora_takes_ring(dt, x, ldx, w, y, ldy, M, N, K, l) &&
-      lora_fused(ctx, dt, (const uint16_t*)x, ldx, (const uint16_t*)w, (const uint16_t*)bias, (uint16_t*)y, ldy, (int)M,
-                 (int)N, (int)K, l))
+      lora_fused(ctx, dt, (const uint16_t*)x, ldx, (const uint16_t*)w, Codes{}, (const uint16_t*)bias, (uint16_t*)y, ldy,
+                 (int)M, (int)N, (int)K, l))
     return 0;
   if (hb_linear(ctx, dt, x, ldx, w, bias, 0, 0, y, ldy, M, N, K, bias ? HB_EPI_BIAS : 0)) return -1;
   add_adapters(ctx, "hb_lora_linear", dt, x, ldx, y, ldy, M, N, K, l);
@@ -642,18 +960,15 @@ int hb_lora_qlinear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t q
   HB_REQUIRE(ldx >= K && ldy >= N, "hb_lora_qlinear: leading dimension smaller than the row");
   HB_REQUIRE((bits == 8 || bits == 4) && (mode == 0 || mode == 1) && group > 0, "hb_lora_qlinear: bad bits, mode or group");
   HB_REQUIRE(qw && qscales && (mode == 0 || zeros), "hb_lora_qlinear: missing weight tensors");
-  if (lora_takes_ring(dt, x, ldx, 0, y, ldy, M, N, K, l) && group % 8 == 0 && qw % 8 == 0 && qscales % 2 == 0 &&
+  if (lora_takes_ring(dt, x, ldx, 0, y, ldy, M, N, K, l) && group % 8 == 0 && N * K < (1ll << 33) && qw % 8 == 0 && qscales % 2 == 0 &&
       zeros % 2 == 0) {
-    // the weight dequantized into a 16-bit copy, as hb_qlinear does
-    CallScratch copy(ctx);
-    if (copy.take((size_t)(N * K * 2))) {
-      const QW q{(const uint8_t*)qw, (const void*)qscales, (const void*)zeros, (int)((K + group - 1) / group), group};
-      dequantize_rows(stream_of(ctx), cu_count(ctx), dt, bits, mode, q, (uint16_t*)copy.p, N, (int)K);
-      check_launch("hb_lora_qlinear (dequantize)");
-      if (lora_fused(ctx, dt, (const uint16_t*)x, ldx, (const uint16_t*)copy.p, (const uint16_t*)bias, (uint16_t*)y, ldy,
-                     (int)M, (int)N, (int)K, l))
-        return 0;
-    }
+    Codes codes{};
+    codes.q = QW{(const uint8_t*)qw, (const void*)qscales, (const void*)zeros, (int)((K + group - 1) / group), group};
+    codes.bits = bits;
+    codes.mode = mode;
+    if (lora_fused(ctx, dt, (const uint16_t*)x, ldx, nullptr, codes, (const uint16_t*)bias, (uint16_t*)y, ldy, (int)M,
+                   (int)N, (int)K, l))
+      return 0;
   }
   if (hb_qlinear(ctx, dt, x, ldx, qw, qscales, zeros, bias, 0, 0, y, ldy, M, N, K, bits, group, mode,
                  bias ? HB_EPI_BIAS : 0))

@@ -534,7 +534,7 @@ class PackedDocs:
 class LoraBank:
     """Low-rank adapters of one projection (HipBackend.loraBank): `count`
     adapters of rank `rank`, a [count, rank, in], b [count, out, rank] and f32
-    scales [count].  16-bit banks hold a whole number of 8 ranks, the last ones
+    scales [count].  Banks hold a whole number of 16 bytes of ranks, the last ones
     zero."""
 
     def __init__(self, be: "HipBackend", a, b, scales, rank: int):
@@ -1994,8 +1994,9 @@ class HipBackend:
         else:
             s = self._held(scales if scales.dtype == "f32" else self.cast(scales, "f32"))
         rank = a.shape[1]
-        if a.dtype != "f32" and rank % 8:
-            a, b = self._padded(a, 1, -rank % 8), self._padded(b, 2, -rank % 8)
+        unit = 4 if a.dtype == "f32" else 8  # ranks of 16 bytes
+        if rank % unit:
+            a, b = self._padded(a, 1, -rank % unit), self._padded(b, 2, -rank % unit)
         return LoraBank(self, self._held(a), self._held(b), s, rank)
 
     def _padded(self, t: HipTensor, axis: int, more: int) -> HipTensor:
