@@ -677,6 +677,64 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
 // B operand of O^T += V^T . P^T takes when MFMA step r multiplies keys 8 (r / 4) +
 // r % 4 and + 4: weights stay in registers, in f32.
 constexpr int kRows32 = 32, kKeys32 = 32;
+// exp of a difference: its rounding before the exponential is below 2^-23 |x|.
+__device__ __forceinline__ float exp32(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// A tile's scores into weights (scale, cap, slope, mask, online softmax); maximum,
+// sum and output follow.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void weigh32(const Packed& p, const Row& row, int k0, int cl, int lg, float16v& st,
+                                        float16v (&o)[2], float& m, float& l) {
+  float mx = -INFINITY;
+  const float icap = 1.f / p.cap;  // (read with a cap alone)
+  const uint32_t seen = cl != 1 ? seen_bits(row, k0) >> (4 * lg) : ~0u;
+#pragma unroll
+  for (int q = 0; q < 16; q++) {
+    const int key = k0 + 8 * (q >> 2) + 4 * lg + (q & 3);
+    float x = st[q] * p.scale;
+    if constexpr (CAP) x = p.cap * tanhf(x * icap);
+    if constexpr (BIAS) x = fmaf(-row.slope, fabsf((float)(row.pos - key)), x);
+    if (cl != 1) x = seen_or(seen, 8 * (q >> 2) + (q & 3), x);
+    st[q] = x;
+    mx = fmaxf(mx, x);
+  }
+  mx = max_xor32(mx);
+  const float mnew = fmaxf(m, mx), mc = mnew == -INFINITY ? 0.f : mnew, alpha = exp32(m - mc);
+  m = mnew;
+  float sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < 16; q++) {
+    st[q] = exp32(st[q] - mc);
+    sum += st[q];
+  }
+  l = l * alpha + sum;
+  if (!__all(alpha == 1.0f)) {
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int q = 0; q < 16; q++) o[e][q] *= alpha;
+  }
+}
+// O += weights . V of one tile, key by key, from memory.
+__device__ __forceinline__ void add_values32(const float* Vb, int64_t vstride, int k0, int lg, int l32, const float16v& st,
+                                             float* kb, float16v (&o)[2]) {
+#pragma unroll
+  for (int q = 0; q < 16; q++) kb[(8 * (q >> 2) + 4 * lg + (q & 3)) * 32 + l32] = st[q];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int j = 0; j < kKeys32; j++) {
+    const float w = kb[j * 32 + l32];
+    if (w == 0.f) continue;  // keys past the document among them
+    const float* vp = Vb + (k0 + j) * vstride + 4 * lg;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int q = 0; q < 16; q++) o[e][q] = fmaf(w, vp[32 * e + 8 * (q >> 2) + (q & 3)], o[e][q]);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void packed_attn_f32(Packed p, Parts part,
                                                                                                int splits) {
@@ -764,34 +822,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     // (the next tile's stores must not overtake these reads)
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    float mx = -INFINITY;
-    const uint32_t seen = cl != 1 ? seen_bits(row, k0) >> (4 * lg) : ~0u;
-#pragma unroll
-    for (int q = 0; q < 16; q++) {
-      const int key = k0 + 8 * (q >> 2) + 4 * lg + (q & 3);
-      float x = st[q] * p.scale;
-      if constexpr (CAP) x = p.cap * tanhf(x / p.cap);
-      if constexpr (BIAS) x = fmaf(-row.slope, fabsf((float)(row.pos - key)), x);
-      if (cl != 1) x = seen_or(seen, 8 * (q >> 2) + (q & 3), x);
-      st[q] = x;
-      mx = fmaxf(mx, x);
-    }
-    mx = max_xor32(mx);
-    const float mnew = fmaxf(m, mx), mc = mnew == -INFINITY ? 0.f : mnew, alpha = expf(m - mc);
-    m = mnew;
-    float sum = 0.f;
-#pragma unroll
-    for (int q = 0; q < 16; q++) {
-      st[q] = expf(st[q] - mc);
-      sum += st[q];
-    }
-    l = l * alpha + sum;
-    if (!__all(alpha == 1.0f)) {
-#pragma unroll
-      for (int e = 0; e < 2; e++)
-#pragma unroll
-        for (int q = 0; q < 16; q++) o[e][q] *= alpha;
-    }
+    weigh32<CAP, BIAS>(p, row, k0, cl, lg, st, o, m, l);
     // A non-finite V must not reach a row whose weight for that key is 0, as 0 *
     // inf in the product would: such a tile is added key by key, zero weights
     // skipped.
@@ -799,22 +830,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
 #pragma unroll
     for (int q = 0; q < 16; q++) fin += v[0][q] * 0.f + v[1][q] * 0.f;
     if (__any(fin != 0.f)) {  // 0 * finite = 0, 0 * (inf or NaN) = NaN
-#pragma unroll
-      for (int q = 0; q < 16; q++) kb[(8 * (q >> 2) + 4 * lg + (q & 3)) * 32 + l32] = st[q];
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-      for (int j = 0; j < kKeys32; j++) {
-        const float w = kb[j * 32 + l32];
-        if (w == 0.f) continue;  // keys past the document among them
-        const float* vp = Vb + (k0 + j) * p.vs[0] + 4 * lg;
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-          for (int q = 0; q < 16; q++) o[e][q] = fmaf(w, vp[32 * e + 8 * (q >> 2) + (q & 3)], o[e][q]);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      add_values32(Vb, p.vs[0], k0, lg, l32, st, kb, o);
       continue;
     }
 #pragma unroll
@@ -862,6 +878,131 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     }
     *(float4v*)(op + 32 * (x >> 4) + 8 * ((x & 15) >> 2) + 4 * lg) = ov;
   }
+}
+
+// 128 rows a block, four waves of 32 that share K and V tiles of 32 keys in a
+// two-buffer LDS ring, for enough blocks to fill the GPU: a quarter of the reads of K
+// and V and of the blocks' set-ups, and no joining.
+__device__ __forceinline__ void dma_piece32(const float* base, int64_t stride, int k0, int piece, int bound, float* dst,
+                                            int lane, bool keys) {
+  const uint64_t a = (uint64_t)(base + (int64_t)k0 * stride);
+  const uint4v rs = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a),
+                     (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu), 0x80000000u, 0x00020000u};
+  // 4 rows of 16 chunks; chunk c of K's row r at c ^ (r & 15) as above, of V's at c ^ 8
+  // in every second group of 4 rows, so that the lane halves' rows meet other banks
+  const int r = piece * 4 + (lane >> 4), c = (lane & 15) ^ (keys ? r & 15 : (r & 4) * 2);
+  const uint32_t off = __umul24(r, (uint32_t)stride) * 4u + (c << 4);
+  const uint32_t lds = (uint32_t)__builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)(dst + piece * 256));
+  buffer_lds16(rs, k0 + r < bound ? off : 0xfffffff0u, lds);
+}
+
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void packed_attn_f32_rows(Packed p, Parts part,
+                                                                                                    int splits) {
+  __shared__ __attribute__((aligned(16))) float Ks[2][kKeys32 * 64];
+  __shared__ __attribute__((aligned(16))) float Vs[2][kKeys32 * 64];
+  __shared__ float weights[4][kKeys32 * 32];
+  const int tid = threadIdx.x, lane = tid & 63, lg = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Hk = p.H / p.G;
+  int slot = blockIdx.x / Hk;
+  const int hk = blockIdx.x - slot * Hk;
+  if (p.causal) slot = (int)(gridDim.x / Hk) - 1 - slot;
+  const int entry = by_g(p, slot), b = p.blocks[2 * entry];
+  if (b < 0) return;  // (the whole block, here and below)
+  const Doc d = packed_doc(p, b);
+  const int t0 = min(max(p.blocks[2 * entry + 1], d.q0), d.q0 + d.nq), rows = min(d.q0 + d.nq - t0, kBlockTokens) * p.G;
+  const int r0 = mod_g(p, slot) * kRowsB, rw0 = r0 + 32 * wave;
+  if (r0 >= rows) return;
+  const int r = rw0 + l32, rc = min(r, rows - 1), t = t0 + by_g(p, rc);
+  auto seen = [&](int q) { return seen_by(p, d, t0 + by_g(p, min(q, rows - 1))); };
+  const Tiles ti = tiles_of<kKeys32>(seen(r0), seen(r0 + kRowsB - 1));
+  const int s = blockIdx.y, i0 = min(s * part.tiles, ti.n), i1 = s + 1 < splits ? min(i0 + part.tiles, ti.n) : ti.n;
+  if (splits > 1 && i0 >= i1) {  // nothing left for this split
+    if (r < rows && lg == 0) part.ml[(int64_t)s * p.Tq * p.H + row_index(p, t, r, hk)] = float2{-INFINITY, 0.f};
+    return;
+  }
+  const float* Kb = (const float*)p.K + hk * p.ks[1];
+  const float* Vb = (const float*)p.V + hk * p.vs[1];
+  auto fetch = [&](int i, int bf) __attribute__((always_inline)) {
+    const int k0 = ti.at<kKeys32>(i);
+#pragma unroll
+    for (int q = 0; q < 2; q++) dma_piece32(Kb, p.ks[0], k0, wave * 2 + q, ti.bound, Ks[bf], lane, true);
+#pragma unroll
+    for (int q = 0; q < 2; q++) dma_piece32(Vb, p.vs[0], k0, wave * 2 + q, ti.bound, Vs[bf], lane, false);
+  };
+  if (i0 < i1) fetch(i0, 0);
+  float4v qf[8];
+  {
+    const float* qp = (const float*)p.Q + t * p.qs[0] + (hk * p.G + mod_g(p, rc)) * p.qs[1] + 4 * lg;
+#pragma unroll
+    for (int i = 0; i < 8; i++) qf[i] = *(const float4v*)(qp + 8 * i);
+  }
+  Row row;
+  static_cast<Seen&>(row) = seen_by(p, d, t);
+  row.f = seen(rw0);
+  row.l = seen(rw0 + 31);
+  row.slope = p.slopes == nullptr ? 0.f : p.slopes[hk * p.G + mod_g(p, rc)];
+  float16v o[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[e][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int at = 0;
+  for (int i = i0; i < i1; i++) {
+    if (i + 1 < i1) fetch(i + 1, at ^ 1);
+    const int k0 = ti.at<kKeys32>(i), cl = rw0 < rows ? tile_class<kKeys32>(row, k0) : 0;
+    if (cl != 0) {
+      const float* kt = Ks[at] + l32 * 64;
+      float16v st;
+#pragma unroll
+      for (int q = 0; q < 16; q++) st[q] = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const float4v kf = *(const float4v*)(kt + (((2 * q + lg) ^ (l32 & 15)) << 2));
+#pragma unroll
+        for (int e = 0; e < 4; e++) st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[q][e], st, 0, 0, 0);
+      }
+      weigh32<CAP, BIAS>(p, row, k0, cl, lg, st, o, m, l);
+      // (row key, column half e ^ lg: the swizzle)
+      const float* vt = Vs[at] + 4 * lg * 64 + l32;
+      float v[2][16], fin = 0.f;
+#pragma unroll
+      for (int q = 0; q < 16; q++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          v[e][q] = vt[(8 * (q >> 2) + (q & 3)) * 64 + 32 * (e ^ lg)];
+          fin = fmaf(v[e][q], 0.f, fin);
+        }
+      if (__any(fin != 0.f)) {
+        add_values32(Vb, p.vs[0], k0, lg, l32, st, weights[wave], o);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 16; q++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) o[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e][q], st[q], o[e], 0, 0, 0);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    at ^= 1;
+    __syncthreads();
+  }
+  const float lt = sum_xor32(l);
+  if (r >= rows) return;
+  const float inv = splits > 1 ? 1.f : lt == 0.f ? 0.f : 1.0f / lt;
+  const int64_t ri = row_index(p, t, r, hk), pr = (int64_t)s * p.Tq * p.H + ri;
+  if (splits > 1 && lg == 0) part.ml[pr] = float2{m, lt};
+  float* op = (splits > 1 ? part.o + pr * 64 : (float*)p.O + ri * 64) + 4 * lg;
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      *(float4v*)(op + 32 * e + 8 * j) =
+          float4v{o[e][4 * j] * inv, o[e][4 * j + 1] * inv, o[e][4 * j + 2] * inv, o[e][4 * j + 3] * inv};
 }
 
 // Joins the parts of split runs: 16 lanes a row, four columns a lane.  E2: scores in
@@ -980,18 +1121,27 @@ static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, in
 
 static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
   const int64_t rows = (int64_t)p.Tq * p.G;
-  const bool f32 = dt == HB_F32, few = f32 || rows <= 64 * (int64_t)p.B;
-  const int per = few ? kRowsF : kRowsB, Hk = p.H / p.G, cus = cu_count(ctx);
+  const bool f32 = dt == HB_F32;
+  const int Hk = p.H / p.G, cus = cu_count(ctx);
+  // Blocks of 32 rows where documents have few, and for f32 where those of 128 would
+  // not go round the CUs (12 heads, 8 documents of up to 400 tokens: 35 us, of 128 rows
+  // 42; 16 heads, 2 of up to 2000, 288 blocks: 281 and 258; 35 of up to 481, windows
+  // with a cap: 143 and 100).
+  const bool few = rows <= 64 * (int64_t)p.B ||
+                   (f32 && std::max<int64_t>((rows + kRowsB - 1) / kRowsB, p.B) * Hk <= cus);
+  const int per = few ? kRowsF : kRowsB;
   // An average document's tiles, and the blocks there are
   const int tile = f32 ? kKeys32 : 64;
   int64_t keys = p.B ? p.Tk / p.B : 0;
   if (p.half >= 0) keys = std::min<int64_t>(keys, 2 * (int64_t)p.half + per / p.G + tile);
   const int64_t tiles = keys / tile, blocks = std::max<int64_t>((rows + per - 1) / per, p.B) * Hk;
   // A run is split where the blocks would leave the GPU short of work: into pieces
-  // of so many tiles that there are `want` of them, at least 8 each, and twice as many
-  // as an average document has (the last piece takes what is left of a longer one).
+  // of so many tiles that there are `want` of them, at least 8 each (24 of 128-row
+  // blocks, where fewer do not pay for writing and joining the parts: 7 documents of up
+  // to 1286 tokens, 16 heads: 47 us in pieces of 8 tiles, 39 whole), and twice as many as
+  // an average document has (the last piece takes what is left of a longer one).
   const int64_t want = (few ? 2 : 4) * (int64_t)cus;
-  Parts part{nullptr, nullptr, (int)std::max<int64_t>(8, blocks * tiles / want)};
+  Parts part{nullptr, nullptr, (int)std::max<int64_t>(few ? 8 : 24, blocks * tiles / want)};
   int splits = (int)std::min<int64_t>(32, (2 * tiles + part.tiles - 1) / part.tiles);
   if (blocks >= want || part.tiles >= tiles) splits = 1;
   CallScratch held(ctx);
@@ -1015,7 +1165,8 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
       else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, (int64_t)p.nblocks * p.G, p, splits, part);
     };
     std::atomic<uint64_t> none{0};
-    if (f32) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, none, 0, slots, p, splits, part);
+    if (f32 && few) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, none, 0, slots, p, splits, part);
+    else if (f32) packed_launch(ctx, packed_attn_f32_rows<CAP, BIAS>, none, 0, (int64_t)p.nblocks * p.G, p, splits, part);
     else if (dt == HB_BF16) half(std::true_type{});
     else half(std::false_type{});
   };

@@ -204,6 +204,17 @@ def test_attention_of_new_tokens(b, dtype, mask):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", range(len(MASKS)))
+def test_attention_of_many_heads(b, dtype, mask):
+    """Blocks enough to go round the CUs, which 128 rows of f32 share then."""
+    opts = dict(MASKS[mask])
+    if "slopes" in opts:
+        opts["slopes"] = opts["slopes"] * 32
+    run_attn(b, dtype, [65, 200, 1, 131, 64], None, 128, 64, 64, mask, **opts)
+    run_attn(b, dtype, [1, 40, 0, 229, 9], [300, 40, 17, 333, 5], 128, 64, 64, mask, **opts)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv,D", [(1, 1, 64), (12, 4, 64), (5, 1, 64), (3, 3, 16), (2, 1, 80), (2, 2, 128), (1, 1, 1),
                                         (2, 2, 65), (1, 1, 512)])
 def test_attention_heads(b, dtype, heads, kv, D):
@@ -240,10 +251,11 @@ def test_attention_rows_behind_the_last_document(b, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
-def test_attention_hidden_keys_hold_anything(b, dtype, what):
+@pytest.mark.parametrize("heads", [2, 150])
+def test_attention_hidden_keys_hold_anything(b, dtype, what, heads):
     """Non-finite keys and values that no mask shows: the finite result."""
     rng = np.random.default_rng(4)
-    q, k, v = (rounded(rng.standard_normal((230, 2, 64)), dtype) for _ in range(3))
+    q, k, v = (rounded(rng.standard_normal((230, heads, 64)), dtype) for _ in range(3))
     hide = [5, 64, 100, 150, 229]
     k[hide], v[hide] = what, what
     # documents of 230 tokens; every row that sees a hidden key is left out of the comparison
