@@ -43,6 +43,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct Score {
   float mul, c1, c2;  // mul: the factor left once a cap or slope has been applied (1), else of the products
   float poly[5], near;  // coefficients of the capped score, and the products they hold for
+  float tiny[3], tiny_near;  // fewer of them, for smaller products
   uint32_t flip;      // a negative scale turns the query round instead
 };
 
@@ -218,8 +219,10 @@ struct Wave {
 // A capped score c2 tanh(c1 x / 2) is c2 - 2 c2 / (1 + 2^(c1 x)) anywhere (c1 in base
 // 2), and where every score of a tile is within 0.75 cap, the odd polynomial of
 // degree 9 through tanh's Chebyshev points there, off by 3.6e-7 at most: 6
-// instructions instead of an exponential and a reciprocal at a quarter of the rate
-// (chunks of 1000 queries over up to 8192 keys: 164 -> 153 us).
+// instructions instead of an exponential and a reciprocal at a lower rate (chunks of
+// 1000 queries over up to 8192 keys: 164 -> 153 us).  Within 0.25 cap that of degree 5,
+// off by 1e-7 at most, does, whose last product is one with the subtraction of the
+// maximum (153 -> 135 us).
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ float score(const Score& s, float slope, int pos, int key, float x) {
   if constexpr (CAP) x = fmaf(-2.f * s.c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * s.c1)), s.c2);
@@ -234,6 +237,11 @@ __device__ __forceinline__ float capped_near(const Score& s, float x) {
   for (int i = 2; i >= 0; i--) r = fmaf(u, r, s.poly[i]);
   return x * r;
 }
+// The factor of x in its capped score, |x| <= tiny_near
+__device__ __forceinline__ float tiny_factor(const Score& s, float x) {
+  const float u = x * x;
+  return fmaf(u, fmaf(u, s.tiny[2], s.tiny[1]), s.tiny[0]);
+}
 static Score score_of(float scale, float cap, bool bias) {
   Score s{};
   // (scale 0: any tiny factor; 0 * -inf would not be a maximum)
@@ -246,9 +254,14 @@ static Score score_of(float scale, float cap, bool bias) {
   // tanh(y) / y in y^2 on [0, 0.75^2]
   const double c[5] = {0.99999942, -0.33328192, 0.13258462, -0.05004161, 0.01291665};
   const double g = capped ? (double)sl / cap : 0.0;
+  const double c3[3] = {0.9999996, -0.33321897, 0.12841434};  // on [0, 0.25^2]
   double f = (double)s.c2 * g;
-  for (int i = 0; i < 5; i++, f *= g * g) s.poly[i] = (float)(f * c[i]);
+  for (int i = 0; i < 5; i++, f *= g * g) {
+    s.poly[i] = (float)(f * c[i]);
+    if (i < 3) s.tiny[i] = (float)(f * c3[i]);
+  }
   s.near = capped ? (float)(0.75 / g) : 0.f;
+  s.tiny_near = capped ? (float)(0.25 / g) : 0.f;
   return s;
 }
 
@@ -301,42 +314,77 @@ __device__ __forceinline__ float max_of(const float16v (&st)[2]) {
     for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[kb][r]);
   return mx;
 }
-// their weights (cap, slope, mask if `mixed`, online softmax).  Weights are rounded
-// to the 16-bit type for the second product, as MFMA takes them, and their sum is of
-// the rounded ones (one dot product a pair),
+// their weights (cap, slope, mask if `mixed`, online softmax).  Weights are relative to
+// w.m, which follows the maximum once it is left behind by a factor of 2^8 for some row
+// of the wave: up to there they fit the 16-bit types as well, and O and the sum need no
+// rescaling.  `top`: no less than the lane's scores; `mx`: their maximum.
+template <class Max>
+__device__ __forceinline__ void follow_maximum(Wave& w, const Score& sc, float top, Max mx) {
+  if (__all(top * sc.mul <= fmaf(w.m, sc.mul, 8.f))) return;
+  const float mnew = fmaxf(w.m, max_xor32(mx())), mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
+  const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc);
+  w.m = mnew;
+  w.l *= alpha;
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) w.o[e][r] *= alpha;
+}
+// Weights are rounded to the 16-bit type for the second product, as MFMA takes them, and
+// their sum is of the rounded ones (one dot product a pair).  exponent(x, mc): a score's
+// distance to mc in base 2
+template <bool BF16, class Exponent>
+__device__ __forceinline__ void wave_exps(Wave& w, const float16v (&st)[2], const Score& sc, uint4v (&pf)[4],
+                                          Exponent exponent) {
+  const float mc = w.m == -INFINITY ? 0.f : w.m * sc.mul;
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    uint32_t pk[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(exponent(st[t >> 1][8 * (t & 1) + e], mc));
+      const float p1 = __builtin_amdgcn_exp2f(exponent(st[t >> 1][8 * (t & 1) + e + 1], mc));
+      pk[e >> 1] = pack2<BF16>(p0, p1);
+      w.l = add_pair<BF16>(pk[e >> 1], w.l);
+    }
+    pf[t] = uint4v{pk[0], pk[1], pk[2], pk[3]};
+  }
+}
 template <bool BF16, bool CAP, bool BIAS>
 __device__ __forceinline__ void wave_weights(Wave& w, float16v (&st)[2], int k0, const Row& row, bool mixed,
                                              const Score& sc, int lg, uint4v (&pf)[4]) {
-  float mx = -INFINITY;
   if constexpr (CAP) {
-    mx = max_of(st);
-    float mn = INFINITY;
+    float far = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) mn = fminf(mn, st[kb][r]);
-    if (__all(mx <= sc.near && mn >= -sc.near)) {
+      for (int r = 0; r < 16; r++) far = fmaxf(far, fabsf(st[kb][r]));
+    if (!BIAS && !mixed && __all(far <= sc.tiny_near)) {
+      auto capped = [&](float x) { return x * tiny_factor(sc, x); };
+      follow_maximum(w, sc, capped(far), [&] { return capped(max_of(st)); });  // (the cap keeps the order)
+      wave_exps<BF16>(w, st, sc, pf, [&](float x, float mc) { return fmaf(x, tiny_factor(sc, x), -mc); });
+      return;
+    }
+    if (__all(far <= sc.near)) {
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
         for (int r = 0; r < 16; r++) st[kb][r] = capped_near(sc, st[kb][r]);
-      mx = capped_near(sc, mx);  // (the maximum's own value: the cap keeps the order)
     } else {
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
         for (int r = 0; r < 16; r++) st[kb][r] = score<true, false>(sc, 0.f, 0, 0, st[kb][r]);
-      mx = score<true, false>(sc, 0.f, 0, 0, mx);
     }
   }
   if constexpr (BIAS) {
+    const float d0 = (float)(row.pos - k0 - 4 * lg);
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * lg + (r & 3);
         const float x = CAP ? st[kb][r] : st[kb][r] * sc.c1;
-        st[kb][r] = fmaf(-row.slope, fabsf((float)(row.pos - key)), x);
+        st[kb][r] = fmaf(-row.slope, fabsf(d0 - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), x);
       }
   }
   if (mixed) {
@@ -347,34 +395,9 @@ __device__ __forceinline__ void wave_weights(Wave& w, float16v (&st)[2], int k0,
       for (int r = 0; r < 16; r++) st[kb][r] = seen_or(seen, 8 * (r >> 2) + (r & 3), st[kb][r]);
     }
   }
-  if (!CAP || BIAS || mixed) mx = max_of(st);
-  mx = max_xor32(mx);
-  // Weights are relative to w.m, which follows the maximum once it is left behind by
-  // a factor of 2^8 for some row of the wave: up to there they fit the 16-bit types
-  // as well, and O and the sum need no rescaling.
-  if (!__all(mx * sc.mul <= fmaf(w.m, sc.mul, 8.f))) {
-    const float mnew = fmaxf(w.m, mx), mc = mnew == -INFINITY ? 0.f : mnew * sc.mul;
-    const float alpha = __builtin_amdgcn_exp2f(w.m * sc.mul - mc);
-    w.m = mnew;
-    w.l *= alpha;
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) w.o[e][r] *= alpha;
-  }
-  const float mc = w.m == -INFINITY ? 0.f : w.m * sc.mul;
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    uint32_t pk[4];
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t >> 1][8 * (t & 1) + e], sc.mul, -mc));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t >> 1][8 * (t & 1) + e + 1], sc.mul, -mc));
-      pk[e >> 1] = pack2<BF16>(p0, p1);
-      w.l = add_pair<BF16>(pk[e >> 1], w.l);
-    }
-    pf[t] = uint4v{pk[0], pk[1], pk[2], pk[3]};
-  }
+  const float mx = max_of(st);
+  follow_maximum(w, sc, mx, [&] { return mx; });
+  wave_exps<BF16>(w, st, sc, pf, [&](float x, float mc) { return fmaf(x, sc.mul, -mc); });
 }
 // and O += weights . V.
 template <bool BF16>
