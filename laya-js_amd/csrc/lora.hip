@@ -57,102 +57,125 @@ struct Prepare {
   void* s;                   // [M, R], of x's type
   Numbers num;
   Codes codes;
-  int br, gx, gy, gz;        // inner products: ranks of a block, row blocks, rank blocks, turns
+  int gx, gy, gz;            // inner products: row blocks, rank blocks, turns
 };
 
-// Inner products.  A block takes 16 MT rows and br ranks; its four waves share out K
-// by 64 and their sums meet in LDS.  The rows' distinct adapters are gone through one
-// after another, for all rows of the block, and a row keeps its own adapter's sums;
-// with few row blocks those are shared out over gz blocks.  f32 rows go through
-// v_mfma_f32_16x16x4: of four k in a lane's registers each product takes one.  Bound by
-// reading x once (and A from the caches); at few rows by the chain of loads, so that a
-// chunk's loads are requested before the last one's products, and by one CU's reading of
-// A, so that blocks take 16 ranks then (48 x 2624, 29 adapters
-// of rank 64: 14.9 -> 8.3 us).  (16k x 1024, rank 64: 24 us of which
-// reading x is 7.)
-template <int DT, int MT>
-__device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int bz, float (*red)[MT * 16][68]) {
-  constexpr int ES = DT == HB_F32 ? 4 : 2, S = ES;  // bytes; 16-byte loads of a lane per 64 k
+// Rows of 128 bytes in LDS, written by direct-to-LDS loads (8 rows a load: 8 lanes a
+// row, so that it reads whole lines; fragments loaded straight into registers, 16 rows
+// by 64 bytes, take a CU's L1 longer: 16k x 1024, rank 64, 24 us against 17; 48 rows x 1024
+// x 2624, 24 adapters of rank 64, 19 against 13 with the projection), read as MFMA fragments: chunk c of
+// row r at c ^ row_f(r), so that the 16 rows of a pass cover all banks.
+__device__ __forceinline__ int row_f(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ uint4v lora_records(const void* p) {
+  const uint64_t a = (uint64_t)p;
+  return uint4v{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a),
+                (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu), 0x80000000u, 0x00020000u};
+}
+// Byte offset of the lane's chunk of piece i of rows of `bytes`, those behind `last`
+// clamped to it
+__device__ __forceinline__ uint32_t piece_offset(int i, int lane, int last, uint32_t bytes) {
+  const int r = i * 8 + (lane >> 3);
+  return (uint32_t)min(r, last) * bytes + (((lane & 7) ^ row_f(r)) << 4);
+}
+__device__ __forceinline__ uint4v row_chunk(const char* rows, int r, int c) {
+  return *(const uint4v*)(rows + r * 128 + ((c ^ row_f(r)) << 4));
+}
+template <int DT>
+__device__ __forceinline__ float4v mfma16(uint4v a, uint4v b, float4v c) {
+  if constexpr (DT == HB_F32) {  // of a lane's four k each product takes one
+    const float4v av = __builtin_bit_cast(float4v, a), bv = __builtin_bit_cast(float4v, b);
+#pragma unroll
+    for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], bv[e], c, 0, 0, 0);
+    return c;
+  } else if constexpr (DT == HB_BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  }
+}
+
+// Inner products.  A block takes 16 MT rows and 16 NT ranks; its four waves share out K
+// by 128 bytes, each through two buffers of its own with no barrier, and their sums meet
+// in LDS.  The rows' distinct adapters are gone through one after another, for all rows
+// of the block, and a row keeps its own adapter's sums; with few row blocks those are
+// shared out over gz blocks.  Bound by reading x once (and A from the caches); at few
+// rows by the chain of loads and one CU's reading of A, so that blocks take 16 ranks
+// then (48 x 2624, 29 adapters of rank 64: 14.9 -> 8.3 us).
+template <int DT, int MT, int NT>
+__device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int bz, char* lds) {
+  constexpr int NW = 4, ES = DT == HB_F32 ? 4 : 2, KC = 128 / ES, BUF = (MT + NT) * 2048, L = 2 * (MT + NT);
+  auto red = (float(*)[MT * 16][NT * 16 + 4])lds;  // [NW], padded against bank conflicts
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int m0 = bx * 16 * MT, r0 = by * p.br, R = p.R, K = p.K;
+  const int m0 = bx * 16 * MT, r0 = by * 16 * NT, R = p.R, K = p.K;
   int a = lane < 16 * MT && m0 + lane < p.M ? p.index[m0 + lane] : -1;
   if (a >= p.n) a = -1;
   uint64_t left = __ballot(a >= 0);
-  const char* xr[MT];
+  uint32_t xo[2 * MT], ao[2 * NT];
 #pragma unroll
-  for (int i = 0; i < MT; i++) xr[i] = p.x + (int64_t)min(m0 + 16 * i + l16, p.M - 1) * p.ldx * ES + 16 * g;
-  const int nt = min((min(R - r0, p.br) + 15) >> 4, 4);  // rank blocks there are
+  for (int i = 0; i < 2 * MT; i++) xo[i] = piece_offset(i, lane, p.M - 1 - m0, (uint32_t)p.ldx * ES);
+#pragma unroll
+  for (int i = 0; i < 2 * NT; i++) ao[i] = piece_offset(i, lane, R - 1 - r0, (uint32_t)K * ES);
+  const uint4v xs = lora_records(p.x + (int64_t)m0 * p.ldx * ES);
+  const char* mine = lds + wave * 2 * BUF;
+  const uint32_t at0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)mine);
   for (int turn = 0; left != 0; turn++) {
     const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
     const uint64_t same = __ballot(a == cur);
     left &= ~same;
     if (turn % p.gz != bz) continue;  // (the same in every wave)
-    const char* ar[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) ar[t] = p.a + ((int64_t)cur * R + min(r0 + 16 * t + l16, R - 1)) * K * ES + 16 * g;
-    float4v acc[MT][4];
+    const float sc = p.scales[cur];
+    const uint4v as = lora_records(p.a + ((int64_t)cur * R + r0) * K * ES);
+    float4v acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int t = 0; t < 4; t++) acc[i][t] = float4v{0.f, 0.f, 0.f, 0.f};
-    struct Chunk {
-      uint4v x[MT][S], a[4][S];
-    } c0, c1;
-    auto load = [&](Chunk& c, int k) __attribute__((always_inline)) {
+      for (int t = 0; t < NT; t++) acc[i][t] = float4v{0.f, 0.f, 0.f, 0.f};
+    auto request = [&](int k, int slot) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the buffer are done
+      const uint32_t to = at0 + (uint32_t)(slot * BUF);
 #pragma unroll
-      for (int s = 0; s < S; s++) {
+      for (int i = 0; i < 2 * MT; i++) buffer_lds16(xs, xo[i], (uint32_t)k * ES, to + 1024u * i);
 #pragma unroll
-        for (int i = 0; i < MT; i++) c.x[i][s] = *(const uint4v*)(xr[i] + (int64_t)k * ES + 64 * s);
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-          if (t < nt) c.a[t][s] = *(const uint4v*)(ar[t] + (int64_t)k * ES + 64 * s);
-      }
+      for (int i = 0; i < 2 * NT; i++) buffer_lds16(as, ao[i], (uint32_t)k * ES, to + 1024u * (2 * MT + i));
     };
-    auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        if (t >= nt) break;
-#pragma unroll
-        for (int s = 0; s < S; s++)
-#pragma unroll
-          for (int i = 0; i < MT; i++) {
-            if constexpr (DT == HB_F32) {
-              const float4v av = __builtin_bit_cast(float4v, c.a[t][s]), xv = __builtin_bit_cast(float4v, c.x[i][s]);
-#pragma unroll
-              for (int e = 0; e < 4; e++) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], xv[e], acc[i][t], 0, 0, 0);
-            } else if constexpr (DT == HB_BF16) {
-              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c.a[t][s]),
-                                                                  __builtin_bit_cast(bf16x8, c.x[i][s]), acc[i][t], 0, 0, 0);
-            } else {
-              acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c.a[t][s]),
-                                                                 __builtin_bit_cast(half8, c.x[i][s]), acc[i][t], 0, 0, 0);
-            }
-          }
+    int slot = 0;
+    if (wave * KC < K) request(wave * KC, 0);
+    for (int k = wave * KC; k < K; k += NW * KC, slot ^= 1) {
+      if (k + NW * KC < K) {
+        request(k + NW * KC, slot ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       }
-    };
-    int k = wave * 64;
-    if (k < K) load(c0, k);
-    for (; k < K; k += 512) {
-      if (k + 256 < K) load(c1, k + 256);
-      multiply(c0);
-      if (k + 256 >= K) break;
-      if (k + 512 < K) load(c0, k + 512);
-      multiply(c1);
+      const char* rows = mine + slot * BUF;
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        uint4v xf[MT], af[NT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) xf[i] = row_chunk(rows, 16 * i + l16, 4 * s + g);
+#pragma unroll
+        for (int t = 0; t < NT; t++) af[t] = row_chunk(rows + MT * 2048, 16 * t + l16, 4 * s + g);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int i = 0; i < MT; i++) acc[i][t] = mfma16<DT>(af[t], xf[i], acc[i][t]);
+      }
     }
+    __syncthreads();  // everybody is done with the buffers
     // lane: row l16 of its block, ranks 16 t + 4 g ..
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int t = 0; t < 4; t++) *(float4v*)&red[wave][16 * i + l16][16 * t + 4 * g] = acc[i][t];
+      for (int t = 0; t < NT; t++) *(float4v*)&red[wave][16 * i + l16][16 * t + 4 * g] = acc[i][t];
     __syncthreads();
-    const float sc = p.scales[cur];
-    for (int q = tid; q < 16 * MT * 16; q += 256) {  // four ranks of a row
-      const int row = q >> 4, r = (q & 15) * 4;
-      if (!((same >> row) & 1) || r >= 16 * nt || r0 + r >= R) continue;  // (R % 4 == 0)
+    for (int q = tid; q < 16 * MT * 4 * NT; q += 64 * NW) {  // four ranks of a row
+      const int row = q / (4 * NT), r = q % (4 * NT) * 4;
+      if (!((same >> row) & 1) || r0 + r >= R) continue;  // (R % 4 == 0)
       float4v v = *(const float4v*)&red[0][row][r];
 #pragma unroll
-      for (int w = 1; w < 4; w++) v += *(const float4v*)&red[w][row][r];
+      for (int w = 1; w < NW; w++) v += *(const float4v*)&red[w][row][r];
       v *= sc;
       const int64_t at = (int64_t)(m0 + row) * R + r0 + r;
       if constexpr (DT == HB_F32) {
@@ -163,7 +186,7 @@ __device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int
         *(uint2v*)((uint16_t*)p.s + at) = uint2v{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
       }
     }
-    __syncthreads();  // the sums are written again
+    __syncthreads();  // the buffers are filled again
   }
 }
 
@@ -208,8 +231,8 @@ __device__ __forceinline__ void lora_number(const Prepare& p, int tile) {
 // 8 codes at a time, four of them requested together.
 template <int QB, bool AFF, bool BF16>
 __device__ __forceinline__ void lora_dequantize(const Codes& c, int block) {
-  const int cpr = c.K >> 3, n = c.N * cpr, step = c.blocks * 256;
-  for (int i0 = block * 256 + (int)threadIdx.x; i0 < n; i0 += 4 * step) {
+  const int threads = blockDim.x, cpr = c.K >> 3, n = c.N * cpr, step = c.blocks * threads;
+  for (int i0 = block * threads + (int)threadIdx.x; i0 < n; i0 += 4 * step) {
     uint32_t w0[4], w1[4], sb[4], zb[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
@@ -233,116 +256,127 @@ __device__ __forceinline__ void lora_dequantize(const Codes& c, int block) {
   }
 }
 
-template <int DT, int MT>
+template <int DT, int MT, int NT>
 __global__ __launch_bounds__(256) void lora_prepare(Prepare p) {
-  __shared__ __attribute__((aligned(16))) float red[4][MT * 16][68];  // 64 ranks, padded against bank conflicts
-  const int b = blockIdx.x, inner = p.gx * p.gy * p.gz;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  int b = blockIdx.x;
+  const int inner = p.gx * p.gy * p.gz;
+  if constexpr (DT != HB_F32) {
+    if (b < p.num.tiles) return lora_number(p, b);
+    b -= p.num.tiles;
+  }
   if (b < inner) {
     const int bx = b % p.gx, q = b / p.gx;
-    return lora_inner<DT, MT>(p, bx, q % p.gy, q / p.gy, red);
+    return lora_inner<DT, MT, NT>(p, bx, q % p.gy, q / p.gy, lds);
   }
   if constexpr (DT != HB_F32) {
     constexpr bool BF16 = DT == HB_BF16;
     const Codes& c = p.codes;
-    const int e = b - inner - p.num.tiles;
-    if (e < 0) lora_number(p, b - inner);
-    else if (c.bits == 8 && c.mode == 0) lora_dequantize<8, false, BF16>(c, e);
-    else if (c.bits == 8) lora_dequantize<8, true, BF16>(c, e);
-    else if (c.mode == 0) lora_dequantize<4, false, BF16>(c, e);
-    else lora_dequantize<4, true, BF16>(c, e);
+    b -= inner;
+    if (c.bits == 8 && c.mode == 0) lora_dequantize<8, false, BF16>(c, b);
+    else if (c.bits == 8) lora_dequantize<8, true, BF16>(c, b);
+    else if (c.mode == 0) lora_dequantize<4, false, BF16>(c, b);
+    else lora_dequantize<4, true, BF16>(c, b);
   }
 }
 
 static void launch_prepare(hipStream_t st, int cus, int dt, Prepare& p) {
-  const int rows = p.M >= 8192 ? 32 : 16;
+  const bool large = p.M >= 8192;
+  const int rows = large ? 64 : 16;
+  auto turns = [&] { return std::max(2, std::min({p.n, rows, cus / (int)std::min<int64_t>((int64_t)p.gx * p.gy, cus)})); };
   p.gx = (p.M + rows - 1) / rows;
-  p.br = 64;
   p.gy = (p.R + 63) / 64;
-  p.gz = std::max(2, std::min({p.n, rows, cus / (int)std::min<int64_t>((int64_t)p.gx * p.gy, cus)}));
-  if ((int64_t)p.gx * p.gy * p.gz < cus) {
-    p.br = 16;
-    p.gy = (p.R + 15) / 16;
-  }
+  p.gz = turns();
+  const bool narrow = p.R <= 16 || (!large && (int64_t)p.gx * p.gy * p.gz < cus);  // 16 ranks a block
+  if (narrow) p.gy = (p.R + 15) / 16;
   const int64_t blocks = (int64_t)p.gx * p.gy * p.gz + p.num.tiles + p.codes.blocks;
   HB_REQUIRE(blocks < (1ll << 31), "hb_lora_linear: too many rows and ranks");
-  auto kernel = rows == 32 ? (dt == HB_F32 ? lora_prepare<HB_F32, 2> : dt == HB_F16 ? lora_prepare<HB_F16, 2> : lora_prepare<HB_BF16, 2>)
-                           : (dt == HB_F32 ? lora_prepare<HB_F32, 1> : dt == HB_F16 ? lora_prepare<HB_F16, 1> : lora_prepare<HB_BF16, 1>);
-  kernel<<<(unsigned)blocks, 256, 0, st>>>(p);
+  auto go = [&](auto kernel, std::atomic<uint64_t>& attr, int mt, int nt) {
+    const int lds = 4 * 2 * (mt + nt) * 2048;
+    if (lds > 64 * 1024)
+      once_per_device(attr, [&] {
+        HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+      });
+    kernel<<<(unsigned)blocks, 256, lds, st>>>(p);
+  };
+  auto type = [&](auto t) {
+    constexpr int DT = decltype(t)::value;
+    static std::atomic<uint64_t> attr[4];
+    if (large && narrow) go(lora_prepare<DT, 4, 1>, attr[0], 4, 1);
+    else if (large) go(lora_prepare<DT, 4, 4>, attr[1], 4, 4);
+    else if (narrow) go(lora_prepare<DT, 1, 1>, attr[2], 1, 1);
+    else go(lora_prepare<DT, 1, 4>, attr[3], 1, 4);
+  };
+  if (dt == HB_F32) type(std::integral_constant<int, HB_F32>{});
+  else if (dt == HB_F16) type(std::integral_constant<int, HB_F16>{});
+  else type(std::integral_constant<int, HB_BF16>{});
 }
 
 // The projection with adapters for few rows: tiles of up to 32 x 32, whose 8 waves share out
-// K, then the adapters' axis (LoraExt), fragments straight from memory into registers,
-// and meet in LDS.  Bound by the chain of loads (the tile's adapters, operands, s and
-// B): a wave's are requested kFewDeep chunks ahead, nothing waits for a barrier
-// before the sums.  K's sum has another order than the other kernels' (a wave per tile
-// in theirs: 12.5 us at the first of these sizes).  Taken up to 5 tiles to 4 CUs (f16;
-// here and on gemm_ring's tiles, with lora_prepare: 48 x 2304 x 768, 24 adapters of rank
-// 16, 10.4 and 15.6 us; 128 x 2304 x 768, 288 tiles, 11.8 and 12.4; 512 x 768 x 1152, 384
-// tiles, 15.0 and 14.6; 128 x 5248 x 1024, 656 tiles, 22 and 18).  The tiles are of 16
-// columns while they leave CUs idle, so that a CU reads less (48 x 1024 x 2624, 24
-// adapters of rank 64: 22.5 -> 19.2 us; 100 x 768 x 1152: 13.4 -> 11.9), and of 16 rows
-// where there are no more.
-constexpr int kFewDeep = 2;
-
+// K, then the adapters' axis (LoraExt), by chunks of 64, each through two buffers of its
+// own with no barrier, and meet in LDS.  Bound by the chain of loads (the tile's
+// adapters, operands, s and B), of which a wave has two chunks' on their way.  K's sum
+// has another order than the other kernels' (a wave per tile in theirs: 12.5 us at the
+// first of these sizes).  Taken up to 2 tiles a CU (f16; here and on gemm_ring's tiles,
+// with lora_prepare: 48 x 2304 x 768, 24 adapters of rank 16, 8.6 and 14.5 us; 256 x 1024
+// x 2624, 256 tiles, 11.5 and 19; 512 x 768 x 1152, 384 tiles, 11.7 and 13.7; 256 x 2304
+// x 768, 576 tiles, 13.8 and 13.3; 128 x 5248 x 1024, 656 tiles, 16.0 and 14.9).  The
+// tiles are of 16 columns while they leave CUs idle, so that a CU reads less (48 x 1024
+// x 2624, 24 adapters of rank 64: 22.5 -> 19.2 us before its loads were of whole lines,
+// 13.3 with them), and of 16 rows where there are no more.
 template <bool BF16, int TM, int TN>
 __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W,
                                                 const uint16_t* __restrict__ bias, uint16_t* __restrict__ Y, int64_t ldy,
                                                 int M, int N, int K, int tiles_m, LoraExt ext) {
-  __shared__ __attribute__((aligned(16))) float red[8][TM * 16][TN * 16 + 4];  // padded against bank conflicts
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  auto red = (float(*)[TM * 16][TN * 16 + 4])lds;  // [8], padded against bank conflicts
   __shared__ int adapter[32];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile = xcd_tile(blockIdx.x, gridDim.x), tn = tile / tiles_m;
   const int m0 = (tile - tn * tiles_m) * TM * 16, n0 = tn * TN * 16, R = ext.R;
   int a = lane < TM * 16 && m0 + lane < M ? ext.index[m0 + lane] : -1;
-  const uint16_t *xr[TM], *wr[TN];
-  int mr[TM], nr[TN];
+  constexpr int BUF = (TM + TN) * 2048, L = 2 * (TM + TN);
+  uint32_t xo[2 * TM], wo[2 * TN];
 #pragma unroll
-  for (int i = 0; i < TM; i++) {
-    mr[i] = min(m0 + 16 * i + l16, M - 1);
-    xr[i] = X + (int64_t)mr[i] * ldx + 8 * g;
-  }
+  for (int i = 0; i < 2 * TM; i++) xo[i] = piece_offset(i, lane, M - 1 - m0, (uint32_t)ldx * 2u);
 #pragma unroll
-  for (int j = 0; j < TN; j++) {
-    nr[j] = min(n0 + 16 * j + l16, N - 1);
-    wr[j] = W + (int64_t)nr[j] * K + 8 * g;
-  }
+  for (int i = 0; i < 2 * TN; i++) wo[i] = piece_offset(i, lane, N - 1 - n0, (uint32_t)K * 2u);
+  const uint4v xs = lora_records(X + (int64_t)m0 * ldx), ws = lora_records(W + (int64_t)n0 * K);
+  const char* buffers = lds + wave * 2 * BUF;
+  const uint32_t at0 = (uint32_t)__builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)buffers);
   float4v acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; i++)
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
-  struct Chunk {  // of 64 k, or of 64 ranks
-    uint4v x[TM][2], w[TN][2];
-  } c[kFewDeep];
-  auto load = [&](Chunk& c, int k) __attribute__((always_inline)) {
+  auto request = [&](int c) __attribute__((always_inline)) {  // chunk wave + 8 c of K
+    const uint32_t to = at0 + (uint32_t)((c & 1) * BUF), k = (uint32_t)(wave + 8 * c) * 128u;
+#pragma unroll
+    for (int i = 0; i < 2 * TM; i++) buffer_lds16(xs, xo[i], k, to + 1024u * i);
+#pragma unroll
+    for (int j = 0; j < 2 * TN; j++) buffer_lds16(ws, wo[j], k, to + 1024u * (2 * TM + j));
+  };
+  auto multiply = [&](int c) __attribute__((always_inline)) {
+    const char* rows = buffers + (c & 1) * BUF;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
+      uint4v xf[TM], wf[TN];
 #pragma unroll
-      for (int i = 0; i < TM; i++) c.x[i][s] = *(const uint4v*)(xr[i] + k + 32 * s);
+      for (int i = 0; i < TM; i++) xf[i] = row_chunk(rows, 16 * i + l16, 4 * s + g);
 #pragma unroll
-      for (int j = 0; j < TN; j++) c.w[j][s] = *(const uint4v*)(wr[j] + k + 32 * s);
-    }
-  };
-  auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int s = 0; s < 2; s++)
+      for (int j = 0; j < TN; j++) wf[j] = row_chunk(rows + TM * 2048, 16 * j + l16, 4 * s + g);
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-          if constexpr (BF16)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c.w[j][s]),
-                                                                __builtin_bit_cast(bf16x8, c.x[i][s]), acc[i][j], 0, 0, 0);
-          else
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c.w[j][s]),
-                                                               __builtin_bit_cast(half8, c.x[i][s]), acc[i][j], 0, 0, 0);
-        }
+        for (int j = 0; j < TN; j++) acc[i][j] = mfma16<BF16 ? HB_BF16 : HB_F16>(wf[j], xf[i], acc[i][j]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the buffer is requested again)
   };
-  const int k0 = wave * 64;
-#pragma unroll
-  for (int b = 0; b < kFewDeep; b++)
-    if (k0 + 512 * b < K) load(c[b], k0 + 512 * b);
+  const int kc = (K / 64 - wave + 7) / 8;  // this wave's chunks of K, from 0 on
+  if (kc > 0) request(0);
+  if (kc > 1) request(1);
   // the tile's adapters by number, as they first occur: lane o has number o's
   if (a >= ext.n) a = -1;
   int num = -1, mine = 0, nd = 0;
@@ -354,47 +388,48 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
     mine = lane == nd ? cur : mine;
   }
   if (tid < 32) adapter[tid] = mine;
-  int xnum[TM];
-#pragma unroll
-  for (int i = 0; i < TM; i++) xnum[i] = __shfl(num, 16 * i + l16);
   const int r8 = R >> 3, chunks = (nd * r8 + 7) >> 3;  // chunks of 8 ranks of an adapter; chunks of 64 ranks
+  const int ec = (chunks - wave + 7) / 8;              // this wave's of those, numbered from kc on
   const float inv8 = 8.f / (float)R;
-  auto load_ranks = [&](Chunk& c, int e) __attribute__((always_inline)) {
+  const uint4v ss = lora_records(ext.s), bs = lora_records(ext.b);
+  int xnum[2 * TM];  // of the rows of the lane's pieces
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      const int ch = e * 8 + s * 4 + g, o = (int)(((float)ch + 0.5f) * inv8), r = (ch - o * r8) * 8;
-      const int who = __shfl(mine, o & 31);
+  for (int i = 0; i < 2 * TM; i++) xnum[i] = __shfl(num, 8 * i + (lane >> 3));
+  auto request_ranks = [&](int c) __attribute__((always_inline)) {
+    const uint32_t to = at0 + (uint32_t)((c & 1) * BUF);
+    auto piece = [&](int i, auto rows) __attribute__((always_inline)) {  // of i's rows
+      const int r = i * 8 + (lane >> 3), ch = (wave + 8 * (c - kc)) * 8 + ((lane & 7) ^ row_f(r));
+      const int o = (int)(((float)ch + 0.5f) * inv8);
+      rows(r, o, (uint32_t)(ch - o * r8) * 8u);
+    };
+    // past the records: zeros
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        c.x[i][s] = uint4v{0u, 0u, 0u, 0u};
-        if (o == xnum[i]) c.x[i][s] = *(const uint4v*)(ext.s + (int64_t)mr[i] * R + r);
-      }
+    for (int i = 0; i < 2 * TM; i++)
+      piece(i, [&](int r, int o, uint32_t rank) {
+        buffer_lds16(ss, o == xnum[i] ? ((uint32_t)min(m0 + r, M - 1) * (uint32_t)R + rank) * 2u : 0xfffffff0u, to + 1024u * i);
+      });
 #pragma unroll
-      for (int j = 0; j < TN; j++) {
-        c.w[j][s] = uint4v{0u, 0u, 0u, 0u};
-        if (o < nd) c.w[j][s] = *(const uint4v*)(ext.b + ((int64_t)who * N + nr[j]) * R + r);
-      }
-    }
+    for (int j = 0; j < 2 * TN; j++)
+      piece(j, [&](int r, int o, uint32_t rank) {
+        const uint32_t who = (uint32_t)__shfl(mine, o & 31), n = (uint32_t)min(n0 + r, N - 1);
+        buffer_lds16(bs, o < nd ? ((who * (uint32_t)N + n) * (uint32_t)R + rank) * 2u : 0xfffffff0u,
+                     to + 1024u * (2 * TM + j));
+      });
   };
-  for (int k = k0; k < K; k += 512 * kFewDeep) {
-#pragma unroll
-    for (int b = 0; b < kFewDeep; b++) {
-      if (k + 512 * b >= K) break;
-      multiply(c[b]);
-      if (k + 512 * (b + kFewDeep) < K) load(c[b], k + 512 * (b + kFewDeep));
-    }
+  const int all = max(kc, 0) + max(ec, 0);
+  auto ask = [&](int c) __attribute__((always_inline)) {
+    if (c < kc) request(c);
+    else request_ranks(c);
+  };
+  if (max(kc, 0) < 1 && all > 0) ask(0);
+  if (max(kc, 0) < 2 && all > 1) ask(1);
+  for (int c = 0; c < all; c++) {
+    if (c + 1 < all) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    multiply(c);
+    if (c + 2 < all) ask(c + 2);
   }
-#pragma unroll
-  for (int b = 0; b < kFewDeep; b++)
-    if (wave + 8 * b < chunks) load_ranks(c[b], wave + 8 * b);
-  for (int e = wave; e < chunks; e += 8 * kFewDeep) {
-#pragma unroll
-    for (int b = 0; b < kFewDeep; b++) {
-      if (e + 8 * b >= chunks) break;
-      multiply(c[b]);
-      if (e + 8 * (b + kFewDeep) < chunks) load_ranks(c[b], e + 8 * (b + kFewDeep));
-    }
-  }
+  __syncthreads();  // everybody is done with the buffers
   // lane: row 16 i + l16, columns 16 j + 4 g ..
 #pragma unroll
   for (int i = 0; i < TM; i++)
@@ -431,7 +466,7 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
 // the outputs go from registers to memory (the lane halves exchange 4 columns, so that
 // a lane stores 8 of a row) while those loads are on their way.  On gemm_ring's blocks
 // of one tile each the same tiles took 269 us, its tiles of 128 x 256 338.
-// What bounds it: 242 us with lora_prepare's 24; without the loads into LDS 197, without
+// What bounds it (242 us with lora_prepare, then 24): without the loads into LDS 197, without
 // the fragment reads too 187: the products alone, at the clock that the card holds under
 // them, and behind them the 32 KB per stage from the L2.
 // Of its numbering only whole-wave scalars are read, by scalar loads (kept in their
@@ -721,14 +756,19 @@ static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, c
     return;
   }
   const int64_t few = (int64_t)((M + 31) / 32) * ((N + 31) / 32);
-  if (4 * few <= 5 * cus) {
-    auto run = [&](auto kernel, int bm, int bn) {
-      const int tm = (M + bm - 1) / bm;
-      kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), 512, 0, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, ext);
+  if (few <= 2 * cus) {
+    auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn) {
+      const int tm = (M + bm - 1) / bm, lds = 8 * 2 * (bm + bn) * 128;
+      if (lds > 64 * 1024)
+        once_per_device(attr, [&] {
+          HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        });
+      kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), 512, lds, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, ext);
     };
+    static std::atomic<uint64_t> attr[4];
     const bool half = 2 * few <= cus;
-    if (M <= 16) half ? run(lora_few<BF16, 1, 1>, 16, 16) : run(lora_few<BF16, 1, 2>, 16, 32);
-    else half ? run(lora_few<BF16, 2, 1>, 32, 16) : run(lora_few<BF16, 2, 2>, 32, 32);
+    if (M <= 16) half ? run(lora_few<BF16, 1, 1>, attr[0], 16, 16) : run(lora_few<BF16, 1, 2>, attr[1], 16, 32);
+    else half ? run(lora_few<BF16, 2, 1>, attr[2], 32, 16) : run(lora_few<BF16, 2, 2>, attr[3], 32, 32);
     return;
   }
   auto go = [&](auto launch) { launch(st, 0u, x, ldx, w, bias, (const uint16_t*)nullptr, (int64_t)0, y, ldy, M, N, K, ext); };
@@ -863,7 +903,7 @@ static bool lora_takes_ring(int dt, uintptr_t x, int64_t ldx, uintptr_t w, uintp
                             int64_t K, const LoraArgs& l) {
   return (dt == HB_F16 || dt == HB_BF16) && M > 0 && N > 0 && K > 0 && l.n > 0 && l.R > 0 && ring_ok(ldx, K) &&
          l.R % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && (x | w | y | l.a | l.b) % 16 == 0 &&
-         l.n * l.R * N * 2 < (1ll << 31) && M * l.R * 2 < (1ll << 31) && ldy < (1 << 22);
+         l.n * l.R * N * 2 < (1ll << 31) && M * l.R * 2 < (1ll << 31) && K < (1 << 22) && ldx < (1 << 22) && ldy < (1 << 22);
 }
 
 // The projection with adapters on 16-bit weights w, or on quantized ones (`codes`);
@@ -906,7 +946,7 @@ static void add_adapters(uintptr_t ctx, const char* op, int dt, uintptr_t x, int
   if (!s.take((size_t)(M * l.R * 4)))
     throw std::runtime_error(std::string(op) + ": out of device memory for the adapters' inner products");
   hipStream_t st = stream_of(ctx);
-  if (dt == HB_F32 && K % 64 == 0 && N % 4 == 0 && l.R % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 &&
+  if (dt == HB_F32 && K % 32 == 0 && N % 4 == 0 && l.R % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && K < (1 << 22) && ldx < (1 << 22) &&
       (x | y | l.a | l.b) % 16 == 0 && (M + 31) / 32 < 65536) {
     Prepare p{(const char*)x, ldx, (const char*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, (int)M,
               (int)l.R, (int)K};
