@@ -312,7 +312,7 @@ static void launch_prepare(hipStream_t st, int cus, int dt, Prepare& p) {
   else type(std::integral_constant<int, HB_BF16>{});
 }
 
-// The projection with adapters for few rows: tiles of up to 32 x 32, whose 8 waves share out
+// The projection with adapters for few rows: tiles of up to 32 x 32, whose NW waves share out
 // K, then the adapters' axis (LoraExt), by chunks of 64, each through two buffers of its
 // own with no barrier, and meet in LDS.  Bound by the chain of loads (the tile's
 // adapters, operands, s and B), of which a wave has two chunks' on their way.  K's sum
@@ -323,14 +323,16 @@ static void launch_prepare(hipStream_t st, int cus, int dt, Prepare& p) {
 // x 768, 576 tiles, 13.8 and 13.3; 128 x 5248 x 1024, 656 tiles, 16.0 and 14.9).  The
 // tiles are of 16 columns while they leave CUs idle, so that a CU reads less (48 x 1024
 // x 2624, 24 adapters of rank 64: 22.5 -> 19.2 us before its loads were of whole lines,
-// 13.3 with them), and of 16 rows where there are no more.
-template <bool BF16, int TM, int TN>
-__global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W,
+// 13.3 with them), and of 16 rows where there are no more.  Tiles of 64 x 64 take over while
+// they go round the CUs once (400 x 2304 x 768, 252 tiles: 12.9 us, gemm_ring's 14.2; 1200 x
+// 1024 x 1024, 304 tiles: 20.3 and 15.6).
+template <bool BF16, int TM, int TN, int NW>
+__global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W,
                                                 const uint16_t* __restrict__ bias, uint16_t* __restrict__ Y, int64_t ldy,
                                                 int M, int N, int K, int tiles_m, LoraExt ext) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  auto red = (float(*)[TM * 16][TN * 16 + 4])lds;  // [8], padded against bank conflicts
-  __shared__ int adapter[32];
+  auto red = (float(*)[TM * 16][TN * 16 + 4])lds;  // [NW], padded against bank conflicts
+  __shared__ int adapter[TM * 16];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile = xcd_tile(blockIdx.x, gridDim.x), tn = tile / tiles_m;
@@ -352,7 +354,7 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
   auto request = [&](int c) __attribute__((always_inline)) {  // chunk wave + 8 c of K
-    const uint32_t to = at0 + (uint32_t)((c & 1) * BUF), k = (uint32_t)(wave + 8 * c) * 128u;
+    const uint32_t to = at0 + (uint32_t)((c & 1) * BUF), k = (uint32_t)(wave + NW * c) * 128u;
 #pragma unroll
     for (int i = 0; i < 2 * TM; i++) buffer_lds16(xs, xo[i], k, to + 1024u * i);
 #pragma unroll
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the buffer is requested again)
   };
-  const int kc = (K / 64 - wave + 7) / 8;  // this wave's chunks of K, from 0 on
+  const int kc = (K / 64 - wave + NW - 1) / NW;  // this wave's chunks of K, from 0 on
   if (kc > 0) request(0);
   if (kc > 1) request(1);
   // the tile's adapters by number, as they first occur: lane o has number o's
@@ -387,9 +389,9 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
     num = a == cur ? nd : num;
     mine = lane == nd ? cur : mine;
   }
-  if (tid < 32) adapter[tid] = mine;
+  if (tid < TM * 16) adapter[tid] = mine;
   const int r8 = R >> 3, chunks = (nd * r8 + 7) >> 3;  // chunks of 8 ranks of an adapter; chunks of 64 ranks
-  const int ec = (chunks - wave + 7) / 8;              // this wave's of those, numbered from kc on
+  const int ec = (chunks - wave + NW - 1) / NW;              // this wave's of those, numbered from kc on
   const float inv8 = 8.f / (float)R;
   const uint4v ss = lora_records(ext.s), bs = lora_records(ext.b);
   int xnum[2 * TM];  // of the rows of the lane's pieces
@@ -398,7 +400,7 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
   auto request_ranks = [&](int c) __attribute__((always_inline)) {
     const uint32_t to = at0 + (uint32_t)((c & 1) * BUF);
     auto piece = [&](int i, auto rows) __attribute__((always_inline)) {  // of i's rows
-      const int r = i * 8 + (lane >> 3), ch = (wave + 8 * (c - kc)) * 8 + ((lane & 7) ^ row_f(r));
+      const int r = i * 8 + (lane >> 3), ch = (wave + NW * (c - kc)) * 8 + ((lane & 7) ^ row_f(r));
       const int o = (int)(((float)ch + 0.5f) * inv8);
       rows(r, o, (uint32_t)(ch - o * r8) * 8u);
     };
@@ -411,7 +413,7 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
 #pragma unroll
     for (int j = 0; j < 2 * TN; j++)
       piece(j, [&](int r, int o, uint32_t rank) {
-        const uint32_t who = (uint32_t)__shfl(mine, o & 31), n = (uint32_t)min(n0 + r, N - 1);
+        const uint32_t who = (uint32_t)__shfl(mine, o & 63), n = (uint32_t)min(n0 + r, N - 1);
         buffer_lds16(bs, o < nd ? ((who * (uint32_t)N + n) * (uint32_t)R + rank) * 2u : 0xfffffff0u,
                      to + 1024u * (2 * TM + j));
       });
@@ -437,25 +439,27 @@ __global__ __launch_bounds__(512) void lora_few(const uint16_t* __restrict__ X, 
     for (int j = 0; j < TN; j++) *(float4v*)&red[wave][16 * i + l16][16 * j + 4 * g] = acc[i][j];
   __syncthreads();
   constexpr int CW = TN * 8;  // threads of a row
-  const int row = tid / CW, col = tid % CW * 2, m = m0 + row, n = n0 + col;
-  if (row >= TM * 16 || m >= M || n >= N) return;
-  float v[2] = {0.f, 0.f};
+  for (int at = tid; at < TM * 16 * CW; at += NW * 64) {
+    const int row = at / CW, col = at % CW * 2, m = m0 + row, n = n0 + col;
+    if (m >= M || n >= N) continue;
+    float v[2] = {0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < 8; w++)
+    for (int w = 0; w < NW; w++)
 #pragma unroll
-    for (int q = 0; q < 2; q++) v[q] += red[w][row][col + q];
-  uint16_t o[2];
+      for (int q = 0; q < 2; q++) v[q] += red[w][row][col + q];
+    uint16_t o[2];
 #pragma unroll
-  for (int q = 0; q < 2; q++) {
-    const int nq = min(n + q, N - 1);
-    o[q] = from_f<BF16>(v[q] + (bias != nullptr ? to_f<BF16>(bias[nq]) : 0.f));
-    // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf)
-    if (v[q] * 0.f != 0.f && lora_mixed<BF16>(ext, adapter, nd, N, m, nq))
-      o[q] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, nq);
+    for (int q = 0; q < 2; q++) {
+      const int nq = min(n + q, N - 1);
+      o[q] = from_f<BF16>(v[q] + (bias != nullptr ? to_f<BF16>(bias[nq]) : 0.f));
+      // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf)
+      if (v[q] * 0.f != 0.f && lora_mixed<BF16>(ext, adapter, nd, N, m, nq))
+        o[q] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, nq);
+    }
+    uint16_t* y = Y + (int64_t)m * ldy + n;
+    if (n + 1 < N) *(uint32_t*)y = (uint32_t)o[0] | ((uint32_t)o[1] << 16);
+    else y[0] = o[0];
   }
-  uint16_t* y = Y + (int64_t)m * ldy + n;
-  if (n + 1 < N) *(uint32_t*)y = (uint32_t)o[0] | ((uint32_t)o[1] << 16);
-  else y[0] = o[0];
 }
 
 // The projection with adapters for large M: 256 x 256 tiles, 8 waves of 128 x 64 (6
@@ -755,22 +759,23 @@ static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, c
                                                                                        K, tm, tn, ext, num);
     return;
   }
-  const int64_t few = (int64_t)((M + 31) / 32) * ((N + 31) / 32);
-  if (few <= 2 * cus) {
-    auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn) {
-      const int tm = (M + bm - 1) / bm, lds = 8 * 2 * (bm + bn) * 128;
-      if (lds > 64 * 1024)
-        once_per_device(attr, [&] {
-          HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        });
-      kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), 512, lds, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, ext);
-    };
-    static std::atomic<uint64_t> attr[4];
-    const bool half = 2 * few <= cus;
-    if (M <= 16) half ? run(lora_few<BF16, 1, 1>, attr[0], 16, 16) : run(lora_few<BF16, 1, 2>, attr[1], 16, 32);
-    else half ? run(lora_few<BF16, 2, 1>, attr[2], 32, 16) : run(lora_few<BF16, 2, 2>, attr[3], 32, 32);
+  auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn, int nw) {
+    const int tm = (M + bm - 1) / bm, lds = nw * 2 * (bm + bn) * 128;
+    if (lds > 64 * 1024)
+      once_per_device(attr, [&] {
+        HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+      });
+    kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), nw * 64, lds, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, ext);
+  };
+  static std::atomic<uint64_t> attr[5];
+  auto tiles = [&](int t) { return (int64_t)((M + t - 1) / t) * ((N + t - 1) / t); };
+  const bool half = 2 * tiles(32) <= cus;
+  if (tiles(32) <= 2 * cus) {
+    if (M <= 16) half ? run(lora_few<BF16, 1, 1, 8>, attr[0], 16, 16, 8) : run(lora_few<BF16, 1, 2, 8>, attr[1], 16, 32, 8);
+    else half ? run(lora_few<BF16, 2, 1, 8>, attr[2], 32, 16, 8) : run(lora_few<BF16, 2, 2, 8>, attr[3], 32, 32, 8);
     return;
   }
+  if (tiles(64) <= cus) return run(lora_few<BF16, 4, 4, 4>, attr[4], 64, 64, 4);
   auto go = [&](auto launch) { launch(st, 0u, x, ldx, w, bias, (const uint16_t*)nullptr, (int64_t)0, y, ldy, M, N, K, ext); };
   LinearKernel tile = LinearKernel::kRing64x64x3;
   ring_tile(cus, M, N, K, false, true, false, &tile);

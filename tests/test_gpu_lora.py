@@ -73,7 +73,8 @@ def check(got, c, dtype, w=None):
 
 SIZES = [(1, 64, 64, 1, 8), (48, 2304, 768, 24, 16), (1, 1, 1, 1, 1), (5, 33, 70, 3, 4), (130, 200, 192, 4, 64),
          (300, 768, 1152, 5, 8), (64, 256, 128, 64, 32), (17, 100, 64, 2, 3), (200, 72, 256, 3, 100), (4100, 192, 128, 6, 16),
-         (33, 520, 64, 40, 72), (700, 1024, 1024, 2, 24), (129, 130, 136, 2, 8), (1000, 640, 320, 3, 128)]
+         (33, 520, 64, 40, 72), (700, 1024, 1024, 2, 24), (129, 130, 136, 2, 8), (1000, 640, 320, 3, 128), (410, 2304, 192, 30, 24), (130, 5250, 64, 100, 8),
+         (400, 2304, 768, 5, 64), (1500, 768, 320, 9, 16)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
