@@ -1159,12 +1159,18 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
   if (p.half >= 0) keys = std::min<int64_t>(keys, 2 * (int64_t)p.half + per / p.G + tile);
   const int64_t tiles = keys / tile, blocks = std::max<int64_t>((rows + per - 1) / per, p.B) * Hk;
   // A run is split where the blocks would leave the GPU short of work: into pieces
-  // of so many tiles that there are `want` of them, at least 8 each (24 of 128-row
-  // blocks, where fewer do not pay for writing and joining the parts: 7 documents of up
-  // to 1286 tokens, 16 heads: 47 us in pieces of 8 tiles, 39 whole), and twice as many as
-  // an average document has (the last piece takes what is left of a longer one).
-  const int64_t want = (few ? 2 : 4) * (int64_t)cus;
-  Parts part{nullptr, nullptr, (int)std::max<int64_t>(few ? 8 : 24, blocks * tiles / want)};
+  // of so many tiles that there are `want` of them, at least `least` each, since fewer do
+  // not pay for writing and joining the parts, and twice as many as an average document
+  // has (the last piece takes what is left of a longer one).
+  // 128-row blocks: 7 documents of up to 1286 tokens, 16 heads, 47 us in pieces of 8
+  // tiles, 39 whole.  32-row blocks, whose waves share out the tiles anyway: a token each
+  // of 48 documents of up to 4096, 192 blocks, 40.5 in 6 pieces, 36.5 whole; 8 such
+  // documents, 32 blocks, 24.9 whole, 20.2 in 3; 16 tokens each of 16, 128 blocks, 25.9
+  // whole, 32.7 in 6.  f32, whose tiles take longer: a token each of 11 of up to 1605, 16
+  // heads, 46.7 whole, 37.8 in 4 pieces, 47.2 in 7.
+  const int64_t want = f32 && few ? 2 * (int64_t)cus : few ? cus / 2 : 4 * (int64_t)cus;
+  const int64_t least = f32 && few ? 16 : few ? 32 : 24;
+  Parts part{nullptr, nullptr, (int)std::max<int64_t>(least, blocks * tiles / want)};
   int splits = (int)std::min<int64_t>(32, (2 * tiles + part.tiles - 1) / part.tiles);
   if (blocks >= want || part.tiles >= tiles) splits = 1;
   CallScratch held(ctx);

@@ -230,6 +230,14 @@ def test_attention_long(b, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_attention_in_pieces(b, dtype):
+    """Runs long enough, and blocks few enough, for them to be split and joined."""
+    run_attn(b, dtype, [300, 200], [5000, 4100], 2, 1, 64, 13, causal=True, prefix=[130, 64], cap=20.0)
+    run_attn(b, dtype, [300, 0, 20], [4900, 70, 4111], 2, 2, 64, 14)
+    run_attn(b, dtype, [400, 100], [2600, 1500], 64, 64, 64, 15, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_many_documents(b, dtype):
     rng = np.random.default_rng(8)
     n = rng.integers(0, 9, 700).tolist()
