@@ -6,14 +6,15 @@
 // with a bank of n adapters A [n, R, K], B [n, N, R]; a row whose index is
 // outside [0, n) has none.
 //
-// lora_prepare: s = scale_i x_m . A_i^T of f16 / bf16 rows on v_mfma_f32_16x16x32,
-// rounded to the 16-bit type for the second product, which the projection's own
-// GEMM takes as ranks beyond K (gemm_ring with LoraExt, or lora_stream for large
-// M): y is rounded once.
+// lora_prepare: s = scale_i x_m . A_i^T on v_mfma_f32_16x16x32 (f32: 16x16x4).  Of f16 /
+// bf16 rows it is rounded to the 16-bit type for the second product, which the
+// projection's own GEMM takes as ranks beyond K: gemm_ring with LoraExt, lora_stream
+// for large M, lora_few for few tiles.  y is rounded once.
 //
-// lora_shrink_any, lora_expand_any: the inner products s = scale_i x_m . A_i^T
-// in f32, then y = round(y + s . B_i^T) on top of the projection, any type and
-// size.
+// lora_expand_f32: y += s . B_i^T of f32 rows, on top of the projection.
+//
+// lora_shrink_any, lora_expand_any: the inner products in f32, then y = round(y + s .
+// B_i^T), any type and size.
 #include <algorithm>
 #include <stdexcept>
 

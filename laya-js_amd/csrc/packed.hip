@@ -25,7 +25,7 @@ namespace hb {
 // offsets in LDS; block 0 also writes the offsets, and the last block the end of the
 // table.  Scanning B lengths again in each block costs less than a second launch
 // would (B / 1024 rounds of one 16-byte read a thread); what bounds it is the
-// launch itself, then the 12 bytes written a token.
+// launch itself, then the 12 bytes written a token (3 us for 300 tokens, 5 for 37k).
 constexpr int kPlanDocs = 1024, kPlanTokens = 1024;
 
 // Exclusive sums over the block's 256 threads, and their total.
@@ -125,7 +125,8 @@ __global__ __launch_bounds__(256) void pack_plan_kernel(const int32_t* __restric
 // ------------------------------------------------------------------ rows
 
 // Moves whole rows, one wave each: the row's source index is the same in all
-// lanes, which take its vectors in turn.  Bound by reading and writing the rows.
+// lanes, which take its vectors in turn.  Bound by reading and writing the rows (64 x
+// 1024 x 1024 in f16: 37 us, 5 TB/s with what the caches hold).
 // UNPACK: row b * L + l of the padded batch is row off_b + l of the packed one;
 // else row t of the packed batch is row idx[t] of the padded one.  Rows without
 // a source are zeros.
@@ -190,7 +191,8 @@ __device__ __forceinline__ float2 rope_at_cs(const RopeAt& f, const int32_t* pos
 // all heads, and rotates the chunk pairs (c, c + D / 2) of its heads, four loads
 // of a thread in flight.  Bound by reading and writing the heads; a sine and
 // cosine in f64 cost a block about as much as 16 KB of traffic, so TB tokens
-// share a block where there are enough of them.
+// share a block where there are enough of them (32768 rows x 32 heads on three axes, bf16:
+// 60 us, 4.5 TB/s; a block a token: 226).
 constexpr int kRopeTokens = 8;  // 256 threads: one angle each at D = 64
 template <class T, int V, bool BF16>
 __device__ __forceinline__ void rope_load(const T* p, float (&v)[V]) {

@@ -161,7 +161,7 @@ def test_lora_adapters_do_not_reach_other_rows(b, dtype, what):
 # sizes whose tiles of 256 x 256 go round the CUs: K of two stages, edges in both
 # directions, tiles without and of many adapters, ranks that end inside a stage
 LARGE = [(8200, 1032, 64, 5, 8), (4099, 2056, 128, 40, 72), (520, 16392, 64, 2, 16), (4096, 2304, 192, 3, 64),
-         (33000, 256, 64, 90, 24), (1, 65544, 64, 2, 8)]
+         (33000, 256, 64, 90, 24), (1, 65544, 64, 2, 8), (4200, 2056, 64, 2, 520), (300, 520, 64, 3, 1024), (257, 16384, 64, 3, 8)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -174,6 +174,26 @@ def test_lora_large(b, dtype, M, N, K, n, R):
     x, bank, index, bias = dev(b, c, dtype)
     w = b.fromHost(to_host(c["w"], dtype))
     check(read32(b, b.loraLinear(x, w, bank, index, bias)), c, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N", [(40, 136), (500, 264), (4100, 2056)])
+def test_lora_wide_rows(b, dtype, M, N):
+    """Rows of x inside wider ones, a bias that is not on a 16-byte boundary, adapter
+    numbers of any value: the values of plain operands, which another kernel may sum
+    in another order: both off by half a step, and by 2^-23 of sums of 8 at most in each of
+    144 additions."""
+    rng = np.random.default_rng(M)
+    c = case(rng, dtype, M, N, 128, 4, 8, index=np.arange(M) // 30 % 5 - 1, bias=True)
+    x, bank, index, bias = dev(b, c, dtype)
+    w = b.fromHost(to_host(c["w"], dtype))
+    want = read32(b, b.loraLinear(x, w, bank, index, bias))
+    check(want, c, dtype)
+    wide = b.fromHost(to_host(np.concatenate([np.full_like(c["x"], np.nan), c["x"]], 1), dtype))
+    off = b.slice(b.fromHost(to_host(np.concatenate([[1.0], c["bias"]]), dtype)), [1], [N + 1])
+    far = np.where(c["index"] < 0, np.where(np.arange(M) % 2, -2 ** 31, 2 ** 31 - 1), c["index"])
+    got = read32(b, b.loraLinear(b.slice(wide, [0, 128], [M, 256]), w, bank, i32(b, far), off))
+    np.testing.assert_allclose(got, want, rtol=2 * U[dtype], atol=(128 + 16) * 2.0 ** -22 * 8)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])

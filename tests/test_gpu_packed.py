@@ -381,6 +381,19 @@ def _model(b, dtype, seed=0):
 
 
 # f32: sums in another order, a few 1e-6 after four layers of values up to 5; f16:
+def test_encode_packed_of_nothing(b):
+    """No documents, and documents without tokens."""
+    enc, _ = _model(b, "f16")
+    for docs in ([], [[]], [[], [1, 2, 3], []]):
+        inp = enc.uploadPacked(docs, adapters=[0] * len(docs), padded=4)
+        y = enc.encodePacked(inp)
+        assert y.shape == (sum(map(len, docs)), enc.config.hiddenSize) and np.isfinite(read32(b, y)).all()
+        rows = read32(b, b.unpackRows(y, inp["docs"]))
+        assert rows.shape == (len(docs), 4, enc.config.hiddenSize)
+        enc.disposePacked(inp)
+        b.dispose(y)
+
+
 # both forwards round every op, 2^-11 of values up to 8 at 30 places, in
 # quadrature 2e-2, doubled
 @pytest.mark.parametrize("dtype,tol", [("f32", 1e-4), ("f16", 4e-2)])
