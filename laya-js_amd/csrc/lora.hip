@@ -463,7 +463,8 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__
   }
 }
 
-// The projection with adapters for large M: 256 x 256 tiles, 8 waves of 128 x 64 (6
+// The projection with adapters for large M: 256 x 256 tiles (or 192 wide, 8 waves of 64
+// x 96), 8 waves of 128 x 64 (6
 // fragment reads per 8 products; 16 waves of 64 x 64 read 8, 16k x 5248 x 1024 rank 64
 // 257 -> 273 us; 4 of 128 x 128 do not fit the registers, 305), a ring of four 32-wide
 // stages as gemm_ring's, and one block per CU that streams its tiles without a pause:
@@ -485,13 +486,14 @@ __device__ __forceinline__ ScalarInts scalar_ints(const void* p) {
 
 __device__ __forceinline__ int stream_f(int r) { return (r >> 2) & 3; }  // swizzle of a row's 4 chunks
 
-template <bool BF16>
+template <bool BF16, int BN>
 __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __restrict__ X, int64_t ldx,
                                                              const uint16_t* __restrict__ W,
                                                              const uint16_t* __restrict__ bias, uint16_t* __restrict__ Y,
                                                              int64_t ldy, int M, int N, int K, int tiles_m, int tiles_n,
                                                              LoraExt ext, Numbers num) {
-  constexpr int NST = kStStages, NW = kStWaves, WM = 2, WN = NW / WM, TM = kStTile / WM / 32, TN = kStTile / WN / 32;
+  constexpr int NST = kStStages, NW = kStWaves, WM = BN == 256 ? 2 : 4, WN = NW / WM, TM = kStTile / WM / 32, TN = BN / WN / 32;
+  static_assert(TN * WN * 32 == BN && BN <= kStTile, "whole blocks of 32");
   constexpr int PW = 2 * kStTile / 16 / NW;  // 1 KB pieces (16 rows) of a stage per wave
   constexpr int ST = TM * TN * 2;            // stores of a tile per lane
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -526,7 +528,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
     const int nd = scalar_ints(num.count)[tm];
     rKT = KT0 + (nd * ext.R + kStBK - 1) / kStBK;
     rk = 0;
-    rn0 = tn * kStTile;
+    rn0 = tn * BN;
     const uint64_t base = xwave ? (uint64_t)(X + (int64_t)tm * kStTile * ldx) : (uint64_t)(W + (int64_t)rn0 * K);
     rsrc = uint4v{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base),
                   (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu), 0x80000000u, 0x00020000u};
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
       const uint32_t c = (slot4 ^ stream_f(r)) * 16;
       // (rows past the operand are clamped: their outputs are never stored)
       off[i] = xwave ? (uint32_t)min(r, M - 1 - tm * kStTile) * (uint32_t)ldx * 2u + c
-                     : (uint32_t)min(r, N - 1 - rn0) * (uint32_t)K * 2u + c;
+                     : r < BN ? (uint32_t)min(r, N - 1 - rn0) * (uint32_t)K * 2u + c : 0xfffffff0u;
       xnum[i] = nd;
       if (xwave) {  // the piece's 16 rows' numbers, two to a word: scalar loads, which no wait for the ring counts
         const ScalarInts nums = scalar_ints(num.number + (int64_t)tm * kStTile + (wave % (NW / 2) * PW + i) * 16);
@@ -582,7 +584,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
         uint32_t at = 0xfffffff0u;  // past the records: zeros
         if (xwave) {
           if (o == xnum[i]) at = ((uint32_t)(tm * kStTile + r) * (uint32_t)ext.R + (uint32_t)c * 8u) * 2u;
-        } else if (o < xnum[i]) {
+        } else if (o < xnum[i] && r < BN) {
           const int a = j == 0 ? who[0] : j == 1 ? who[1] : j == 2 ? who[2] : who[3];
           const int n = min(rn0 + r, N - 1);
           at = (((uint32_t)a * (uint32_t)N + (uint32_t)n) * (uint32_t)ext.R + (uint32_t)c * 8u) * 2u;
@@ -662,7 +664,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
       multiply(1);
     }
     // ---- write-out: lane l32 holds row l32 of a 32 x 32 block, columns 8 g + 4 lg ..
-    const int m0 = tm * kStTile + wm * TM * 32, n0 = tn * kStTile + wn * TN * 32;
+    const int m0 = tm * kStTile + wm * TM * 32, n0 = tn * BN + wn * TN * 32;
     float z = 0.f;
 #pragma unroll
     for (int i = 0; i < TM; i++)
@@ -681,7 +683,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
 #pragma unroll
         for (int e = 0; e < 4; e++) bv[j][g][e] = to_f<BF16>((uint16_t)(b[e >> 1] >> (16 * (e & 1))));
       }
-    const auto ys = __builtin_amdgcn_make_buffer_rsrc((void*)(Y + (int64_t)(tm * kStTile) * ldy + tn * kStTile), 0,
+    const auto ys = __builtin_amdgcn_make_buffer_rsrc((void*)(Y + (int64_t)(tm * kStTile) * ldy + tn * BN), 0,
                                                       0x80000000u, 0x00020000u);
 #pragma unroll
     for (int i = 0; i < TM; i++) {
@@ -707,7 +709,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
           const int n = n0 + 32 * j + 16 * h + 8 * lg;
           // as many stores whatever the edges: those past them fall outside the records
           const uint32_t at = m < M && n < N
-                                  ? (uint32_t)(m - tm * kStTile) * (uint32_t)ldy * 2u + (uint32_t)(n - tn * kStTile) * 2u
+                                  ? (uint32_t)(m - tm * kStTile) * (uint32_t)ldy * 2u + (uint32_t)(n - tn * BN) * 2u
                                   : 0xfffffff0u;
           __builtin_amdgcn_raw_buffer_store_b128(o, ys, at, 0, 0);
         }
@@ -736,10 +738,22 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
   }
 }
 
+// lora_stream's width of tile: 192 columns where the rounds that the CUs take with them are shorter
+// by a fifth, which their operands, 17% more a product, leave a gain of (f16: 4096 x 5248
+// x 1024, two rounds of either, 75 -> 69 us; 8192 x 2304 x 768 61 -> 56; 16.2k x 5248 x
+// 1024, 7 rounds of 192 against 6 of 256, 262 and 274).
+static int lora_stream_width(int cus, int M, int N) {
+  auto cost = [&](int bn) {
+    const int64_t tiles = (int64_t)((M + kStTile - 1) / kStTile) * ((N + bn - 1) / bn);
+    return (tiles + cus - 1) / cus * bn;
+  };
+  return 5 * cost(192) <= 4 * cost(256) ? 192 : 256;
+}
 // The GEMM's tile, by the rules of the plain projection (ring_tile); on the streaming
 // kernel, which stores 16 bytes at a time, once its tiles occupy half of the CUs
-// (f16, 4 adapters in runs of 512 rows, streaming and by ring_tile: 4096 x 2304 x 768, 144 tiles, 36 and 45 us; 3000 x
-// 5248 x 1024 47 and 102; 16384 x 768 x 1152 51 and 81; 16k x 5248 x 1024 262 and 502).
+// (f16, 4 adapters in runs of 512 rows, streaming and by ring_tile: 4096 x 2304 x 768, 144
+// tiles, 36 and 45 us; 3000 x 5248 x 1024 47 and 102; 16384 x 768 x 1152 51 and 81; 16k x
+// 5248 x 1024 262 and 502).
 // Its tiles of 256 rows suit rows that come in runs of one request: a tile of all
 // different adapters multiplies 256 R ranks, gemm_ring's tile of 64 rows 64 R.
 static bool lora_streams(int cus, int64_t M, int64_t N, const uint16_t* bias, const uint16_t* y, int64_t ldy) {
@@ -750,14 +764,16 @@ template <bool BF16>
 static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, const uint16_t* w, const uint16_t* bias,
                       uint16_t* y, int64_t ldy, int M, int N, int K, const LoraExt& ext, const Numbers& num) {
   if (num.tiles > 0) {
-    auto kernel = lora_stream<BF16>;
-    static std::atomic<uint64_t> attr{0};
-    once_per_device(attr, [&] {
-      HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kStLds));
-    });
-    const int tm = (M + kStTile - 1) / kStTile, tn = (N + kStTile - 1) / kStTile;
-    kernel<<<(unsigned)std::min<int64_t>(cus, (int64_t)tm * tn), kStWaves * 64, kStLds, st>>>(x, ldx, w, bias, y, ldy, M, N,
-                                                                                       K, tm, tn, ext, num);
+    static std::atomic<uint64_t> attr[2];
+    auto run = [&](auto kernel, std::atomic<uint64_t>& at, int bn) {
+      once_per_device(at, [&] {
+        HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kStLds));
+      });
+      const int tm = (M + kStTile - 1) / kStTile, tn = (N + bn - 1) / bn;
+      kernel<<<(unsigned)cus, kStWaves * 64, kStLds, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, tn, ext, num);
+    };
+    if (lora_stream_width(cus, M, N) == 256) run(lora_stream<BF16, 256>, attr[0], 256);
+    else run(lora_stream<BF16, 192>, attr[1], 192);
     return;
   }
   auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn, int nw) {
