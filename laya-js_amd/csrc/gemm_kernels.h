@@ -450,37 +450,37 @@ __device__ __forceinline__ void ring_wait_stages(int later) {
 // products, a stage of 64 ranks at a time, and ranks below 64 share one.
 struct NoExt {};
 struct LoraExt {
-  const uint16_t* s;     // [M, R], scaled; rows without an adapter are not read
-  const uint16_t* b;     // [n, N, R], below 2^31 bytes
+  const void* s;         // [M, R], scaled, of x's type; rows without an adapter are not read
+  const void* b;         // [n, N, R], below 2^31 bytes
   const int32_t* index;  // [M]
-  int n, R;              // R % 8 == 0
+  int n, R;              // R a whole number of 16 bytes
 };
 
 // Whether an adapter of the tile other than row m's own holds a non-finite element of
 // column n's B: only then do the zeros of other rows change an output (0 * inf).
-template <bool BF16>
+template <int DT>
 __device__ __forceinline__ bool lora_mixed(const LoraExt& ext, const int* adapters, int nd, int N, int m, int n) {
   const int own = ext.index[m];
   for (int o = 0; o < nd; o++) {
     const int a = adapters[o];
     if (a == own) continue;
     for (int r = 0; r < ext.R; r++)
-      if (to_f<BF16>(ext.b[((int64_t)a * N + n) * ext.R + r]) * 0.f != 0.f) return true;
+      if (load_f(ext.b, ((int64_t)a * N + n) * ext.R + r, DT) * 0.f != 0.f) return true;
   }
   return false;
 }
 
 // One output of a projection with adapters, on its own (slow: see its callers).
-template <bool BF16>
-__device__ __forceinline__ uint16_t lora_output(const uint16_t* X, int64_t ldx, const uint16_t* W, const uint16_t* bias,
-                                                int N, int K, const LoraExt& ext, int m, int n) {
+template <int DT>
+__device__ __forceinline__ float lora_output(const void* X, int64_t ldx, const void* W, const void* bias, int N, int K,
+                                             const LoraExt& ext, int m, int n) {
   float sum = 0.f;
-  for (int k = 0; k < K; k++) sum = fmaf(to_f<BF16>(X[(int64_t)m * ldx + k]), to_f<BF16>(W[(int64_t)n * K + k]), sum);
+  for (int k = 0; k < K; k++) sum = fmaf(load_f(X, (int64_t)m * ldx + k, DT), load_f(W, (int64_t)n * K + k, DT), sum);
   const int a = ext.index[m];
   if (a >= 0 && a < ext.n)
     for (int r = 0; r < ext.R; r++)
-      sum = fmaf(to_f<BF16>(ext.s[(int64_t)m * ext.R + r]), to_f<BF16>(ext.b[((int64_t)a * N + n) * ext.R + r]), sum);
-  return from_f<BF16>(sum + (bias != nullptr ? to_f<BF16>(bias[n]) : 0.f));
+      sum = fmaf(load_f(ext.s, (int64_t)m * ext.R + r, DT), load_f(ext.b, ((int64_t)a * N + n) * ext.R + r, DT), sum);
+  return sum + (bias != nullptr ? load_f(bias, n, DT) : 0.f);
 }
 
 template <int BM, int BN, int WM, int WN, int NST, bool BF16, bool GEGLU, class EXT = NoExt>
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
         uint32_t at = 0xfffffff0u;  // past the records: zeros
         uint64_t base;
         if (p * 8 < BM) {
-          base = (uint64_t)(ext.s + (int64_t)m0 * ext.R);
+          base = (uint64_t)ext.s + (uint64_t)((int64_t)m0 * ext.R * 2);
           if (xnum[i] == o) at = (uint32_t)(r * ext.R + c * 8) * 2u;
         } else {
           base = (uint64_t)ext.b;
@@ -733,8 +733,9 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
       for (int q = tid; q < BM * BN; q += NT) {
         const int m = m0 + q / BN, n = n0 + q % BN;
         const float v = to_f<BF16>(Cs[q]);
-        if (m >= M || n >= N || v * 0.f == 0.f || !lora_mixed<BF16>(ext, adapter, nd, N, m, n)) continue;
-        Cs[q] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, n);
+        constexpr int DT = BF16 ? HB_BF16 : HB_F16;
+        if (m >= M || n >= N || v * 0.f == 0.f || !lora_mixed<DT>(ext, adapter, nd, N, m, n)) continue;
+        Cs[q] = from_f<BF16>(lora_output<DT>(X, ldx, W, bias, N, K, ext, m, n));
       }
     }
   }

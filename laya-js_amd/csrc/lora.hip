@@ -11,7 +11,7 @@
 // projection's own GEMM takes as ranks beyond K: gemm_ring with LoraExt, lora_stream
 // for large M, lora_few for few tiles.  y is rounded once.
 //
-// lora_expand_f32: y += s . B_i^T of f32 rows, on top of the projection.
+// lora_expand_f32: y += s . B_i^T of f32 rows past lora_few, on top of the projection.
 //
 // lora_shrink_any, lora_expand_any: the inner products in f32, then y = round(y + s .
 // B_i^T), any type and size.
@@ -327,10 +327,11 @@ static void launch_prepare(hipStream_t st, int cus, int dt, Prepare& p) {
 // 13.3 with them), and of 16 rows where there are no more.  Tiles of 64 x 64 take over while
 // they go round the CUs once (400 x 2304 x 768, 252 tiles: 12.9 us, gemm_ring's 14.2; 1200 x
 // 1024 x 1024, 304 tiles: 20.3 and 15.6).
-template <bool BF16, int TM, int TN, int NW>
-__global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W,
-                                                const uint16_t* __restrict__ bias, uint16_t* __restrict__ Y, int64_t ldy,
-                                                int M, int N, int K, int tiles_m, LoraExt ext) {
+template <int DT, int TM, int TN, int NW>
+__global__ __launch_bounds__(NW * 64) void lora_few(const char* __restrict__ X, int64_t ldx, const char* __restrict__ W,
+                                                    const char* __restrict__ bias, char* __restrict__ Y, int64_t ldy,
+                                                    int M, int N, int K, int tiles_m, LoraExt ext) {
+  constexpr int ES = DT == HB_F32 ? 4 : 2, KC = 128 / ES, V = 16 / ES;  // bytes, k of a chunk, ranks of 16 bytes
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   auto red = (float(*)[TM * 16][TN * 16 + 4])lds;  // [NW], padded against bank conflicts
   __shared__ int adapter[TM * 16];
@@ -342,10 +343,10 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__
   constexpr int BUF = (TM + TN) * 2048, L = 2 * (TM + TN);
   uint32_t xo[2 * TM], wo[2 * TN];
 #pragma unroll
-  for (int i = 0; i < 2 * TM; i++) xo[i] = piece_offset(i, lane, M - 1 - m0, (uint32_t)ldx * 2u);
+  for (int i = 0; i < 2 * TM; i++) xo[i] = piece_offset(i, lane, M - 1 - m0, (uint32_t)ldx * ES);
 #pragma unroll
-  for (int i = 0; i < 2 * TN; i++) wo[i] = piece_offset(i, lane, N - 1 - n0, (uint32_t)K * 2u);
-  const uint4v xs = lora_records(X + (int64_t)m0 * ldx), ws = lora_records(W + (int64_t)n0 * K);
+  for (int i = 0; i < 2 * TN; i++) wo[i] = piece_offset(i, lane, N - 1 - n0, (uint32_t)K * ES);
+  const uint4v xs = lora_records(X + (int64_t)m0 * ldx * ES), ws = lora_records(W + (int64_t)n0 * K * ES);
   const char* buffers = lds + wave * 2 * BUF;
   const uint32_t at0 = (uint32_t)__builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)buffers);
@@ -373,11 +374,11 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = mfma16<BF16 ? HB_BF16 : HB_F16>(wf[j], xf[i], acc[i][j]);
+        for (int j = 0; j < TN; j++) acc[i][j] = mfma16<DT>(wf[j], xf[i], acc[i][j]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the buffer is requested again)
   };
-  const int kc = (K / 64 - wave + NW - 1) / NW;  // this wave's chunks of K, from 0 on
+  const int kc = (K / KC - wave + NW - 1) / NW;  // this wave's chunks of K, from 0 on
   if (kc > 0) request(0);
   if (kc > 1) request(1);
   // the tile's adapters by number, as they first occur: lane o has number o's
@@ -391,9 +392,9 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__
     mine = lane == nd ? cur : mine;
   }
   if (tid < TM * 16) adapter[tid] = mine;
-  const int r8 = R >> 3, chunks = (nd * r8 + 7) >> 3;  // chunks of 8 ranks of an adapter; chunks of 64 ranks
+  const int rv = R / V, chunks = (nd * rv + 7) >> 3;   // 16 bytes of ranks of an adapter; chunks of 8 such
   const int ec = (chunks - wave + NW - 1) / NW;              // this wave's of those, numbered from kc on
-  const float inv8 = 8.f / (float)R;
+  const float inv = (float)V / (float)R;
   const uint4v ss = lora_records(ext.s), bs = lora_records(ext.b);
   int xnum[2 * TM];  // of the rows of the lane's pieces
 #pragma unroll
@@ -402,20 +403,20 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__
     const uint32_t to = at0 + (uint32_t)((c & 1) * BUF);
     auto piece = [&](int i, auto rows) __attribute__((always_inline)) {  // of i's rows
       const int r = i * 8 + (lane >> 3), ch = (wave + NW * (c - kc)) * 8 + ((lane & 7) ^ row_f(r));
-      const int o = (int)(((float)ch + 0.5f) * inv8);
-      rows(r, o, (uint32_t)(ch - o * r8) * 8u);
+      const int o = (int)(((float)ch + 0.5f) * inv);
+      rows(r, o, (uint32_t)(ch - o * rv) * V);
     };
     // past the records: zeros
 #pragma unroll
     for (int i = 0; i < 2 * TM; i++)
       piece(i, [&](int r, int o, uint32_t rank) {
-        buffer_lds16(ss, o == xnum[i] ? ((uint32_t)min(m0 + r, M - 1) * (uint32_t)R + rank) * 2u : 0xfffffff0u, to + 1024u * i);
+        buffer_lds16(ss, o == xnum[i] ? ((uint32_t)min(m0 + r, M - 1) * (uint32_t)R + rank) * ES : 0xfffffff0u, to + 1024u * i);
       });
 #pragma unroll
     for (int j = 0; j < 2 * TN; j++)
       piece(j, [&](int r, int o, uint32_t rank) {
         const uint32_t who = (uint32_t)__shfl(mine, o & 63), n = (uint32_t)min(n0 + r, N - 1);
-        buffer_lds16(bs, o < nd ? ((who * (uint32_t)N + n) * (uint32_t)R + rank) * 2u : 0xfffffff0u,
+        buffer_lds16(bs, o < nd ? ((who * (uint32_t)N + n) * (uint32_t)R + rank) * ES : 0xfffffff0u,
                      to + 1024u * (2 * TM + j));
       });
   };
@@ -448,19 +449,49 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const uint16_t* __restrict__
     for (int w = 0; w < NW; w++)
 #pragma unroll
       for (int q = 0; q < 2; q++) v[q] += red[w][row][col + q];
-    uint16_t o[2];
 #pragma unroll
     for (int q = 0; q < 2; q++) {
       const int nq = min(n + q, N - 1);
-      o[q] = from_f<BF16>(v[q] + (bias != nullptr ? to_f<BF16>(bias[nq]) : 0.f));
       // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf)
-      if (v[q] * 0.f != 0.f && lora_mixed<BF16>(ext, adapter, nd, N, m, nq))
-        o[q] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, nq);
+      const bool alone = v[q] * 0.f != 0.f && lora_mixed<DT>(ext, adapter, nd, N, m, nq);
+      v[q] += bias != nullptr ? load_f(bias, nq, DT) : 0.f;
+      if (alone) v[q] = lora_output<DT>(X, ldx, W, bias, N, K, ext, m, nq);
     }
-    uint16_t* y = Y + (int64_t)m * ldy + n;
-    if (n + 1 < N) *(uint32_t*)y = (uint32_t)o[0] | ((uint32_t)o[1] << 16);
-    else y[0] = o[0];
+    char* y = Y + ((int64_t)m * ldy + n) * ES;
+    if constexpr (DT == HB_F32) {
+      if (n + 1 < N) *(float2*)y = float2{v[0], v[1]};
+      else *(float*)y = v[0];
+    } else {
+      const uint32_t lo = from_f<DT == HB_BF16>(v[0]), hi = from_f<DT == HB_BF16>(v[1]);
+      if (n + 1 < N) *(uint32_t*)y = lo | (hi << 16);
+      else *(uint16_t*)y = (uint16_t)lo;
+    }
   }
+}
+
+// Its tiles, if it takes the call; false: it does not.
+template <int DT>
+static bool lora_few_tiles(hipStream_t st, int cus, const void* x, int64_t ldx, const void* w, const void* bias, void* y,
+                           int64_t ldy, int M, int N, int K, const LoraExt& ext, bool launch) {
+  auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn, int nw) {
+    if (!launch) return true;
+    const int tm = (M + bm - 1) / bm, lds = nw * 2 * (bm + bn) * 128;
+    if (lds > 64 * 1024)
+      once_per_device(attr, [&] {
+        HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+      });
+    kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), nw * 64, lds, st>>>(
+        (const char*)x, ldx, (const char*)w, (const char*)bias, (char*)y, ldy, M, N, K, tm, ext);
+    return true;
+  };
+  static std::atomic<uint64_t> attr[5];
+  auto tiles = [&](int t) { return (int64_t)((M + t - 1) / t) * ((N + t - 1) / t); };
+  const bool half = 2 * tiles(32) <= cus;
+  if (tiles(32) <= 2 * cus) {
+    if (M <= 16) return half ? run(lora_few<DT, 1, 1, 8>, attr[0], 16, 16, 8) : run(lora_few<DT, 1, 2, 8>, attr[1], 16, 32, 8);
+    return half ? run(lora_few<DT, 2, 1, 8>, attr[2], 32, 16, 8) : run(lora_few<DT, 2, 2, 8>, attr[3], 32, 32, 8);
+  }
+  return tiles(64) <= cus && run(lora_few<DT, 4, 4, 4>, attr[4], 64, 64, 4);
 }
 
 // The projection with adapters for large M: 256 x 256 tiles (or 192 wide, 8 waves of 64
@@ -727,8 +758,9 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
         const int m = m0 + q / (TN * 32), n = n0 + q % (TN * 32);
         if (m >= M || n >= N) continue;
         const float v = to_f<BF16>(__builtin_nontemporal_load(Y + (int64_t)m * ldy + n));
-        if (v * 0.f == 0.f || !lora_mixed<BF16>(ext, list, nd, N, m, n)) continue;
-        Y[(int64_t)m * ldy + n] = lora_output<BF16>(X, ldx, W, bias, N, K, ext, m, n);
+        constexpr int DT = BF16 ? HB_BF16 : HB_F16;
+        if (v * 0.f == 0.f || !lora_mixed<DT>(ext, list, nd, N, m, n)) continue;
+        Y[(int64_t)m * ldy + n] = from_f<BF16>(lora_output<DT>(X, ldx, W, bias, N, K, ext, m, n));
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -776,23 +808,7 @@ static void lora_gemm(hipStream_t st, int cus, const uint16_t* x, int64_t ldx, c
     else run(lora_stream<BF16, 192>, attr[1], 192);
     return;
   }
-  auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn, int nw) {
-    const int tm = (M + bm - 1) / bm, lds = nw * 2 * (bm + bn) * 128;
-    if (lds > 64 * 1024)
-      once_per_device(attr, [&] {
-        HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-      });
-    kernel<<<(unsigned)((int64_t)tm * ((N + bn - 1) / bn)), nw * 64, lds, st>>>(x, ldx, w, bias, y, ldy, M, N, K, tm, ext);
-  };
-  static std::atomic<uint64_t> attr[5];
-  auto tiles = [&](int t) { return (int64_t)((M + t - 1) / t) * ((N + t - 1) / t); };
-  const bool half = 2 * tiles(32) <= cus;
-  if (tiles(32) <= 2 * cus) {
-    if (M <= 16) half ? run(lora_few<BF16, 1, 1, 8>, attr[0], 16, 16, 8) : run(lora_few<BF16, 1, 2, 8>, attr[1], 16, 32, 8);
-    else half ? run(lora_few<BF16, 2, 1, 8>, attr[2], 32, 16, 8) : run(lora_few<BF16, 2, 2, 8>, attr[3], 32, 32, 8);
-    return;
-  }
-  if (tiles(64) <= cus) return run(lora_few<BF16, 4, 4, 4>, attr[4], 64, 64, 4);
+  if (lora_few_tiles<BF16 ? HB_BF16 : HB_F16>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, true)) return;
   auto go = [&](auto launch) { launch(st, 0u, x, ldx, w, bias, (const uint16_t*)nullptr, (int64_t)0, y, ldy, M, N, K, ext); };
   LinearKernel tile = LinearKernel::kRing64x64x3;
   ring_tile(cus, M, N, K, false, true, false, &tile);
@@ -954,9 +970,47 @@ static bool lora_fused(uintptr_t ctx, int dt, const uint16_t* x, int64_t ldx, co
   hipStream_t st = stream_of(ctx);
   launch_prepare(st, cus, dt, p);
   check_launch("hb_lora_linear");
-  const LoraExt ext{(const uint16_t*)p.s, (const uint16_t*)l.b, p.index, p.n, p.R};
+  const LoraExt ext{p.s, (const void*)l.b, p.index, p.n, p.R};
   if (dt == HB_BF16) lora_gemm<true>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
   else lora_gemm<false>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
+  check_launch("hb_lora_linear");
+  return true;
+}
+
+// f32 rows on the matrix cores: whole 128 bytes of K, 16 bytes of ranks and of y.
+static bool lora_takes_f32(int dt, uintptr_t x, int64_t ldx, uintptr_t y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                           const LoraArgs& l) {
+  return dt == HB_F32 && M > 0 && N > 0 && K > 0 && l.n > 0 && l.R > 0 && K % 32 == 0 && N % 4 == 0 && l.R % 4 == 0 &&
+         ldx % 4 == 0 && ldy % 4 == 0 && K < (1 << 22) && ldx < (1 << 22) && (x | y | l.a | l.b) % 16 == 0 &&
+         (M + 31) / 32 < 65536;
+}
+static Prepare prepare_f32(uintptr_t x, int64_t ldx, int64_t M, int64_t K, const LoraArgs& l, void* s) {
+  Prepare p{(const char*)x, ldx, (const char*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, (int)M,
+            (int)l.R, (int)K};
+  p.s = s;
+  return p;
+}
+// The projection of f32 rows with adapters where lora_few takes it (76 x 1024 x 2624, 21
+// adapters of rank 16: 21.4 us, hb_linear and lora_expand_f32 33.5; 300 x 768 x 768, rank
+// 64: 13.4 and 21.5; 256 x 5248 x 1024, past it, 48); false: it does not, or there is no
+// memory for the inner products.
+static bool lora_few_f32(uintptr_t ctx, uintptr_t x, int64_t ldx, uintptr_t w, uintptr_t bias, uintptr_t y, int64_t ldy,
+                         int64_t M, int64_t N, int64_t K, const LoraArgs& l) {
+  if (w % 16 != 0 || l.n * l.R * N * 4 >= (1ll << 31) || M * l.R * 4 >= (1ll << 31)) return false;
+  const int cus = cu_count(ctx);
+  hipStream_t st = stream_of(ctx);
+  LoraExt ext{nullptr, (const void*)l.b, (const int32_t*)l.index, (int)l.n, (int)l.R};
+  auto few = [&](bool launch) {
+    return lora_few_tiles<HB_F32>(st, cus, (const void*)x, ldx, (const void*)w, (const void*)bias, (void*)y, ldy, (int)M,
+                                  (int)N, (int)K, ext, launch);
+  };
+  CallScratch s(ctx);
+  if (!few(false) || !s.take((size_t)(M * l.R * 4))) return false;
+  Prepare p = prepare_f32(x, ldx, M, K, l, s.p);
+  launch_prepare(st, cus, HB_F32, p);
+  check_launch("hb_lora_linear");
+  ext.s = s.p;
+  few(true);
   check_launch("hb_lora_linear");
   return true;
 }
@@ -968,11 +1022,8 @@ static void add_adapters(uintptr_t ctx, const char* op, int dt, uintptr_t x, int
   if (!s.take((size_t)(M * l.R * 4)))
     throw std::runtime_error(std::string(op) + ": out of device memory for the adapters' inner products");
   hipStream_t st = stream_of(ctx);
-  if (dt == HB_F32 && K % 32 == 0 && N % 4 == 0 && l.R % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && K < (1 << 22) && ldx < (1 << 22) &&
-      (x | y | l.a | l.b) % 16 == 0 && (M + 31) / 32 < 65536) {
-    Prepare p{(const char*)x, ldx, (const char*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, (int)M,
-              (int)l.R, (int)K};
-    p.s = s.p;
+  if (lora_takes_f32(dt, x, ldx, y, ldy, M, N, K, l)) {
+    Prepare p = prepare_f32(x, ldx, M, K, l, s.p);
     launch_prepare(st, cu_count(ctx), dt, p);
     const int64_t tiles = (N + 255) / 256 * ((M + 31) / 32);
     const dim3 blocks((unsigned)((N + 255) / 256), (unsigned)((M + 31) / 32),
@@ -1008,6 +1059,7 @@ int hb_lora_linear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t w,
       lora_fused(ctx, dt, (const uint16_t*)x, ldx, (const uint16_t*)w, Codes{}, (const uint16_t*)bias, (uint16_t*)y, ldy,
                  (int)M, (int)N, (int)K, l))
     return 0;
+  if (lora_takes_f32(dt, x, ldx, y, ldy, M, N, K, l) && lora_few_f32(ctx, x, ldx, w, bias, y, ldy, M, N, K, l)) return 0;
   if (hb_linear(ctx, dt, x, ldx, w, bias, 0, 0, y, ldy, M, N, K, bias ? HB_EPI_BIAS : 0)) return -1;
   add_adapters(ctx, "hb_lora_linear", dt, x, ldx, y, ldy, M, N, K, l);
   HB_API_END
