@@ -698,9 +698,9 @@ class HipBackend:
         return t
 
     def _new(self, shape, dtype: str) -> HipTensor:
-        shape = tuple(int(d) for d in shape)
-        st = self._malloc(_numel(shape) * DT[dtype][1])
-        return self._track(HipTensor(shape, dtype, st))
+        t = HipTensor(shape, dtype, None)
+        t._st = self._malloc(_numel(t.shape) * DT[dtype][1])
+        return self._track(t)
 
     def _view(self, t: HipTensor, shape, strides, off) -> HipTensor:
         return self._track(HipTensor(shape, t.dtype, t._st.retain(), off, strides))
