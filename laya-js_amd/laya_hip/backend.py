@@ -921,9 +921,10 @@ class HipBackend:
         if t._st is not None:
             t._st.release()
             t._st = None
-        for k, v in list((t._meta or {}).items()):
-            if isinstance(v, HipTensor):
-                self.dispose(v)
+        if t._meta:
+            for v in list(t._meta.values()):
+                if isinstance(v, HipTensor):
+                    self.dispose(v)
         t._meta = None
 
     def scope(self, fn: Callable[[], Any]):
