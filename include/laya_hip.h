@@ -416,8 +416,8 @@ int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t 
  * tokens: query i of n_q is at position i + n_k - n_q among its n_k keys.
  * Query i sees key j if j < prefix[b] (i32 [B], or 0: none), or if (not causal,
  * or j <= pos) and (window -1, or |pos - j| <= window / 2).  Scores are scale *
- * q . k, then cap * tanh(score / cap) unless cap is 0, then less slopes[h] *
- * |pos - j| (f32 [H]) unless slopes is 0.  Rows without a visible key, and rows
+ * q . k, then cap * tanh(score / cap) unless cap is 0 (a normal number else), then
+ * less slopes[h] * |pos - j| (f32 [H]) unless slopes is 0.  Rows without a visible key, and rows
  * behind the last document, are zeros.  Values of hidden keys are not used,
  * whatever they hold. */
 int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t* qs, uintptr_t k, const int64_t* ks, uintptr_t v,

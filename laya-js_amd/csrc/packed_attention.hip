@@ -25,6 +25,7 @@
 // packed_attn_f32_rows, packed_attn_f32: the same for f32, on v_mfma_f32_32x32x2_f32.
 //
 // packed_attn_any: any head dimension, type and strides.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -247,7 +248,8 @@ static Score score_of(float scale, float cap, bool bias) {
   const float sl = fmaxf(fabsf(scale), 1e-30f);
   const bool capped = cap > 0.f;
   s.mul = capped || bias ? 1.f : sl * kLog2e;
-  s.c1 = capped ? 2.f * sl / cap * kLog2e : sl * kLog2e;
+  // (finite, so that 0 * c1 is 0 under the smallest caps)
+  s.c1 = capped ? fminf(2.f * sl / cap * kLog2e, FLT_MAX) : sl * kLog2e;
   s.c2 = cap * kLog2e;
   s.flip = scale < 0.f ? 0x80008000u : 0u;
   // tanh(y) / y in y^2 on [0, 0.75^2]
@@ -261,6 +263,7 @@ static Score score_of(float scale, float cap, bool bias) {
   }
   s.near = capped ? (float)(0.75 / g) : 0.f;
   s.tiny_near = capped ? (float)(0.25 / g) : 0.f;
+  if (!std::isfinite(s.poly[4])) s.near = s.tiny_near = -1.f;  // a cap far below the scale: never those
   return s;
 }
 
@@ -1235,6 +1238,7 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   HB_REQUIRE(D >= 1 && D <= 64 * kAnyCols, "hb_sdpa_packed: head dimension must be 1 to 512");
   HB_REQUIRE(qs && ks && vs, "hb_sdpa_packed: null strides");
   HB_REQUIRE(std::isfinite(scale) && std::isfinite(cap) && cap >= 0.f, "hb_sdpa_packed: scale and cap must be finite");
+  HB_REQUIRE(cap == 0.f || cap >= FLT_MIN, "hb_sdpa_packed: a cap is 0 (none) or a normal number");
   HB_REQUIRE(window >= -1, "hb_sdpa_packed: a window is not negative (-1: none)");
   if (Tq == 0) return 0;
   HB_REQUIRE(q && o && q_doc && q_blocks && q_offsets && k_offsets && (Tk == 0 || (k && v)), "hb_sdpa_packed: null argument");
@@ -1264,8 +1268,8 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   p.causal = causal ? 1 : 0;
   p.half = window < 0 ? -1 : (int)(window / 2 < (1ll << 30) ? window / 2 : (1ll << 30) - 1);
   p.scale = scale;
-  p.cap = cap;
-  p.sc = score_of(scale, cap, slopes != 0);
+  p.cap = fminf(cap, 0x1p100f);  // (scores below 2^88 round to themselves under either; its reciprocal is normal)
+  p.sc = score_of(scale, p.cap, slopes != 0);
   if (packed_takes_mfma(p, dt == HB_F32 ? 4 : 8)) packed_mfma(ctx, dt, p);
   else packed_any(ctx, dt, p);
   check_launch("hb_sdpa_packed");

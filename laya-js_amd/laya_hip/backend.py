@@ -1941,7 +1941,7 @@ class HipBackend:
             raise ValueError(f"sdpaPacked: {H} heads over {Hk} key heads of dimension {D}")
         if window is not None and window < 0:
             raise ValueError(f"sdpaPacked: window {window}")
-        if cap is not None and not 0.0 < cap < math.inf or not math.isfinite(scale):
+        if cap is not None and not 2.0 ** -126 <= cap < 2.0 ** 128 or not math.isfinite(scale):
             raise ValueError(f"sdpaPacked: scale {scale}, cap {cap}")
         tmp: list = []
         if prefix is not None:
@@ -1970,7 +1970,7 @@ class HipBackend:
                        self._ptr(k), F.i64s(k._strides), self._ptr(v), F.i64s(v._strides), out._st.ptr,
                        self._ptr(docs.doc), self._ptr(docs.offsets) + 4 * docs.table, self._ptr(docs.offsets), self._ptr(keys.offsets),
                        docs.count, T, Tk, H, Hk, D, float(scale),
-                       1 if causal else 0, -1 if window is None else int(window),
+                       1 if causal else 0, -1 if window is None else min(int(window), 1 << 31),
                        0 if prefix is None else self._ptr(prefix), float(cap or 0.0),
                        0 if slopes is None else self._ptr(slopes))
         for t in tmp:

@@ -290,6 +290,27 @@ def test_attention_scales(b, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_attention_caps(b, dtype):
+    """The smallest caps, also where a score is 0, and large ones, which leave the
+    scores as they are: s (1 - s^2 / (3 cap^2)), the tanh off by 2^-20 s at most there."""
+    def zero_rows(q, k, v):
+        q[::5] = 0
+    for nq in ([70, 133], [1, 1]):
+        for cap in (2.0 ** -126, 1e-30, 1e-6, 1e-3):
+            for opts in (dict(), dict(slopes=[0.25, 0.0])):
+                run_attn(b, dtype, nq, [70, 133], 2, 2, 64, 4, scale=3.0, cap=cap, mangle=zero_rows, **opts)
+    rng = np.random.default_rng(5)
+    q, k, v = (rounded(rng.standard_normal((203, 2, 64)), dtype) for _ in range(3))
+    docs, t = b.packDocs(i32(b, [70, 133]), 203), [b.fromHost(to_host(x, dtype)) for x in (q, k, v)]
+    off = ref.offsets([70, 133], 203)
+    o, w, e = ref.sdpa_packed(q, k, v, off, off, 0.125)
+    for cap in (1e5, 1e20, 3e38):
+        got = read32(b, b.sdpaPacked(*t, docs, 0.125, cap=cap, causal=False))
+        tol = attn_tolerance(dtype, o, w, e, 64, 133) + (2 * 2.0 ** -20 * e) * w
+        assert not (np.abs(got - o) > tol).any(), (cap, np.abs(got - o).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_of_views(b, dtype):
     """q, k, v as slices of one projection, transposed heads, and unaligned
     slices: the values of contiguous operands."""

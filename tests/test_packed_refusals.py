@@ -92,7 +92,7 @@ def test_attention_refusals(b):
     refused(b, ValueError, "key heads", call(q, b.t(9, 0, 64), b.t(9, 0, 64)))
     refused(b, ValueError, "key heads", call(b.t(6, 4, 513), b.t(9, 2, 513), b.t(9, 2, 513)))
     refused(b, ValueError, "window", call(q, k, v, window=-1))
-    for cap in (0.0, -1.0, float("inf"), float("nan")):
+    for cap in (0.0, -1.0, float("inf"), float("nan"), 1e-39, 1e39):
         refused(b, ValueError, "cap", call(q, k, v, cap=cap))
     for scale in (float("inf"), float("nan")):
         refused(b, ValueError, "scale", lambda: b.sdpaPacked(q, k, v, docs, scale, keys=keys))
@@ -159,7 +159,7 @@ def test_entry_points_refuse_before_they_touch_a_context():
         return (dt, q, three, P, three, P, three, P, P, P, P, P, B, Tq, Tk, H, Hk, D, scale, 0, window, 0, cap, 0)
     for match, bad in (("dtype", dict(dt=F.HB_U8)), ("bad sizes", dict(B=-1)), ("bad sizes", dict(Tk=1 << 30)),
                        ("multiple", dict(H=3, Hk=2)), ("multiple", dict(Hk=0)), ("head dimension", dict(D=513)),
-                       ("finite", dict(scale=float("nan"))), ("finite", dict(cap=-1.0)), ("window", dict(window=-2)),
+                       ("finite", dict(scale=float("nan"))), ("finite", dict(cap=-1.0)), ("normal", dict(cap=1e-39)), ("window", dict(window=-2)),
                        ("null argument", dict(q=0))):
         refuses("hb_sdpa_packed", match, *attn(**bad))
 
