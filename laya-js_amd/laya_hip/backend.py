@@ -1990,15 +1990,24 @@ class HipBackend:
             raise ValueError(f"loraBank: rank {a.shape[1]} above 1024")
         if scales is not None and scales.shape != (a.shape[0],):
             raise ValueError(f"loraBank: scales {list(scales.shape)} of {a.shape[0]} adapters")
-        if scales is None:
-            s = self.fromHost(HostTensor("f32", (a.shape[0],), np.ones(a.shape[0], np.float32)))
-        else:
-            s = self._held(scales if scales.dtype == "f32" else self.cast(scales, "f32"))
-        rank = a.shape[1]
+        count, rank = a.shape[:2]
         unit = 4 if a.dtype == "f32" else 8  # ranks of 16 bytes
+        tmp: list = []
+        if scales is None:
+            s = self.fromHost(HostTensor("f32", (count,), np.ones(count, np.float32)))
+            tmp.append(s)
+        else:
+            s = self._plain(scales, "f32", tmp)
         if rank % unit:
             a, b = self._padded(a, 1, -rank % unit), self._padded(b, 2, -rank % unit)
-        return LoraBank(self, self._held(a), self._held(b), s, rank)
+            tmp += [a, b]
+        else:
+            a, b = self._plain(a, a.dtype, tmp), self._plain(b, b.dtype, tmp)
+        # (references of the bank's own; those of the copies end here)
+        held = [self._view(t, t.shape, _contig(t.shape), t._off) for t in (a, b, s)]
+        for t in tmp:
+            self.dispose(t)
+        return LoraBank(self, *held, rank)
 
     def _padded(self, t: HipTensor, axis: int, more: int) -> HipTensor:
         """A contiguous copy of t with `more` zeros behind `axis`."""
@@ -2010,11 +2019,6 @@ class HipBackend:
         if t.size:
             self._copy_into(t, out._st.ptr, _contig(shape))
         return out
-
-    def _held(self, t: HipTensor) -> HipTensor:
-        """A contiguous tensor of t's values with a reference of its own."""
-        c = self._contiguous(t)
-        return self._view(c, c.shape, _contig(c.shape), c._off)
 
     def _lora_operands(self, op: str, x: HipTensor, N: int, K: int, bank: LoraBank, index: HipTensor, bias, tmp: list):
         if not isinstance(bank, LoraBank):

@@ -189,3 +189,20 @@ def test_bank_from_a_scope_outlives_it():
     assert not (bank.a._dead or bank.b._dead or bank.scales._dead)
     docs = b.scope(lambda: b.packDocs(b.fromHost(HostTensor("i32", (2,), np.zeros(2, np.int32))), 4, 2))
     assert not any(t._dead for t in (docs.offsets, docs.doc, docs.pos, docs.slots))
+
+
+@pytest.mark.parametrize("rank", [8, 5])
+def test_bank_holds_no_more_than_its_tensors(b, rank):
+    """Copies that a bank is made from (padded ranks, scales cast, views) end with it."""
+    stores, malloc = [], b._malloc
+    b._malloc = lambda n: (stores.append(malloc(n)), stores[-1])[1]
+    given = [b.t(2, rank, 64), b.t(2, 32, rank), b.t(2, dtype="f16")]
+    swapped = b.t(2, 64, rank)
+    view = b.transpose(swapped, [0, 2, 1])
+    for scales in (given[2], b.t(2, dtype="f32"), None):
+        for a in (given[0], view):
+            b.loraBank(a, given[1], scales).dispose()
+        b.dispose(scales)
+    for t in (*given, swapped, view):
+        b.dispose(t)
+    assert len(stores) > 4 and all(s.refs == 0 for s in stores)
