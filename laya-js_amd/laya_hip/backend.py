@@ -1981,7 +1981,9 @@ class HipBackend:
     def loraBank(self, a: HipTensor, b: HipTensor, scales: Optional[HipTensor] = None) -> LoraBank:
         """The low-rank adapters of one projection, for loraLinear: a [count,
         rank, in], b [count, out, rank] of the activations' type, scales [count]
-        (1 each unless given).  The bank holds the tensors; dispose() frees it."""
+        (1 each unless given).  The bank holds the tensors, or copies where those are
+        not contiguous or ranks are padded, so values written to them later may not
+        show: make another bank then.  dispose() frees it."""
         self._live(a, b, scales, op="loraBank")
         if (len(a.shape) != 3 or len(b.shape) != 3 or a.dtype != b.dtype or a.dtype not in FLOAT_DT
                 or (a.shape[0], a.shape[1]) != (b.shape[0], b.shape[2])):
