@@ -216,26 +216,32 @@ struct Wave {
   float16v o[2];  // columns 32 d + 8 (r / 4) + 4 lg + r % 4
   float m, l;     // running maximum (before mul), the lane's sum of weights
 };
-// A capped score c2 tanh(c1 x / 2) is c2 - 2 c2 / (1 + 2^(c1 x)) anywhere (c1 in base
-// 2), and where every score of a tile is within 0.75 cap, the odd polynomial of
-// degree 9 through tanh's Chebyshev points there, off by 3.6e-7 at most: 6
-// instructions instead of an exponential and a reciprocal at a lower rate (chunks of
+// A capped score c2 tanh(c1 x / 2) is c2 - 2 c2 / (1 + 2^(c1 x)) (c1 in base 2), which
+// cancels for scores that are small against the cap (off by 2e-7 c2): it is taken past
+// 0.75 cap alone, score by score, since a tile may hold hidden scores of any size beside
+// small ones.  Within 0.75 cap the odd polynomial of degree 9 through tanh's Chebyshev
+// points there, off by 3.6e-7 at most; where that holds for every score of a tile it
+// takes 6 instructions instead of an exponential and a reciprocal at a lower rate (chunks of
 // 1000 queries over up to 8192 keys: 164 -> 153 us).  Within 0.25 cap that of degree 5,
 // off by 1e-7 at most, does, whose last product is one with the subtraction of the
 // maximum (153 -> 135 us).
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ float score(const Score& s, float slope, int pos, int key, float x) {
-  if constexpr (CAP) x = fmaf(-2.f * s.c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * s.c1)), s.c2);
-  else if constexpr (BIAS) x *= s.c1;
-  if constexpr (BIAS) x = fmaf(-slope, fabsf((float)(pos - key)), x);
-  return x;
-}
 __device__ __forceinline__ float capped_near(const Score& s, float x) {
   const float u = x * x;
   float r = fmaf(u, s.poly[4], s.poly[3]);
 #pragma unroll
   for (int i = 2; i >= 0; i--) r = fmaf(u, r, s.poly[i]);
   return x * r;
+}
+__device__ __forceinline__ float capped(const Score& s, float x) {
+  const float far = fmaf(-2.f * s.c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * s.c1)), s.c2);
+  return fabsf(x) <= s.near ? capped_near(s, x) : far;
+}
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float score(const Score& s, float slope, int pos, int key, float x) {
+  if constexpr (CAP) x = capped(s, x);
+  else if constexpr (BIAS) x *= s.c1;
+  if constexpr (BIAS) x = fmaf(-slope, fabsf((float)(pos - key)), x);
+  return x;
 }
 // The factor of x in its capped score, |x| <= tiny_near
 __device__ __forceinline__ float tiny_factor(const Score& s, float x) {
@@ -362,8 +368,8 @@ __device__ __forceinline__ void wave_weights(Wave& w, float16v (&st)[2], int k0,
 #pragma unroll
       for (int r = 0; r < 16; r++) far = fmaxf(far, fabsf(st[kb][r]));
     if (!BIAS && !mixed && __all(far <= sc.tiny_near)) {
-      auto capped = [&](float x) { return x * tiny_factor(sc, x); };
-      follow_maximum(w, sc, capped(far), [&] { return capped(max_of(st)); });  // (the cap keeps the order)
+      auto tiny = [&](float x) { return x * tiny_factor(sc, x); };
+      follow_maximum(w, sc, tiny(far), [&] { return tiny(max_of(st)); });  // (the cap keeps the order)
       wave_exps<BF16>(w, st, sc, pf, [&](float x, float mc) { return fmaf(x, tiny_factor(sc, x), -mc); });
       return;
     }
@@ -376,7 +382,7 @@ __device__ __forceinline__ void wave_weights(Wave& w, float16v (&st)[2], int k0,
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) st[kb][r] = score<true, false>(sc, 0.f, 0, 0, st[kb][r]);
+        for (int r = 0; r < 16; r++) st[kb][r] = capped(sc, st[kb][r]);
     }
   }
   if constexpr (BIAS) {

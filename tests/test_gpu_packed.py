@@ -476,3 +476,100 @@ def test_encode_packed_with_adapters_is_merged_weights(b):
             bank.dispose()
     enc.disposePacked(inp)
     enc.dispose()
+
+
+# ------------------------------------------------------------------ caps over what is hidden, and over large products
+
+def capped_tolerance(dtype, o, w, e, nk, cap):
+    """A capped score is off by 2^-20 of itself where it is small against the cap and
+    by 2^-20 cap anywhere; a score is at most e."""
+    soft = 2.0 ** -20 * min(cap, 2 * e) if cap else 0.0
+    return attn_tolerance(dtype, o, w, e, 64, nk) + soft * w
+
+
+HIDDEN = [dict(), dict(cap=5.0), dict(cap=1e5), dict(cap=1e8), dict(cap=1e20), dict(cap=3e38), dict(slopes=True),
+          dict(cap=5.0, slopes=True), dict(cap=1e8, slopes=True)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("opts", range(len(HIDDEN)))
+@pytest.mark.parametrize("what", [np.nan, np.inf, 6e4])
+@pytest.mark.parametrize("nq,nk,heads,kv", [([230, 70], None, 2, 2), ([230, 70], None, 130, 130), ([1, 1, 2], [300, 64, 90], 4, 4),
+                                            ([1, 1, 2], [300, 64, 90], 4, 1), ([33, 1], [333, 200], 64, 64)])
+def test_attention_hidden_keys_do_not_move_scores(b, dtype, opts, what, nq, nk, heads, kv):
+    """Keys and values that a window hides, non-finite or with products far above any
+    cap, leave the rows that do not see them as they are: in the same tiles, with caps,
+    slopes and grouped heads, few queries and many."""
+    opts = dict(HIDDEN[opts])
+    rng = np.random.default_rng(31)
+    nk = nq if nk is None else nk
+    T, Tk = sum(nq), sum(nk)
+    q = rounded(rng.standard_normal((T, heads, 64)), dtype)
+    k, v = (rounded(rng.standard_normal((Tk, kv, 64)), dtype) for _ in range(2))
+    qoff, koff = ref.offsets(nq, T), ref.offsets(nk, Tk)
+    # hidden: two keys in three documents' middles and one near their ends, seen by few rows or none
+    hide = np.unique([int(koff[i] + at) for i, n in enumerate(nk) for at in (3, n // 2, n - 12) if 0 <= at < n])
+    dk, dv = k.copy(), v.copy()
+    dk[hide], dv[hide] = what, what
+    if opts.get("slopes"):
+        opts["slopes"] = (0.25 * 0.5 ** (np.arange(heads) % 4)).astype(np.float32)
+    dev = dict(opts)
+    if "slopes" in opts:
+        dev["slopes"] = b.fromHost(HostTensor("f32", (heads,), opts["slopes"]))
+    docs, keys = b.packDocs(i32(b, nq), T), b.packDocs(i32(b, nk), Tk)
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, dk, dv)), docs, 0.125, keys=keys, window=16,
+                                 **dev))
+    o, w, e = ref.sdpa_packed(q, k, v, qoff, koff, 0.125, window=16, **opts)
+    clean = np.ones(T, bool)
+    for i in range(len(nq)):
+        pos = np.arange(nq[i]) + nk[i] - nq[i]
+        for h in hide[(hide >= koff[i]) & (hide < koff[i + 1])] - koff[i]:
+            clean[qoff[i]:qoff[i + 1]] &= np.abs(pos - h) > 8
+    assert clean.sum() >= T - 2 * 3 * 17 and clean.any()
+    bad = (np.abs(got - o) > capped_tolerance(dtype, o, w, e, max(nk), opts.get("cap"))) | ~np.isfinite(got)
+    assert not bad[clean].any(), f"{bad[clean].sum()}, worst {np.abs(got - o)[clean].max()}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [None, 8.0, 1e8])
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_attention_hidden_keys_in_pieces(b, dtype, cap, what):
+    """The same where runs are split and joined: causal rows over long keys, of
+    which the documents' last ones, that no row but the last sees, hold anything."""
+    rng = np.random.default_rng(32)
+    for nq, nk, heads, kv in (([300, 200], [5000, 4100], 2, 1), ([2, 3], [5000, 4100], 2, 2)):
+        T, Tk = sum(nq), sum(nk)
+        q = rounded(rng.standard_normal((T, heads, 64)), dtype)
+        k, v = (rounded(rng.standard_normal((Tk, kv, 64)), dtype) for _ in range(2))
+        qoff, koff = ref.offsets(nq, T), ref.offsets(nk, Tk)
+        dk, dv = k.copy(), v.copy()
+        last = koff[1:] - 1
+        dk[last], dv[last] = what, what
+        docs, keys = b.packDocs(i32(b, nq), T), b.packDocs(i32(b, nk), Tk)
+        got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, dk, dv)), docs, 0.125, keys=keys,
+                                     causal=True, cap=cap))
+        o, w, e = ref.sdpa_packed(q, k, v, qoff, koff, 0.125, causal=True, cap=cap)
+        clean = np.ones(T, bool)
+        clean[qoff[1:] - 1] = False
+        bad = (np.abs(got - o) > capped_tolerance(dtype, o, w, e, max(nk), cap)) | ~np.isfinite(got)
+        assert not bad[clean].any(), f"{bad[clean].sum()}, worst {np.abs(got - o)[clean].max()}"
+
+
+@pytest.mark.parametrize("dtype,cap", [("f32", 1e4), ("f32", 1e6), ("f32", 1e10), ("f16", 1e4), ("f16", 1e6), ("bf16", 1e4),
+                                       ("bf16", 1e6), ("bf16", 1e10)])
+def test_attention_small_scores_beside_one_near_a_large_cap(b, dtype, cap):
+    """One key whose score, -0.9 cap, leaves it no weight, beside scores of a few: those
+    keep their 2^-20 of themselves."""
+    rng = np.random.default_rng(33)
+    T, H = 150, 2
+    k, v = (rounded(rng.standard_normal((T, H, 64)), dtype) for _ in range(2))
+    q = rounded(rng.standard_normal((T, H, 64)), dtype) * np.float32(2.0 ** round(np.log2(16384 / cap)))
+    q[..., 0], k[..., 0], k[7, :, 0] = 1.0, 0.0, -16384.0
+    scale = cap / 16384 * 0.9
+    docs, off = b.packDocs(i32(b, [T]), T), [0, T]
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, scale, cap=cap))
+    o, w, _ = ref.sdpa_packed(q, k, v, off, off, scale, cap=cap)
+    rest = np.delete(k, 7, 0).astype(np.float64)
+    e = float(np.max(scale * np.einsum("thc,jhc->htj", np.abs(q.astype(np.float64)), np.abs(rest))))
+    bad = np.abs(got - o) > capped_tolerance(dtype, o, w, e, T, cap)
+    assert np.isfinite(got).all() and not bad.any(), (bad.sum(), np.abs(got - o).max())
