@@ -42,8 +42,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Scores to base 2 (the 16-bit kernels).
 struct Score {
   float mul, c1, c2;  // mul: the factor left once a cap or slope has been applied (1), else of the products
-  float poly[5], near;  // coefficients of the capped score, and the products they hold for
-  float tiny[3], tiny_near;  // fewer of them, for smaller products
+  float g, odd[5], far;      // score / cap of a product; coefficients of the capped score in that, and the products they hold for
+  float poly[5], near;       // coefficients in the product itself
+  float tiny[3], tiny_near;  // fewer of them for smaller products
   uint32_t flip;      // a negative scale turns the query round instead
 };
 
@@ -220,21 +221,23 @@ struct Wave {
 // cancels for scores that are small against the cap (off by 2e-7 c2): it is taken past
 // 0.75 cap alone, score by score, since a tile may hold hidden scores of any size beside
 // small ones.  Within 0.75 cap the odd polynomial of degree 9 through tanh's Chebyshev
-// points there, off by 3.6e-7 at most; where that holds for every score of a tile it
-// takes 6 instructions instead of an exponential and a reciprocal at a lower rate (chunks of
-// 1000 queries over up to 8192 keys: 164 -> 153 us).  Within 0.25 cap that of degree 5,
-// off by 1e-7 at most, does, whose last product is one with the subtraction of the
-// maximum (153 -> 135 us).
-__device__ __forceinline__ float capped_near(const Score& s, float x) {
-  const float u = x * x;
-  float r = fmaf(u, s.poly[4], s.poly[3]);
+// points there, off by 3.6e-7 at most, in y = score / cap, whose square is in range
+// whatever the products.  Where every score of a tile is within 0.75 cap, the same in the
+// product itself, if its squares and the coefficients are normal numbers: 6 instructions
+// instead of an exponential and a reciprocal at a lower rate (chunks of 1000 queries over
+// up to 8192 keys: 164 -> 153 us).  Within 0.25 cap that of degree 5, off by 1e-7 at most,
+// does, whose last product is one with the subtraction of the maximum (153 -> 135 us).
+__device__ __forceinline__ float odd_polynomial(const float (&c)[5], float u, float x) {
+  float r = fmaf(u, c[4], c[3]);
 #pragma unroll
-  for (int i = 2; i >= 0; i--) r = fmaf(u, r, s.poly[i]);
+  for (int i = 2; i >= 0; i--) r = fmaf(u, r, c[i]);
   return x * r;
 }
+__device__ __forceinline__ float capped_near(const Score& s, float x) { return odd_polynomial(s.poly, x * x, x); }
 __device__ __forceinline__ float capped(const Score& s, float x) {
+  const float y = x * s.g;
   const float far = fmaf(-2.f * s.c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * s.c1)), s.c2);
-  return fabsf(x) <= s.near ? capped_near(s, x) : far;
+  return fabsf(x) <= s.far ? odd_polynomial(s.odd, y * y, x) : far;
 }
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ float score(const Score& s, float slope, int pos, int key, float x) {
@@ -250,26 +253,35 @@ __device__ __forceinline__ float tiny_factor(const Score& s, float x) {
 }
 static Score score_of(float scale, float cap, bool bias) {
   Score s{};
-  // (scale 0: any tiny factor; 0 * -inf would not be a maximum)
-  const float sl = fmaxf(fabsf(scale), 1e-30f);
+  // (scale 0: the smallest number, since 0 * -inf would not be a maximum; no product gives it
+  // a score that counts.  Finite times log2 e.)
+  constexpr float kTiny = 0x1p-149f;
+  const float sl = fminf(fmaxf(fabsf(scale), kTiny), 0x1p126f);
   const bool capped = cap > 0.f;
   s.mul = capped || bias ? 1.f : sl * kLog2e;
-  // (finite, so that 0 * c1 is 0 under the smallest caps)
-  s.c1 = capped ? fminf(2.f * sl / cap * kLog2e, FLT_MAX) : sl * kLog2e;
+  s.c1 = sl * kLog2e;
   s.c2 = cap * kLog2e;
   s.flip = scale < 0.f ? 0x80008000u : 0u;
-  // tanh(y) / y in y^2 on [0, 0.75^2]
-  const double c[5] = {0.99999942, -0.33328192, 0.13258462, -0.05004161, 0.01291665};
-  const double g = capped ? (double)sl / cap : 0.0;
-  const double c3[3] = {0.9999996, -0.33321897, 0.12841434};  // on [0, 0.25^2]
-  double f = (double)s.c2 * g;
+  if (!capped) return s;
+  const double c[5] = {0.99999942, -0.33328192, 0.13258462, -0.05004161, 0.01291665};  // tanh(y) / y in y^2 on [0, 0.75^2]
+  const double c3[3] = {0.9999996, -0.33321897, 0.12841434};                           // on [0, 0.25^2]
+  // (finite, so that 0 * c1 is 0 under the smallest caps, and inf * c1 inf under the largest)
+  const double g = std::min((double)sl / cap, (double)FLT_MAX / 4);
+  s.g = (float)g;
+  s.c1 = fmaxf((float)(2 * g * kLog2e), kTiny);
+  double f = sl * kLog2e;
+  bool normal = true;
   for (int i = 0; i < 5; i++, f *= g * g) {
+    s.odd[i] = (float)(sl * kLog2e * c[i]);
     s.poly[i] = (float)(f * c[i]);
     if (i < 3) s.tiny[i] = (float)(f * c3[i]);
+    normal = normal && std::isnormal(s.poly[i]);
+    if (i == 2) s.tiny_near = normal ? 1.f : -1.f;
   }
-  s.near = capped ? (float)(0.75 / g) : 0.f;
-  s.tiny_near = capped ? (float)(0.25 / g) : 0.f;
-  if (!std::isfinite(s.poly[4])) s.near = s.tiny_near = -1.f;  // a cap far below the scale: never those
+  // (finite: an infinite product takes the exponential)
+  s.far = (float)std::min(0.75 / g, (double)FLT_MAX);
+  s.near = normal && s.far < 0x1p63f ? s.far : -1.f;
+  s.tiny_near = s.tiny_near > 0.f && s.far < 0x1p63f ? (float)(0.25 / g) : -1.f;
   return s;
 }
 
@@ -1274,7 +1286,8 @@ extern "C" int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t*
   p.causal = causal ? 1 : 0;
   p.half = window < 0 ? -1 : (int)(window / 2 < (1ll << 30) ? window / 2 : (1ll << 30) - 1);
   p.scale = scale;
-  p.cap = fminf(cap, 0x1p100f);  // (scores below 2^88 round to themselves under either; its reciprocal is normal)
+  // (its reciprocal is normal and twice its score to base 2 finite; scores below 2^114 round to themselves under either)
+  p.cap = fminf(cap, 0x1p126f);
   p.sc = score_of(scale, p.cap, slopes != 0);
   if (packed_takes_mfma(p, dt == HB_F32 ? 4 : 8)) packed_mfma(ctx, dt, p);
   else packed_any(ctx, dt, p);

@@ -573,3 +573,70 @@ def test_attention_small_scores_beside_one_near_a_large_cap(b, dtype, cap):
     e = float(np.max(scale * np.einsum("thc,jhc->htj", np.abs(q.astype(np.float64)), np.abs(rest))))
     bad = np.abs(got - o) > capped_tolerance(dtype, o, w, e, T, cap)
     assert np.isfinite(got).all() and not bad.any(), (bad.sum(), np.abs(got - o).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap", [None, 2.0, 30.0, 1e6, 1e25, 2.0 ** 100, 3e38])
+def test_attention_of_products_whose_squares_overflow(b, dtype, cap):
+    """Products of 2^66 and more under a scale that brings them back to a few: scores,
+    and their caps, as of small products."""
+    for nq, nk in (([70, 133], [70, 133]), ([1, 2], [170, 133])):
+        rng = np.random.default_rng(34)
+        q = rounded(rng.standard_normal((sum(nq), 2, 64)), dtype) * np.float32(2.0 ** 34)
+        k = rounded(rng.standard_normal((sum(nk), 2, 64)), dtype) * np.float32(2.0 ** 34)
+        v = rounded(rng.standard_normal((sum(nk), 2, 64)), dtype)
+        scale = 2.0 ** -71
+        docs, keys = b.packDocs(i32(b, nq), sum(nq)), b.packDocs(i32(b, nk), sum(nk))
+        got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, scale, keys=keys, cap=cap))
+        o, w, e = ref.sdpa_packed(q, k, v, ref.offsets(nq, sum(nq)), ref.offsets(nk, sum(nk)), scale, cap=cap)
+        assert np.isfinite(got).all()
+        bad = np.abs(got - o) > capped_tolerance(dtype, o, w, e, max(nk), cap)
+        assert not bad.any(), (bad.sum(), np.abs(got - o).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_scores_above_2_to_the_100_under_larger_caps(b, dtype):
+    """Scores of 2^105 and 2^110 under caps of 2^120 and more: the largest has all the
+    weight, as without a cap."""
+    rng = np.random.default_rng(35)
+    T = 90
+    q, k = np.zeros((T, 1, 64), np.float32), np.zeros((T, 1, 64), np.float32)
+    q[..., 0] = 2.0 ** 50
+    k[..., 0] = (2.0 ** 55 + 2.0 ** 50 * np.arange(T))[:, None]
+    k[40, 0, 0] = 2.0 ** 60
+    v = rounded(rng.standard_normal((T, 1, 64)), dtype)
+    docs = b.packDocs(i32(b, [T]), T)
+    for cap in (None, 2.0 ** 120, 3e38):
+        got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, 1.0, cap=cap))
+        np.testing.assert_array_equal(got, np.broadcast_to(v[40], got.shape), err_msg=str(cap))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [50.0, 1e6, 1e20, 3e38])
+def test_attention_of_an_infinite_product_under_a_cap(b, dtype, cap):
+    """A visible key whose product is infinite has the cap as its score: all the weight
+    where the others stay 40 below."""
+    rng = np.random.default_rng(36)
+    q, k, v = (rounded(rng.uniform(-1, 1, (70, 2, 64)), dtype) for _ in range(3))
+    q[..., 0], k[33], k[33, :, 0] = 1.0, 0.0, np.inf
+    docs = b.packDocs(i32(b, [70]), 70)
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, 0.0625, cap=cap))
+    np.testing.assert_array_equal(got, np.broadcast_to(v[33], got.shape))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("opts", [dict(), dict(cap=3.0), dict(cap=1e9), dict(slopes=[0.25, 0.0])])
+def test_attention_of_large_products_under_small_scales(b, dtype, opts):
+    """Products around 2^115 under scales of 2^-115, of 2^-140 and of 0: scores of a few, of
+    less than any weight shows, and of nothing."""
+    opts = dict(opts)
+    rng = np.random.default_rng(37)
+    q, k, v = (rounded(rng.standard_normal((90, 2, 64)), dtype) for _ in range(3))
+    q, k = q * np.float32(2.0 ** 56), k * np.float32(2.0 ** 56)
+    off, docs, slopes = [0, 70, 90], b.packDocs(i32(b, [70, 20]), 90), opts.pop("slopes", None)
+    dev = {} if slopes is None else {"slopes": b.fromHost(HostTensor("f32", (2,), np.array(slopes, np.float32)))}
+    for scale in (2.0 ** -115, -2.0 ** -115, 2.0 ** -140, 0.0):
+        got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), docs, scale, **opts, **dev))
+        o, w, e = ref.sdpa_packed(q, k, v, off, off, scale, slopes=slopes, **opts)
+        bad = np.abs(got - o) > capped_tolerance(dtype, o, w, e, 70, opts.get("cap"))
+        assert np.isfinite(got).all() and not bad.any(), (scale, np.abs(got - o).max())
