@@ -430,7 +430,11 @@ int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t* qs, uintpt
  * y_m = x_m . w^T (+ bias, unless 0) + scales[i] * (x_m . A_i^T) . B_i^T with i =
  * index[m] (i32 [M]); a row whose index is outside [0, n) has no adapter.  The
  * bank is a [n, R, K] and b [n, N, R] of x's type and scales f32 [n]; R at
- * most 1024.  x, w, bias, y as in hb_linear (the reference has no adapters). */
+ * most 1024.  The inner products scales[i] * (x_m . A_i^T) are summed in f32 and, of
+ * 16-bit types on the matrix cores (K a multiple of 64, R of 8, operands and rows on 16
+ * bytes), rounded to the type for the product with B; those past its range (f16:
+ * 65504) stay f32, on a slow path.  x, w, bias, y as in hb_linear (the reference has no
+ * adapters). */
 int hb_lora_linear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t w, uintptr_t bias, uintptr_t y,
                    int64_t ldy, int64_t M, int64_t N, int64_t K, uintptr_t a, uintptr_t b, uintptr_t scales, int64_t n,
                    int64_t R, uintptr_t index);

@@ -451,6 +451,7 @@ __device__ __forceinline__ void ring_wait_stages(int later) {
 struct NoExt {};
 struct LoraExt {
   const void* s;         // [M, R], scaled, of x's type; rows without an adapter are not read
+  const float* wide;     // [M, R]: those elements of s that are past a 16-bit type's range, the others are not written
   const void* b;         // [n, N, R], below 2^31 bytes
   const int32_t* index;  // [M]
   int n, R;              // R a whole number of 16 bytes
@@ -470,6 +471,20 @@ __device__ __forceinline__ bool lora_mixed(const LoraExt& ext, const int* adapte
   return false;
 }
 
+// Whether an inner product of row m is finite but past the 16-bit type's range (its
+// element of s is infinite then): the row's outputs are computed again from `wide`.
+template <int DT>
+__device__ __forceinline__ bool lora_past(const LoraExt& ext, int m) {
+  if constexpr (DT == HB_F32) return false;
+  const int a = ext.index[m];
+  if (a < 0 || a >= ext.n) return false;
+  for (int r = 0; r < ext.R; r++) {
+    const int64_t i = (int64_t)m * ext.R + r;
+    if (load_f(ext.s, i, DT) * 0.f != 0.f && ext.wide[i] * 0.f == 0.f) return true;
+  }
+  return false;
+}
+
 // One output of a projection with adapters, on its own (slow: see its callers).
 template <int DT>
 __device__ __forceinline__ float lora_output(const void* X, int64_t ldx, const void* W, const void* bias, int N, int K,
@@ -478,8 +493,14 @@ __device__ __forceinline__ float lora_output(const void* X, int64_t ldx, const v
   for (int k = 0; k < K; k++) sum = fmaf(load_f(X, (int64_t)m * ldx + k, DT), load_f(W, (int64_t)n * K + k, DT), sum);
   const int a = ext.index[m];
   if (a >= 0 && a < ext.n)
-    for (int r = 0; r < ext.R; r++)
-      sum = fmaf(load_f(ext.s, (int64_t)m * ext.R + r, DT), load_f(ext.b, ((int64_t)a * N + n) * ext.R + r, DT), sum);
+    for (int r = 0; r < ext.R; r++) {
+      const int64_t i = (int64_t)m * ext.R + r;
+      float s = load_f(ext.s, i, DT);
+      if constexpr (DT != HB_F32) {
+        if (s * 0.f != 0.f) s = ext.wide[i];
+      }
+      sum = fmaf(s, load_f(ext.b, ((int64_t)a * N + n) * ext.R + r, DT), sum);
+    }
   return sum + (bias != nullptr ? load_f(bias, n, DT) : 0.f);
 }
 
@@ -719,8 +740,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
   }
   if constexpr (LORA) {
     // The zeros of other rows do not keep a non-finite B out of a row's sums (0 *
-    // inf): an output that has come out non-finite is computed again with its own
-    // row's adapter alone.
+    // inf), and an inner product may be past the type's range: an output that has come
+    // out non-finite is computed again with its own row's adapter alone.
     float z = 0.f;
 #pragma unroll
     for (int i = 0; i < TM; i++)
@@ -734,7 +755,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_ring(const uint16_t* __restr
         const int m = m0 + q / BN, n = n0 + q % BN;
         const float v = to_f<BF16>(Cs[q]);
         constexpr int DT = BF16 ? HB_BF16 : HB_F16;
-        if (m >= M || n >= N || v * 0.f == 0.f || !lora_mixed<DT>(ext, adapter, nd, N, m, n)) continue;
+        if (m >= M || n >= N || v * 0.f == 0.f) continue;
+        if (!lora_past<DT>(ext, m) && !lora_mixed<DT>(ext, adapter, nd, N, m, n)) continue;
         Cs[q] = from_f<BF16>(lora_output<DT>(X, ldx, W, bias, N, K, ext, m, n));
       }
     }

@@ -9,7 +9,9 @@
 // lora_prepare: s = scale_i x_m . A_i^T on v_mfma_f32_16x16x32 (f32: 16x16x4).  Of f16 /
 // bf16 rows it is rounded to the 16-bit type for the second product, which the
 // projection's own GEMM takes as ranks beyond K: gemm_ring with LoraExt, lora_stream
-// for large M, lora_few for few tiles.  y is rounded once.
+// for large M, lora_few for few tiles.  y is rounded once.  An element of s past the
+// type's range (f16: 65504) makes the row's outputs infinite or NaN there; they are
+// computed again one by one with its f32 value, a slow path for rows that are rare.
 //
 // lora_expand_f32: y += s . B_i^T of f32 rows past lora_few, on top of the projection.
 //
@@ -56,6 +58,7 @@ struct Prepare {
   const int32_t* index;
   int n, M, R, K;
   void* s;                   // [M, R], of x's type
+  float* wide;               // [M, R], 16-bit types: four elements of s where one of them is past the type's range
   Numbers num;
   Codes codes;
   int gx, gy, gz;            // inner products: row blocks, rank blocks, turns
@@ -185,6 +188,10 @@ __device__ __forceinline__ void lora_inner(const Prepare& p, int bx, int by, int
         constexpr bool BF16 = DT == HB_BF16;
         const uint32_t h[4] = {from_f<BF16>(v[0]), from_f<BF16>(v[1]), from_f<BF16>(v[2]), from_f<BF16>(v[3])};
         *(uint2v*)((uint16_t*)p.s + at) = uint2v{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+        float z = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) z = fmaf(to_f<BF16>((uint16_t)h[e]), 0.f, z);
+        if (z != 0.f) *(float4v*)(p.wide + at) = v;
       }
     }
     __syncthreads();  // the buffers are filled again
@@ -452,8 +459,9 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const char* __restrict__ X, 
 #pragma unroll
     for (int q = 0; q < 2; q++) {
       const int nq = min(n + q, N - 1);
-      // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf)
-      const bool alone = v[q] * 0.f != 0.f && lora_mixed<DT>(ext, adapter, nd, N, m, nq);
+      // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf), and
+      // an inner product may be past the type's range
+      const bool alone = v[q] * 0.f != 0.f && (lora_past<DT>(ext, m) || lora_mixed<DT>(ext, adapter, nd, N, m, nq));
       v[q] += bias != nullptr ? load_f(bias, nq, DT) : 0.f;
       if (alone) v[q] = lora_output<DT>(X, ldx, W, bias, N, K, ext, m, nq);
     }
@@ -749,8 +757,8 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
     if (odd) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       // the zeros of other rows do not keep a non-finite B out of a row's sums (0 *
-      // inf): an output that has come out non-finite is computed again with its own
-      // row's adapter alone
+      // inf), and an inner product may be past the type's range: an output that has come
+      // out non-finite is computed again with its own row's adapter alone
       const int* list = num.list + (int64_t)tm * kStTile;
       const int nd = num.count[tm];
 #pragma unroll 1
@@ -759,7 +767,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
         if (m >= M || n >= N) continue;
         const float v = to_f<BF16>(__builtin_nontemporal_load(Y + (int64_t)m * ldy + n));
         constexpr int DT = BF16 ? HB_BF16 : HB_F16;
-        if (v * 0.f == 0.f || !lora_mixed<DT>(ext, list, nd, N, m, n)) continue;
+        if (v * 0.f == 0.f || (!lora_past<DT>(ext, m) && !lora_mixed<DT>(ext, list, nd, N, m, n))) continue;
         Y[(int64_t)m * ldy + n] = from_f<BF16>(lora_output<DT>(X, ldx, W, bias, N, K, ext, m, n));
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -951,9 +959,10 @@ static bool lora_fused(uintptr_t ctx, int dt, const uint16_t* x, int64_t ldx, co
   const int cus = cu_count(ctx);
   const int tiles = lora_streams(cus, M, N, bias, y, ldy) ? (M + kStTile - 1) / kStTile : 0;
   const int64_t rows = (int64_t)tiles * kStTile, s_bytes = ((int64_t)M * l.R * 2 + 255) / 256 * 256;
+  const int64_t wide_bytes = 2 * s_bytes;
   CallScratch held(ctx);
   const int64_t w_bytes = codes.bits ? (int64_t)N * K * 2 : 0;  // (K % 64 == 0)
-  if (!held.take((size_t)(w_bytes + s_bytes + rows * 6 + tiles * 4))) return false;
+  if (!held.take((size_t)(w_bytes + s_bytes + wide_bytes + rows * 6 + tiles * 4))) return false;
   Prepare p{(const char*)x, ldx, (const char*)l.a, (const float*)l.scales, (const int32_t*)l.index, (int)l.n, M, (int)l.R, K};
   if (codes.bits) {
     codes.blocks = (int)std::min<int64_t>(((int64_t)N * K / 8 + 1023) / 1024, (int64_t)cus * 16);
@@ -963,14 +972,15 @@ static bool lora_fused(uintptr_t ctx, int dt, const uint16_t* x, int64_t ldx, co
   }
   p.codes = codes;
   p.s = (char*)held.p + w_bytes;
-  p.num.list = (int32_t*)((char*)p.s + s_bytes);
+  p.wide = (float*)((char*)p.s + s_bytes);
+  p.num.list = (int32_t*)((char*)p.wide + wide_bytes);
   p.num.count = p.num.list + rows;
   p.num.number = (int16_t*)(p.num.count + tiles);
   p.num.tiles = tiles;
   hipStream_t st = stream_of(ctx);
   launch_prepare(st, cus, dt, p);
   check_launch("hb_lora_linear");
-  const LoraExt ext{p.s, (const void*)l.b, p.index, p.n, p.R};
+  const LoraExt ext{p.s, p.wide, (const void*)l.b, p.index, p.n, p.R};
   if (dt == HB_BF16) lora_gemm<true>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
   else lora_gemm<false>(st, cus, x, ldx, w, bias, y, ldy, M, N, K, ext, p.num);
   check_launch("hb_lora_linear");
@@ -999,7 +1009,7 @@ static bool lora_few_f32(uintptr_t ctx, uintptr_t x, int64_t ldx, uintptr_t w, u
   if (w % 16 != 0 || l.n * l.R * N * 4 >= (1ll << 31) || M * l.R * 4 >= (1ll << 31)) return false;
   const int cus = cu_count(ctx);
   hipStream_t st = stream_of(ctx);
-  LoraExt ext{nullptr, (const void*)l.b, (const int32_t*)l.index, (int)l.n, (int)l.R};
+  LoraExt ext{nullptr, nullptr, (const void*)l.b, (const int32_t*)l.index, (int)l.n, (int)l.R};
   auto few = [&](bool launch) {
     return lora_few_tiles<HB_F32>(st, cus, (const void*)x, ldx, (const void*)w, (const void*)bias, (void*)y, ldy, (int)M,
                                   (int)N, (int)K, ext, launch);

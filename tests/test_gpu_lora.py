@@ -258,3 +258,72 @@ def test_lora_recorded(b, M):
     out = g.out
     g.destroy()
     b.dispose(out)
+
+
+# ------------------------------------------------------------------ inner products past the 16-bit type, what stays with its rows
+
+# one of each kernel's sizes: lora_few (16 x 16, 16 x 32, 32 x 16, 32 x 32 and 64 x 64 tiles), gemm_ring's tiles, lora_stream (256
+# and 192 wide), and the general path
+KERNELS = [(9, 64, 64), (16, 5250, 64), (48, 520, 128), (130, 2304, 128), (400, 2304, 128), (700, 1024, 192), (1900, 768, 64),
+           (3000, 520, 64), (4100, 2064, 64), (33000, 256, 64), (200, 130, 72)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", KERNELS)
+def test_lora_inner_products_past_f16(b, dtype, M, N, K):
+    """Adapters whose inner products pass 65504 beside small B: y is finite, and theirs
+    (the tolerance counts the inner products' rounding, which those past the type do not have)."""
+    rng = np.random.default_rng(M)
+    c = case(rng, dtype, M, N, K, 4, 8, index=np.arange(M) // 3 % 6 - 1, bias=True)
+    for i in (1, 3):  # one of them in a single rank
+        r = slice(None) if i == 1 else slice(2, 3)
+        c["a"][i, r] = rounded(c["a"][i, r] * 4000, dtype)
+        c["b"][i, :, r] = rounded(c["b"][i, :, r] * 0.01, dtype)
+        c["scales"][i] = 64.0
+    x, bank, index, bias = dev(b, c, dtype)
+    got = read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index, bias))
+    s = 64.0 * c["x"].astype(np.float64) @ c["a"][1].astype(np.float64).T
+    assert (np.abs(s) > 65520).mean() > 0.1
+    y = ref.lora_linear(c["x"], c["w"], c["bias"], c["a"], c["b"], c["scales"].astype(np.float64), c["index"])[0]
+    assert dtype != "f16" or np.abs(y).max() < 65000
+    check(got, c, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("bits,mode", [(8, "symmetric"), (4, "affine")])
+def test_lora_inner_products_past_f16_on_quantized_weights(b, dtype, bits, mode):
+    rng = np.random.default_rng(bits)
+    c = case(rng, dtype, 300, 520, 128, 3, 8, bias=True)
+    c["a"][1], c["b"][1], c["scales"][1] = rounded(c["a"][1] * 4000, dtype), rounded(c["b"][1] * 0.01, dtype), 64.0
+    q = b.fromHostQuantized(quantized(rng, 520, 128, bits, mode, 64), dtype)
+    x, bank, index, bias = dev(b, c, dtype)
+    got = read32(b, lora_linear_any(b, x, q, bank, index, bias))
+    w = read32(b, b.quantizedLinear(b.fromHost(to_host(np.eye(128), dtype)), q.w, q.scales, q.biases, q)).T
+    check(got, c, dtype, w=w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+@pytest.mark.parametrize("M,N,K", KERNELS)
+def test_lora_non_finite_elements_stay_with_their_rows(b, dtype, what, M, N, K):
+    """Non-finite elements of two adapters' B, of a third's A and of a row of x, with a
+    fourth whose inner products pass 65504: on every kernel, the other outputs are theirs."""
+    rng = np.random.default_rng(M + 1)
+    c = case(rng, dtype, M, N, K, 6, 8, index=np.arange(M) // 2 % 7 - 1)
+    c["a"][5], c["b"][5], c["scales"][5] = rounded(c["a"][5] * 4000, dtype), rounded(c["b"][5] * 0.01, dtype), 64.0
+    dirty = {k: v.copy() for k, v in c.items() if v is not None}
+    dirty["bias"] = None
+    cols = np.array([1, 2, N // 2, N - 1])
+    dirty["b"][1, cols, 3], dirty["b"][4, 2:4, 0], dirty["a"][2, 3, 5], dirty["x"][0, 1] = what, what, what, what
+    x, bank, index, _ = dev(b, dirty, dtype)
+    got = read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index))
+    lost = np.zeros((M, N), bool)
+    lost[np.ix_(c["index"] == 1, cols)] = True
+    lost[np.ix_(c["index"] == 4, [2, 3])] = True
+    lost[c["index"] == 2], lost[0] = True, True
+    assert not np.isfinite(got[lost]).any()
+    y, mass, delta = ref.lora_linear(c["x"], c["w"], None, c["a"], c["b"], c["scales"].astype(np.float64), c["index"])
+    u = U[dtype]
+    tol = u * np.abs(y) + u * delta + u * np.minimum(mass, np.abs(y) + 2 * delta) + (K + 16) * 2.0 ** -23 * (mass + delta)
+    bad = ~(np.abs(got - y) <= tol + 1e-30) & ~lost
+    assert not bad.any(), f"{bad.sum()}, first at {np.argwhere(bad)[0]}"
