@@ -448,6 +448,8 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const char* __restrict__ X, 
     for (int j = 0; j < TN; j++) *(float4v*)&red[wave][16 * i + l16][16 * j + 4 * g] = acc[i][j];
   __syncthreads();
   constexpr int CW = TN * 8;  // threads of a row
+  static_assert(NW * 64 % CW == 0, "a thread has the same two columns in every row");
+  int dirty[2] = {kUnknown, kUnknown};
   for (int at = tid; at < TM * 16 * CW; at += NW * 64) {
     const int row = at / CW, col = at % CW * 2, m = m0 + row, n = n0 + col;
     if (m >= M || n >= N) continue;
@@ -461,7 +463,12 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const char* __restrict__ X, 
       const int nq = min(n + q, N - 1);
       // the zeros of other rows do not keep a non-finite B out of a row's sums (0 * inf), and
       // an inner product may be past the type's range
-      const bool alone = v[q] * 0.f != 0.f && (lora_past<DT>(ext, m) || lora_mixed<DT>(ext, adapter, nd, N, m, nq));
+      bool alone = false;
+      if (v[q] * 0.f != 0.f) {
+        alone = lora_past<DT>(ext, m);
+        if (!alone && dirty[q] == kUnknown) dirty[q] = lora_dirty<DT>(ext, adapter, nd, N, nq);
+        alone = alone || lora_mixed(ext, dirty[q], m);
+      }
       v[q] += bias != nullptr ? load_f(bias, nq, DT) : 0.f;
       if (alone) v[q] = lora_output<DT>(X, ldx, W, bias, N, K, ext, m, nq);
     }
@@ -762,13 +769,19 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
       const int* list = num.list + (int64_t)tm * kStTile;
       const int nd = num.count[tm];
 #pragma unroll 1
-      for (int q = lane; q < TM * TN * 1024; q += 64) {
-        const int m = m0 + q / (TN * 32), n = n0 + q % (TN * 32);
-        if (m >= M || n >= N) continue;
-        const float v = to_f<BF16>(__builtin_nontemporal_load(Y + (int64_t)m * ldy + n));
-        constexpr int DT = BF16 ? HB_BF16 : HB_F16;
-        if (v * 0.f == 0.f || (!lora_past<DT>(ext, m) && !lora_mixed<DT>(ext, list, nd, N, m, n))) continue;
-        Y[(int64_t)m * ldy + n] = from_f<BF16>(lora_output<DT>(X, ldx, W, bias, N, K, ext, m, n));
+      for (int n = n0 + lane; n < min(n0 + TN * 32, N); n += 64) {
+        int dirty = kUnknown;
+#pragma unroll 1
+        for (int m = m0; m < min(m0 + TM * 32, M); m++) {
+          const float v = to_f<BF16>(__builtin_nontemporal_load(Y + (int64_t)m * ldy + n));
+          constexpr int DT = BF16 ? HB_BF16 : HB_F16;
+          if (v * 0.f == 0.f) continue;
+          if (!lora_past<DT>(ext, m)) {
+            if (dirty == kUnknown) dirty = lora_dirty<DT>(ext, list, nd, N, n);
+            if (!lora_mixed(ext, dirty, m)) continue;
+          }
+          Y[(int64_t)m * ldy + n] = from_f<BF16>(lora_output<DT>(X, ldx, W, bias, N, K, ext, m, n));
+        }
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }

@@ -327,3 +327,14 @@ def test_lora_non_finite_elements_stay_with_their_rows(b, dtype, what, M, N, K):
     tol = u * np.abs(y) + u * delta + u * np.minimum(mass, np.abs(y) + 2 * delta) + (K + 16) * 2.0 ** -23 * (mass + delta)
     bad = ~(np.abs(got - y) <= tol + 1e-30) & ~lost
     assert not bad.any(), f"{bad.sum()}, first at {np.argwhere(bad)[0]}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(130, 2304, 128), (1900, 768, 64), (4100, 2064, 64)])
+def test_lora_of_non_finite_rows(b, dtype, M, N, K):
+    """Every row non-finite, every row with an adapter of its own: no finite output."""
+    rng = np.random.default_rng(M + 2)
+    c = case(rng, dtype, M, N, K, 300, 64, index=rng.integers(0, 300, M))
+    c["x"][:, K - 1] = np.nan
+    x, bank, index, _ = dev(b, c, dtype)
+    assert np.isnan(read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index))).all()
