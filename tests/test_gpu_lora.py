@@ -338,3 +338,18 @@ def test_lora_of_non_finite_rows(b, dtype, M, N, K):
     c["x"][:, K - 1] = np.nan
     x, bank, index, _ = dev(b, c, dtype)
     assert np.isnan(read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], dtype)), bank, index))).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(3000, 520, 128), (1900, 768, 64), (4100, 2064, 64), (8200, 2304, 64), (33000, 256, 64)])
+def test_lora_rows_without_an_adapter_are_linear(b, dtype, M, N, K):
+    """On the tiles that sum K in the linear layers' order, rows without an adapter have
+    `linear`'s bits, whatever their neighbours' adapters."""
+    rng = np.random.default_rng(M + 3)
+    c = case(rng, dtype, M, N, K, 5, 16, index=rng.integers(-1, 6, M), bias=True)
+    x, bank, index, bias = dev(b, c, dtype)
+    w = b.fromHost(to_host(c["w"], dtype))
+    got, plain = read32(b, b.loraLinear(x, w, bank, index, bias)), read32(b, b.linear(x, w, bias))
+    none = (c["index"] < 0) | (c["index"] >= 5)
+    assert none.sum() > M // 10
+    np.testing.assert_array_equal(got[none], plain[none])
