@@ -821,12 +821,11 @@ class HipBackend:
         self._call("copy", "hb_unary", self.ctx, op, DT[t.dtype][0], self._ptr(t), F.i64s(xs), DT[dd][0], dst_ptr,
                    ys, F.i64s(shape), len(shape), alpha)
 
-    def _rows(self, t: HipTensor):
-        """(storage, ptr, rows, K, ld) for a tensor whose leading dims collapse
-        to rows of stride ld with a contiguous last dim; copies otherwise."""
-        self._ready(t)
+    @staticmethod
+    def _row_stride(t: HipTensor) -> Optional[int]:
+        """The stride of t's rows if its leading dims collapse to rows with a
+        contiguous last dim, else None."""
         K = t.shape[-1] if t.shape else 1
-        rows = _numel(t.shape[:-1])
         ok = len(t.shape) >= 1 and (t._strides[-1] == 1 or K == 1)
         ld = K
         if ok and len(t.shape) >= 2:
@@ -839,10 +838,18 @@ class HipBackend:
                         ok = False
                 if ld < K:
                     ok = False
-        if not ok:
+        return ld if ok else None
+
+    def _rows(self, t: HipTensor):
+        """(storage, ptr, rows, K, ld) for a tensor whose leading dims collapse
+        to rows of stride ld with a contiguous last dim; copies otherwise."""
+        self._ready(t)
+        K = t.shape[-1] if t.shape else 1
+        ld = self._row_stride(t)
+        if ld is None:
             t = self._contiguous(t)
             ld = K
-        return (t._st, self._ptr(t), rows, K, ld)
+        return (t._st, self._ptr(t), _numel(t.shape[:-1]), K, ld)
 
     @staticmethod
     def _bhld(shape):
@@ -2038,6 +2045,9 @@ class HipBackend:
         idx = self._plain(index, "i32", tmp)
         if bias is not None:
             bias = self._plain(bias, x.dtype, tmp)
+        if self._row_stride(self._ready(x)) is None:
+            x = self._contiguous(x)
+            tmp.append(x)
         _, xp, M, _, ldx = self._rows(x)
         out = self._new(x.shape[:-1] + (N,), x.dtype)
         tail = (self._ptr(bank.a), self._ptr(bank.b), self._ptr(bank.scales), bank.count, bank.held_rank, self._ptr(idx))

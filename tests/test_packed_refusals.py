@@ -206,3 +206,26 @@ def test_bank_holds_no_more_than_its_tensors(b, rank):
     for t in (*given, swapped, view):
         b.dispose(t)
     assert len(stores) > 4 and all(s.refs == 0 for s in stores)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_adapters_hold_no_copy_of_strided_rows(b, quantized):
+    """A copy of rows that do not lie behind one another, and the other operands' copies,
+    end with the call; rows inside wider ones are not copied."""
+    from types import SimpleNamespace
+    stores, malloc = [], b._malloc
+    b._malloc = lambda n: (stores.append(malloc(n)), stores[-1])[1]
+    x, w, bias, index = b.t(64, 5), b.t(64, 32), b.t(32, dtype="f32"), b.t(5, dtype="u8")
+    wide, codes, scales = b.t(5, 96), b.t(32, 64, dtype="u8"), b.t(32, 1)
+    bank = b.loraBank(b.t(3, 8, 64), b.t(3, 32, 8), b.t(3, dtype="f32"))
+    opts = SimpleNamespace(bits=8, groupSize=64, mode="symmetric")
+    for rows, ldx in ((b.transpose(x, [1, 0]), 64), (b.slice(wide, [0, 16], [5, 80]), 96)):
+        live = [s for s in stores if s.refs]
+        if quantized:
+            y = b.quantizedLoraLinear(rows, codes, scales, None, opts, bank, index, bias)
+        else:
+            y = b.loraLinear(rows, b.transpose(w, [1, 0]), bank, index, bias)
+        b.dispose(y)
+        assert [s for s in stores if s.refs] == live
+        name, args = b.calls[-1]
+        assert name == ("hb_lora_qlinear" if quantized else "hb_lora_linear") and args[3] == ldx
