@@ -261,6 +261,13 @@ inline unsigned grid_for(int64_t n, int block) {
   return (unsigned)(g < 1 ? 1 : g);
 }
 
+// Blocks of `threads` threads for `blocks` blocks' work, for kernels that go round with
+// the grid's stride: a launch holds fewer than 2^32 threads a dimension.
+inline unsigned capped_grid(int64_t blocks, int threads) {
+  const int64_t most = ((1ll << 32) - 1) / threads;
+  return (unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+}
+
 // Blocks are dealt to the 8 XCDs in turn (block b runs on XCD b % 8, each
 // XCD with its own L2).  This maps block `bid` of `nb` to a work index so
 // that every XCD takes one contiguous run of indices, in order: work items

@@ -298,7 +298,7 @@ static void launch_prepare(hipStream_t st, int cus, int dt, Prepare& p) {
   const bool narrow = p.R <= 16 || (!large && (int64_t)p.gx * p.gy * p.gz < cus);  // 16 ranks a block
   if (narrow) p.gy = (p.R + 15) / 16;
   const int64_t blocks = (int64_t)p.gx * p.gy * p.gz + p.num.tiles + p.codes.blocks;
-  HB_REQUIRE(blocks < (1ll << 31), "hb_lora_linear: too many rows and ranks");
+  HB_REQUIRE(blocks < (1ll << 24), "hb_lora_linear: too many rows and ranks");  // (2^32 threads)
   auto go = [&](auto kernel, std::atomic<uint64_t>& attr, int mt, int nt) {
     const int lds = 4 * 2 * (mt + nt) * 2048;
     if (lds > 64 * 1024)
@@ -912,17 +912,17 @@ __global__ __launch_bounds__(256) void lora_shrink_any(int dt, const void* __res
                                                        const int32_t* __restrict__ index, int n, int64_t M, int R,
                                                        int K, float* __restrict__ S) {
   const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= M * R) return;
-  const int64_t m = i / R;
-  const int r = (int)(i - m * R), a = index[m];
-  float s = 0.f;
-  if (a >= 0 && a < n) {
-    const int64_t row = ((int64_t)a * R + r) * K;
-    for (int k = lane; k < K; k += 64) s = fmaf(load_f(X, m * ldx + k, dt), load_f(A, row + k, dt), s);
-    s = wave_sum(s) * scales[a];
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < M * R; i += (int64_t)gridDim.x * 4) {
+    const int64_t m = i / R;
+    const int r = (int)(i - m * R), a = index[m];
+    float s = 0.f;
+    if (a >= 0 && a < n) {
+      const int64_t row = ((int64_t)a * R + r) * K;
+      for (int k = lane; k < K; k += 64) s = fmaf(load_f(X, m * ldx + k, dt), load_f(A, row + k, dt), s);
+      s = wave_sum(s) * scales[a];
+    }
+    if (lane == 0) S[i] = s;
   }
-  if (lane == 0) S[i] = s;
 }
 
 // One thread per output.
@@ -1055,8 +1055,7 @@ static void add_adapters(uintptr_t ctx, const char* op, int dt, uintptr_t x, int
                                             (int)N, (int)l.R, (float*)y, ldy);
     return check_launch(op);
   }
-  HB_REQUIRE((M * l.R + 3) / 4 < (1ll << 31), "hb_lora_linear: too many rows and ranks");
-  lora_shrink_any<<<(unsigned)((M * l.R + 3) / 4), 256, 0, st>>>(dt, (const void*)x, ldx, (const void*)l.a,
+  lora_shrink_any<<<capped_grid((M * l.R + 3) / 4, 256), 256, 0, st>>>(dt, (const void*)x, ldx, (const void*)l.a,
                                                                  (const float*)l.scales, (const int32_t*)l.index,
                                                                  (int)l.n, M, (int)l.R, (int)K, (float*)s.p);
   const dim3 grid((unsigned)((N + 255) / 256), (unsigned)(M < 65535 ? M : 65535));

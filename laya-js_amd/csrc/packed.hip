@@ -135,25 +135,26 @@ __global__ __launch_bounds__(256) void move_rows_kernel(const V* __restrict__ sr
                                                         const int32_t* __restrict__ idx, int L, int64_t rows,
                                                         V* __restrict__ out) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (r >= rows) return;
-  int64_t s;
-  if constexpr (UNPACK) {
-    const int64_t b = r / L, l = r - b * L, o = idx[b], n = idx[b + 1] - o;
-    s = l < n ? o + l : -1;
-  } else {
-    s = idx[r];
+  for (int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows;
+       r += (int64_t)gridDim.x * 4) {
+    int64_t s;
+    if constexpr (UNPACK) {
+      const int64_t b = r / L, l = r - b * L, o = idx[b], n = idx[b + 1] - o;
+      s = l < n ? o + l : -1;
+    } else {
+      s = idx[r];
+    }
+    const bool ok = s >= 0 && s < nsrc;
+    const V* from = src + (ok ? s : 0) * vecs;
+    V* to = out + r * vecs;
+    for (int64_t i = lane; i < vecs; i += 64) to[i] = ok ? from[i] : V{};
   }
-  const bool ok = s >= 0 && s < nsrc;
-  const V* from = src + (ok ? s : 0) * vecs;
-  V* to = out + r * vecs;
-  for (int64_t i = lane; i < vecs; i += 64) to[i] = ok ? from[i] : V{};
 }
 
 template <bool UNPACK>
 static void launch_move_rows(hipStream_t st, uintptr_t src, int64_t nsrc, int64_t row_bytes, const int32_t* idx, int L,
                              int64_t rows, uintptr_t out) {
-  const unsigned grid = (unsigned)((rows + 3) / 4);
+  const unsigned grid = capped_grid((rows + 3) / 4, 256);
   auto go = [&](auto v) {
     using V = decltype(v);
     move_rows_kernel<V, UNPACK><<<grid, 256, 0, st>>>((const V*)src, nsrc, row_bytes / (int64_t)sizeof(V), idx, L, rows,
@@ -229,7 +230,9 @@ __global__ __launch_bounds__(256) void rope_at_vec_kernel(const T* __restrict__ 
                                                           T* __restrict__ y, int T_, int H, int D, int tb,
                                                           const int32_t* __restrict__ positions, RopeAt f) {
   extern __shared__ float2 cs[];  // [tb][D / 2]
-  const int half = D / 2, C = half / V, t0 = blockIdx.x * tb, nt = T_ - t0 < tb ? T_ - t0 : tb;
+  const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * tb;
+  if (first >= T_) return;  // (the whole block)
+  const int half = D / 2, C = half / V, t0 = (int)first, nt = T_ - t0 < tb ? T_ - t0 : tb;
   for (int i = threadIdx.x; i < nt * half; i += 256) cs[i] = rope_at_cs(f, positions, T_, t0 + i / half, i % half);
   __syncthreads();
   const int per = H * C, n = nt * per;
@@ -354,7 +357,9 @@ int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t 
   const int per = dt == HB_F32 ? 4 : 8;  // values of a 16-byte chunk
   if (D / 2 % per == 0 && xs[2] == 1 && xs[0] % per == 0 && xs[1] % per == 0 && x % 16 == 0 && y % 16 == 0) {
     const int tb = T >= 2048 ? kRopeTokens : 1;
-    const unsigned grid = (unsigned)((T + tb - 1) / tb);
+    const int64_t blocks = (T + tb - 1) / tb;
+    const unsigned gx = capped_grid(blocks, 256);
+    const dim3 grid(gx, (unsigned)((blocks + gx - 1) / gx));
     const size_t lds = (size_t)tb * (D / 2) * sizeof(float2);
     auto go = [&](auto kern, auto v) {
       using E = decltype(v);
@@ -365,7 +370,7 @@ int hb_rope_at(uintptr_t ctx, int dt, uintptr_t x, const int64_t* xs, uintptr_t 
     else if (dt == HB_F16) go(rope_at_vec_kernel<uint16_t, 8, false>, (uint16_t)0);
     else go(rope_at_vec_kernel<uint16_t, 8, true>, (uint16_t)0);
   } else {
-    rope_at_kernel<<<grid_for(T * H * (D / 2), 256), 256, 0, stream_of(ctx)>>>(
+    rope_at_kernel<<<capped_grid((T * H * (D / 2) + 255) / 256, 256), 256, 0, stream_of(ctx)>>>(
         dt, (const void*)x, xs[0], xs[1], xs[2], (void*)y, T, H, (int)D, (const int32_t*)positions, f);
   }
   check_launch("hb_rope_at");

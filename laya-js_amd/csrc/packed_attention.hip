@@ -1097,65 +1097,71 @@ constexpr int kAnyCols = 8;  // columns per lane: D <= 512
 __global__ __launch_bounds__(64) void packed_attn_any(Packed p, int dt) {
   extern __shared__ float sh[];  // [D] query, [64] weights
   float* w = sh + p.D;
-  const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, D = p.D;
-  const uint32_t b = (uint32_t)p.doc[t];
-  const Seen d = seen_by(p, packed_doc(p, b < (uint32_t)p.B ? (int)b : p.B), t);
-  for (int c = lane; c < D; c += 64) sh[c] = load_f(p.Q, t * p.qs[0] + h * p.qs[1] + c * p.qs[2], dt);
-  __syncthreads();
-  const float slope = p.slopes == nullptr ? 0.f : p.slopes[h];
-  float o[kAnyCols] = {}, m = -INFINITY, l = 0.f;
-  const int64_t kh = (h / p.G) * p.ks[1], vh = (h / p.G) * p.vs[1];
-  const int bound = max(d.end, d.pend);
-  for (int j0 = d.p0; j0 < bound; j0 += 64) {
-    // (the same in every lane: nothing of these keys is visible)
-    if (j0 >= d.pend && (j0 >= d.end || j0 + 64 <= d.lo)) continue;
-    const int j = j0 + lane;
-    const bool seen = j < d.pend || (j >= d.lo && j < d.end);
-    float x = -INFINITY;
-    if (seen) {
-      const int64_t row = (int64_t)j * p.ks[0] + kh;
-      float a = 0.f;
-      for (int c = 0; c < D; c++) a = fmaf(sh[c], load_f(p.K, row + c * p.ks[2], dt), a);
-      x = a * p.scale;
-      if (p.cap > 0.f) x = p.cap * tanhf(x / p.cap);
-      x -= slope * fabsf((float)(d.pos - j));
-    }
-    const float mn = fmaxf(m, wave_max(x));
-    const float mc = mn == -INFINITY ? 0.f : mn, alpha = expf(m - mc);
-    m = mn;
-    const float pr = seen ? expf(x - mc) : 0.f;  // (NaN scores stay NaN)
-    l = l * alpha + wave_sum(pr);
-    __syncthreads();  // the last keys' weights are used up
-    w[lane] = pr;
+  const int lane = threadIdx.x, h = blockIdx.y, D = p.D;
+  for (int64_t t64 = blockIdx.x; t64 < p.Tq; t64 += gridDim.x) {
+    const int t = (int)t64;
+    __syncthreads();  // the last query and weights are used up
+    const uint32_t b = (uint32_t)p.doc[t];
+    const Seen d = seen_by(p, packed_doc(p, b < (uint32_t)p.B ? (int)b : p.B), t);
+    for (int c = lane; c < D; c += 64) sh[c] = load_f(p.Q, t * p.qs[0] + h * p.qs[1] + c * p.qs[2], dt);
     __syncthreads();
-    for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++) {
-      float a = o[i] * alpha;
-      const int64_t col = vh + (i * 64 + lane) * p.vs[2];
-      for (int k = 0; k < 64 && j0 + k < bound; k++)
-        if (w[k] != 0.f) a = fmaf(w[k], load_f(p.V, (int64_t)(j0 + k) * p.vs[0] + col, dt), a);
-      o[i] = a;
+    const float slope = p.slopes == nullptr ? 0.f : p.slopes[h];
+    float o[kAnyCols] = {}, m = -INFINITY, l = 0.f;
+    const int64_t kh = (h / p.G) * p.ks[1], vh = (h / p.G) * p.vs[1];
+    const int bound = max(d.end, d.pend);
+    for (int j0 = d.p0; j0 < bound; j0 += 64) {
+      // (the same in every lane: nothing of these keys is visible)
+      if (j0 >= d.pend && (j0 >= d.end || j0 + 64 <= d.lo)) continue;
+      const int j = j0 + lane;
+      const bool seen = j < d.pend || (j >= d.lo && j < d.end);
+      float x = -INFINITY;
+      if (seen) {
+        const int64_t row = (int64_t)j * p.ks[0] + kh;
+        float a = 0.f;
+        for (int c = 0; c < D; c++) a = fmaf(sh[c], load_f(p.K, row + c * p.ks[2], dt), a);
+        x = a * p.scale;
+        if (p.cap > 0.f) x = p.cap * tanhf(x / p.cap);
+        x -= slope * fabsf((float)(d.pos - j));
+      }
+      const float mn = fmaxf(m, wave_max(x));
+      const float mc = mn == -INFINITY ? 0.f : mn, alpha = expf(m - mc);
+      m = mn;
+      const float pr = seen ? expf(x - mc) : 0.f;  // (NaN scores stay NaN)
+      l = l * alpha + wave_sum(pr);
+      __syncthreads();  // the last keys' weights are used up
+      w[lane] = pr;
+      __syncthreads();
+      for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++) {
+        float a = o[i] * alpha;
+        const int64_t col = vh + (i * 64 + lane) * p.vs[2];
+        for (int k = 0; k < 64 && j0 + k < bound; k++)
+          if (w[k] != 0.f) a = fmaf(w[k], load_f(p.V, (int64_t)(j0 + k) * p.vs[0] + col, dt), a);
+        o[i] = a;
+      }
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++)
+      store_f(p.O, ((int64_t)t * p.H + h) * D + i * 64 + lane, dt, o[i] * inv);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int i = 0; i < kAnyCols && i * 64 + lane < D; i++)
-    store_f(p.O, ((int64_t)t * p.H + h) * D + i * 64 + lane, dt, o[i] * inv);
 }
 
 // ------------------------------------------------------------------ dispatch
 
 // The MFMA kernels' conditions: D = 64, unit column strides, 16-byte aligned rows
-// (`per` elements), and K / V row strides that 32-bit offsets within a tile reach.
+// (`per` elements), K / V row strides that 32-bit offsets within a tile reach, and fewer
+// than 2^32 threads in their grids.
 static bool packed_takes_mfma(const Packed& p, int per) {
   auto rows16 = [&](const void* t, const int64_t* s) {
     return (uintptr_t)t % 16 == 0 && s[2] == 1 && s[0] % per == 0 && s[1] % per == 0;
   };
   auto near = [](int64_t s) { return s >= 0 && s < (1 << 23); };
-  return p.D == 64 && (int64_t)p.Tq * p.G < (1ll << 30) && rows16(p.Q, p.qs) && rows16(p.K, p.ks) && rows16(p.V, p.vs) && near(p.ks[0]) && near(p.vs[0]) &&
+  const int64_t blocks = std::max((int64_t)p.Tq * p.G / 32 + p.B + 1, (int64_t)p.nblocks * p.G) * (p.H / p.G);
+  return p.D == 64 && (int64_t)p.Tq * p.G < (1ll << 30) && blocks < (1ll << 24) && rows16(p.Q, p.qs) && rows16(p.K, p.ks) && rows16(p.V, p.vs) && near(p.ks[0]) && near(p.vs[0]) &&
          (uintptr_t)p.O % 16 == 0;
 }
 
 static void packed_any(uintptr_t ctx, int dt, const Packed& p) {
-  packed_attn_any<<<dim3((unsigned)p.Tq, (unsigned)p.H), 64, (size_t)(p.D + 64) * 4, stream_of(ctx)>>>(p, dt);
+  packed_attn_any<<<dim3(capped_grid(p.Tq, 64), (unsigned)p.H), 64, (size_t)(p.D + 64) * 4, stream_of(ctx)>>>(p, dt);
 }
 
 template <class K>
@@ -1166,7 +1172,7 @@ static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, in
       HB_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     });
   const int64_t grid = blocks * (p.H / p.G);
-  HB_REQUIRE(grid < (1ll << 31), "hb_sdpa_packed: too many rows and heads");
+  HB_REQUIRE(grid < (1ll << 24), "hb_sdpa_packed: too many rows and heads");  // (packed_takes_mfma)
   kern<<<dim3((unsigned)grid, (unsigned)splits), 256, (size_t)lds, stream_of(ctx)>>>(p, part, splits);
 }
 

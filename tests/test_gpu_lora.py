@@ -353,3 +353,13 @@ def test_lora_rows_without_an_adapter_are_linear(b, dtype, M, N, K):
     none = (c["index"] < 0) | (c["index"] >= 5)
     assert none.sum() > M // 10
     np.testing.assert_array_equal(got[none], plain[none])
+
+
+def test_lora_of_more_than_2_to_the_26_inner_products(b):
+    """A wave an inner product is 2^32 threads from 2^26 of them on."""
+    rng = np.random.default_rng(45)
+    M, N, K, R = 2 ** 16 + 9, 8, 8, 1024
+    c = case(rng, "f16", M, N, K, 1, R, index=np.arange(M) % 2 - 1)
+    x, bank, index, _ = dev(b, c, "f16")
+    got = read32(b, b.loraLinear(x, b.fromHost(to_host(c["w"], "f16")), bank, index))
+    check(got, c, "f16")

@@ -640,3 +640,79 @@ def test_attention_of_large_products_under_small_scales(b, dtype, opts):
         o, w, e = ref.sdpa_packed(q, k, v, off, off, scale, slopes=slopes, **opts)
         bad = np.abs(got - o) > capped_tolerance(dtype, o, w, e, 70, opts.get("cap"))
         assert np.isfinite(got).all() and not bad.any(), (scale, np.abs(got - o).max())
+
+
+# ------------------------------------------------------------------ more than 2^32 threads' work
+
+def test_rows_of_more_than_2_to_the_26(b):
+    """A wave a row is 2^32 threads from 2^26 rows on."""
+    rng = np.random.default_rng(41)
+    count, L, T = 2 ** 16 + 16, 1024, 100
+    n = np.zeros(count, np.int32)
+    n[[0, 5, count - 1]] = 30, 40, 25
+    x = rng.integers(1, 100, T).astype(np.uint8)
+    p = b.packDocs(i32(b, n), T, L)
+    slots = ref.plan([30, 40, 25], T, L)[3]
+    slots = np.where(slots < 0, -1, np.array([0, 5, count - 1])[slots // L] * L + slots % L)
+    got = b.read(b.unpackRows(b.fromHost(HostTensor("u8", (T,), x)), p)).data.reshape(-1)
+    want = np.zeros(count * L, np.uint8)
+    want[slots[slots >= 0]] = x[slots >= 0]
+    np.testing.assert_array_equal(got, want)
+    p.dispose()
+    T = 2 ** 26 + 5
+    p = b.packDocs(i32(b, [T - 9, 3, 2]), T, T - 9)
+    back = b.packRows(b.unpackRows(b.fromHost(HostTensor("u8", (T,), np.arange(T, dtype=np.uint64).astype(np.uint8))), p), p)
+    got = b.read(back).data
+    np.testing.assert_array_equal(got[:T - 4], np.arange(T - 4, dtype=np.uint64).astype(np.uint8))
+    assert (got[T - 4:] == 0).all()
+    b.dispose(back)
+    p.dispose()
+
+
+def test_rope_at_of_more_than_2_to_the_27_rows(b):
+    """Rows shared by all tokens (stride 0) at positions of their own."""
+    T, D = 2 ** 27 + 11, 16
+    x = rounded(np.random.default_rng(42).standard_normal((1, 1, D)), "f16")
+    one = b.fromHost(to_host(x, "f16"))
+    rows = b._view(one, (T, 1, D), (0, D, 1), 0)
+    pos = (np.arange(T, dtype=np.int64) % 977).astype(np.int32)
+    y = b.ropeAt(rows, i32(b, pos), 10000.0)
+    for at in (0, 12345, 2 ** 27 - 8, T - 40):
+        got = read32(b, b.slice(y, [at, 0, 0], [at + 19, 1, D]))
+        want = ref.rope_at(np.broadcast_to(x, (19, 1, D)), pos[None, at:at + 19], 10000.0, [D // 2])
+        assert np.abs(got - want).max() <= U["f16"] * np.abs(want).max() + 2.0 ** -20
+    b.dispose(y)
+
+
+def test_attention_of_more_than_2_to_the_26_rows(b):
+    """A wave a row, of a head dimension without matrix cores; rows behind the last document
+    zero."""
+    T = 2 ** 26 + 70
+    rng = np.random.default_rng(43)
+    docs = b.packDocs(i32(b, [3, 40]), T)
+    x = np.zeros((T, 1, 1), np.float16)
+    x[:43] = rng.standard_normal((43, 1, 1))
+    q = b.fromHost(HostTensor("f16", x.shape, x))
+    y = b.sdpaPacked(q, q, q, docs, 1.0)
+    got = read32(b, y).reshape(-1)
+    o, w, e = ref.sdpa_packed(x[:43], x[:43], x[:43], [0, 3, 43], [0, 3, 43], 1.0)
+    assert (np.abs(got[:43] - o.reshape(-1)) <= attn_tolerance("f16", o, w, e, 1, 40).reshape(-1)).all()
+    assert not got[43:].any()
+    b.dispose(y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_more_documents_than_blocks_in_a_grid(b, dtype):
+    """2^20 documents of 17 heads, most of them empty, have more blocks than a grid of the
+    matrix-core kernels holds."""
+    rng = np.random.default_rng(44)
+    B, T, H = 2 ** 20, 100, 17
+    n = np.zeros(B, np.int32)
+    at, lens = [0, 7, B // 2, B - 1], [30, 1, 60, 9]
+    n[at] = lens
+    q, k, v = (rounded(rng.standard_normal((T, H, 64)), dtype) for _ in range(3))
+    got = read32(b, b.sdpaPacked(*(b.fromHost(to_host(t, dtype)) for t in (q, k, v)), b.packDocs(i32(b, n), T), 0.125,
+                                 causal=True))
+    off = ref.offsets(lens, T)
+    o, w, e = ref.sdpa_packed(q, k, v, off, off, 0.125, causal=True)
+    assert (np.abs(got - o) <= attn_tolerance(dtype, o, w, e, 64, 60)).all()
