@@ -491,7 +491,7 @@ static bool lora_few_tiles(hipStream_t st, int cus, const void* x, int64_t ldx, 
   auto run = [&](auto kernel, std::atomic<uint64_t>& attr, int bm, int bn, int nw) {
     if (!launch) return true;
     const int tm = (M + bm - 1) / bm, lds = nw * 2 * (bm + bn) * 128;
-    if (lds > 64 * 1024)
+    if (lds >= 64 * 1024)  // (with its static LDS past the 64 KB that a launch has without the attribute)
       once_per_device(attr, [&] {
         HB_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
       });

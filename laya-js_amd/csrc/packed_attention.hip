@@ -1165,12 +1165,7 @@ static void packed_any(uintptr_t ctx, int dt, const Packed& p) {
 }
 
 template <class K>
-static void packed_launch(uintptr_t ctx, K kern, std::atomic<uint64_t>& attr, int lds, int64_t blocks, const Packed& p,
-                          int splits, const Parts& part) {
-  if (lds > 64 * 1024)
-    once_per_device(attr, [&] {
-      HB_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    });
+static void packed_launch(uintptr_t ctx, K kern, int lds, int64_t blocks, const Packed& p, int splits, const Parts& part) {
   const int64_t grid = blocks * (p.H / p.G);
   HB_REQUIRE(grid < (1ll << 24), "hb_sdpa_packed: too many rows and heads");  // (packed_takes_mfma)
   kern<<<dim3((unsigned)grid, (unsigned)splits), 256, (size_t)lds, stream_of(ctx)>>>(p, part, splits);
@@ -1223,13 +1218,20 @@ static void packed_mfma(uintptr_t ctx, int dt, const Packed& p) {
     constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
     auto half = [&](auto bf) {
       constexpr bool BF = decltype(bf)::value;
-      static std::atomic<uint64_t> attr{0};
-      if (few) packed_launch(ctx, packed_attn_few<BF, CAP, BIAS>, attr, kFewLds, slots, p, splits, part);
-      else packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, attr, 0, (int64_t)p.nblocks * p.G, p, splits, part);
+      if (few) {
+        // (with its static LDS past the 64 KB that a launch has without the attribute)
+        static std::atomic<uint64_t> attr{0};
+        const auto kern = packed_attn_few<BF, CAP, BIAS>;
+        once_per_device(attr, [&] {
+          HB_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds));
+        });
+        packed_launch(ctx, kern, kFewLds, slots, p, splits, part);
+      } else {
+        packed_launch(ctx, packed_attn_rows<BF, CAP, BIAS>, 0, (int64_t)p.nblocks * p.G, p, splits, part);
+      }
     };
-    std::atomic<uint64_t> none{0};
-    if (f32 && few) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, none, 0, slots, p, splits, part);
-    else if (f32) packed_launch(ctx, packed_attn_f32_rows<CAP, BIAS>, none, 0, (int64_t)p.nblocks * p.G, p, splits, part);
+    if (f32 && few) packed_launch(ctx, packed_attn_f32<CAP, BIAS>, 0, slots, p, splits, part);
+    else if (f32) packed_launch(ctx, packed_attn_f32_rows<CAP, BIAS>, 0, (int64_t)p.nblocks * p.G, p, splits, part);
     else if (dt == HB_BF16) half(std::true_type{});
     else half(std::false_type{});
   };
