@@ -716,3 +716,106 @@ def test_attention_of_more_documents_than_blocks_in_a_grid(b, dtype):
     off = ref.offsets(lens, T)
     o, w, e = ref.sdpa_packed(q, k, v, off, off, 0.125, causal=True)
     assert (np.abs(got - o) <= attn_tolerance(dtype, o, w, e, 64, 60)).all()
+
+
+# ------------------------------------------------------------------ documents around the lanes of a wave, other encoders
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count", [62, 63, 64, 65, 129])
+def test_attention_around_64_documents(b, dtype, count):
+    """Few queries a document, of as many documents as a wave has lanes and one more or
+    less, empty ones among them, with rows behind the last."""
+    rng = np.random.default_rng(count)
+    nk = rng.integers(0, 70, count)
+    nk[-1] = 5
+    nq = np.minimum(nk, rng.integers(0, 4, count))
+    nq[-1] = 2
+    for heads, kv in ((2, 2), (6, 2)):
+        run_attn(b, dtype, nq.tolist(), nk.tolist(), heads, kv, 64, count, total=int(nq.sum()) + 37, causal=True, window=60)
+        run_attn(b, dtype, nq.tolist(), None, heads, kv, 64, count, total=int(nq.sum()) + 1)
+
+
+def _quantized_model(b, dtype, bits, seed=0):
+    """_model with quantized Linear weights: the encoder and the weights it multiplies
+    with, q s + z rounded to its type."""
+    from laya_hip.host import HostQuantized, pack_quantized
+    from laya_hip.modernbert import loadModernBert
+    from laya_hip.quant import quantize_matrix
+    enc, W = _model(b, dtype, seed)
+    cfg = enc.config
+    enc.dispose()
+    host, W = {}, {k: rounded(w, dtype) for k, w in W.items()}
+    for name, w in W.items():
+        if not bits or "norm" in name or "embeddings" in name:
+            host[name] = to_host(w, dtype)
+            continue
+        q, s, z = quantize_matrix(w, *w.shape, bits, 64)
+        host[name] = HostQuantized(w.shape, bits, 64, "affine" if bits == 4 else "symmetric", pack_quantized(q, bits),
+                                   HostTensor("f16", s.shape, s), None if z is None else HostTensor("f16", z.shape, z))
+        val = q * np.repeat(s.astype(np.float64), 64, 1) + (0 if z is None else np.repeat(z.astype(np.float64), 64, 1))
+        W[name] = rounded(val, dtype)
+    return loadModernBert(b, cfg, host.get, dtype=dtype, prefix=""), W
+
+
+# both forwards round every op, at 30 places, values up to 8: f16 2^-11, in quadrature
+# 2e-2, doubled; bf16 eight times that
+ENCODERS = [("bf16", 0, 0.35), ("f16", 8, 4e-2), ("f16", 4, 4e-2), ("bf16", 8, 0.35), ("f32", 8, 1e-4)]
+
+
+@pytest.mark.parametrize("dtype,bits,tol", ENCODERS)
+def test_encode_packed_of_other_encoders_is_encode(b, dtype, bits, tol):
+    enc, _ = _quantized_model(b, dtype, bits)
+    rng = np.random.default_rng(3)
+    n, L = [50, 1, 83, 64, 29], 83
+    docs = [rng.integers(0, 500, k) for k in n]
+    ids, valid = np.zeros((len(n), L), np.int32), np.zeros((len(n), L), np.uint8)
+    for i, d in enumerate(docs):
+        ids[i, :d.size], valid[i, :d.size] = d, 1
+    want = read32(b, enc.forward(ids, valid, len(n), L))
+    inp = enc.uploadPacked(docs, padded=L)
+    y = enc.encodePacked(inp)
+    got = read32(b, b.unpackRows(y, inp["docs"]))
+    for i, k in enumerate(n):
+        assert np.abs(got[i, :k] - want[i, :k]).max() <= tol
+    b.dispose(y)
+    enc.disposePacked(inp)
+    enc.dispose()
+
+
+@pytest.mark.parametrize("dtype,bits,tol", [("f16", 0, 4e-2), *ENCODERS])
+def test_encode_packed_with_adapters_on_other_encoders(b, dtype, bits, tol):
+    """16-bit and quantized encoders with adapters against f32 ones with each document's
+    adapter merged into their weights: one side's roundings of the other tests' two."""
+    from laya_hip.modernbert import loadModernBert
+    enc, W = _quantized_model(b, dtype, bits)
+    rng = np.random.default_rng(4)
+    H, I, R, n = 256, 384, 4, 2
+    sizes = {"Wqkv": ("attn.Wqkv", 3 * H, H), "Wo": ("attn.Wo", H, H), "Wi": ("mlp.Wi", 2 * I, H),
+             "WoMlp": ("mlp.Wo", H, I)}
+    host = [{k: (rounded(rng.standard_normal((n, R, i)) * i ** -0.5, dtype), rounded(rng.standard_normal((n, o, R)) * 0.05, dtype))
+             for k, (_, o, i) in sizes.items()} for _ in range(4)]
+    scales = np.array([1.5, -0.5], np.float32)
+    banks = [{k: b.loraBank(b.fromHost(to_host(a, dtype)), b.fromHost(to_host(c, dtype)),
+                            b.fromHost(HostTensor("f32", (n,), scales))) for k, (a, c) in layer.items()} for layer in host]
+    lens, which = [40, 64, 17, 33], [1, -1, 0, 5]
+    docs = [rng.integers(0, 500, k) for k in lens]
+    inp = enc.uploadPacked(docs, adapters=which)
+    got = read32(b, enc.encodePacked(inp, banks))
+    at = 0
+    for d, k, a in zip(docs, lens, which):
+        merged = {m: w.astype(np.float64) for m, w in W.items()}
+        if 0 <= a < n:
+            for i in range(4):
+                for key, (name, _, _) in sizes.items():
+                    A, C = (t[a].astype(np.float64) for t in host[i][key])
+                    merged[f"layers.{i}.{name}.weight"] += float(scales[a]) * C @ A
+        one = loadModernBert(b, enc.config, lambda m: to_host(merged[m], "f32") if m in merged else None, prefix="")
+        want = read32(b, one.forward(d[None], np.ones((1, k), np.uint8), 1, k))[0]
+        assert np.abs(got[at:at + k] - want).max() <= tol
+        one.dispose()
+        at += k
+    for layer in banks:
+        for bank in layer.values():
+            bank.dispose()
+    enc.disposePacked(inp)
+    enc.dispose()
