@@ -319,6 +319,10 @@ class ModernBert:
         if adapters is not None and (len(adapters) != c.numHiddenLayers or inp["adapters"] is None):
             raise ValueError(f"modernbert: adapters of {len(adapters)} layers for {c.numHiddenLayers}, with a number per "
                              "document in uploadPacked")
+        for banks in adapters or ():
+            for name in banks or ():
+                if name not in ("Wqkv", "Wo", "Wi", "WoMlp"):
+                    raise ValueError(f"modernbert: adapters of {name!r}, which is no projection of a layer")
 
         def f():
             x = self.embeddings(inp["ids"])

@@ -229,3 +229,17 @@ def test_adapters_hold_no_copy_of_strided_rows(b, quantized):
         assert [s for s in stores if s.refs] == live
         name, args = b.calls[-1]
         assert name == ("hb_lora_qlinear" if quantized else "hb_lora_linear") and args[3] == ldx
+
+
+def test_encode_packed_refusals():
+    """Adapters of projections that a layer does not have, of too few layers, or of a batch
+    without adapter numbers."""
+    from types import SimpleNamespace
+    from laya_hip.modernbert import ModernBert
+    b = Recorder()
+    enc = ModernBert(b, SimpleNamespace(numHiddenLayers=2), {}, "f16")
+    inp = {"ids": b.t(5, dtype="i32"), "docs": b.packDocs(b.t(1, dtype="i32"), 5), "adapters": b.t(5, dtype="i32")}
+    for adapters in ([{"wqkv": None}, {}], [None, {"mlp.Wo": None}]):
+        refused(b, ValueError, "no projection", lambda: enc.encodePacked(inp, adapters))
+    refused(b, ValueError, "1 layers for 2", lambda: enc.encodePacked(inp, [{}]))
+    refused(b, ValueError, "number per", lambda: enc.encodePacked({**inp, "adapters": None}, [{}, {}]))
