@@ -433,8 +433,9 @@ int hb_sdpa_packed(uintptr_t ctx, int dt, uintptr_t q, const int64_t* qs, uintpt
  * most 1024.  The inner products scales[i] * (x_m . A_i^T) are summed in f32 and, of
  * 16-bit types on the matrix cores (K a multiple of 64, R of 8, operands and rows on 16
  * bytes), rounded to the type for the product with B; those past its range (f16:
- * 65504) stay f32, on a slow path.  x, w, bias, y as in hb_linear (the reference has no
- * adapters). */
+ * 65504) stay f32, on a slow path.  y is rounded once there and in f32 rows of few
+ * tiles; elsewhere the projection is rounded to y's type before the adapter's part
+ * is added to it.  x, w, bias, y as in hb_linear (the reference has no adapters). */
 int hb_lora_linear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t w, uintptr_t bias, uintptr_t y,
                    int64_t ldy, int64_t M, int64_t N, int64_t K, uintptr_t a, uintptr_t b, uintptr_t scales, int64_t n,
                    int64_t R, uintptr_t index);

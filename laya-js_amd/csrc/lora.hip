@@ -362,7 +362,7 @@ __global__ __launch_bounds__(NW * 64) void lora_few(const char* __restrict__ X, 
   for (int i = 0; i < TM; i++)
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
-  auto request = [&](int c) __attribute__((always_inline)) {  // chunk wave + 8 c of K
+  auto request = [&](int c) __attribute__((always_inline)) {  // chunk wave + NW c of K
     const uint32_t to = at0 + (uint32_t)((c & 1) * BUF), k = (uint32_t)(wave + NW * c) * 128u;
 #pragma unroll
     for (int i = 0; i < 2 * TM; i++) buffer_lds16(xs, xo[i], k, to + 1024u * i);

@@ -2045,10 +2045,11 @@ class HipBackend:
         idx = self._plain(index, "i32", tmp)
         if bias is not None:
             bias = self._plain(bias, x.dtype, tmp)
-        if self._row_stride(self._ready(x)) is None:
-            x = self._contiguous(x)
+        ldx = self._row_stride(self._ready(x))
+        if ldx is None:
+            x, ldx = self._contiguous(x), K
             tmp.append(x)
-        _, xp, M, _, ldx = self._rows(x)
+        xp, M = self._ptr(x), _numel(x.shape[:-1])
         out = self._new(x.shape[:-1] + (N,), x.dtype)
         tail = (self._ptr(bank.a), self._ptr(bank.b), self._ptr(bank.scales), bank.count, bank.held_rank, self._ptr(idx))
         return xp, M, ldx, self._ptr(bias) if bias is not None else 0, out, tail

@@ -401,7 +401,6 @@ def _model(b, dtype, seed=0):
                           prefix=""), W
 
 
-# f32: sums in another order, a few 1e-6 after four layers of values up to 5; f16:
 def test_encode_packed_of_nothing(b):
     """No documents, and documents without tokens."""
     enc, _ = _model(b, "f16")
@@ -415,6 +414,7 @@ def test_encode_packed_of_nothing(b):
         b.dispose(y)
 
 
+# f32: sums in another order, a few 1e-6 after four layers of values up to 5; f16:
 # both forwards round every op, 2^-11 of values up to 8 at 30 places, in
 # quadrature 2e-2, doubled
 @pytest.mark.parametrize("dtype,tol", [("f32", 1e-4), ("f16", 4e-2)])
