@@ -946,7 +946,8 @@ struct LoraArgs {
   int64_t n, R;
 };
 
-static void check_lora(const char* op, int dt, int64_t M, int64_t N, int64_t K, const LoraArgs& l) {
+static void check_lora(const char* op, int dt, uintptr_t x, uintptr_t w, uintptr_t y, int64_t M, int64_t N, int64_t K,
+                       const LoraArgs& l) {
   auto need = [&](bool ok, const char* what) {
     if (!ok) throw std::runtime_error(std::string(op) + ": " + what);
   };
@@ -954,6 +955,7 @@ static void check_lora(const char* op, int dt, int64_t M, int64_t N, int64_t K, 
   need(M >= 0 && N >= 0 && K >= 0 && M < (1ll << 31) && N < (1ll << 30) && K < (1ll << 30), "bad sizes");
   need(l.n >= 0 && l.n < (1ll << 30) && l.R >= 0 && l.R <= 1024, "bad adapter count or rank (at most 1024)");
   need(l.n * l.R == 0 || M == 0 || N == 0 || K == 0 || (l.a && l.b && l.scales && l.index), "null adapter argument");
+  need(M == 0 || N == 0 || (y && (K == 0 || (x && w))), "null argument");
 }
 
 // The MFMA path: 16-bit types, K and the operands as the ring takes them, whole
@@ -1075,7 +1077,7 @@ int hb_lora_linear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t w,
                    int64_t R, uintptr_t index) {
   HB_API_BEGIN
   const LoraArgs l{a, b, scales, index, n, R};
-  check_lora("hb_lora_linear", dt, M, N, K, l);
+  check_lora("hb_lora_linear", dt, x, w, y, M, N, K, l);
   HB_REQUIRE(ldx >= K && ldy >= N, "hb_lora_linear: leading dimension smaller than the row");
   if (lora_takes_ring(dt, x, ldx, w, y, ldy, M, N, K, l) &&
       lora_fused(ctx, dt, (const uint16_t*)x, ldx, (const uint16_t*)w, Codes{}, (const uint16_t*)bias, (uint16_t*)y, ldy,
@@ -1092,7 +1094,7 @@ int hb_lora_qlinear(uintptr_t ctx, int dt, uintptr_t x, int64_t ldx, uintptr_t q
                     int mode, uintptr_t a, uintptr_t b, uintptr_t scales, int64_t n, int64_t R, uintptr_t index) {
   HB_API_BEGIN
   const LoraArgs l{a, b, scales, index, n, R};
-  check_lora("hb_lora_qlinear", dt, M, N, K, l);
+  check_lora("hb_lora_qlinear", dt, x, qw, y, M, N, K, l);
   HB_REQUIRE(ldx >= K && ldy >= N, "hb_lora_qlinear: leading dimension smaller than the row");
   HB_REQUIRE((bits == 8 || bits == 4) && (mode == 0 || mode == 1) && group > 0, "hb_lora_qlinear: bad bits, mode or group");
   HB_REQUIRE(qw && qscales && (mode == 0 || zeros), "hb_lora_qlinear: missing weight tensors");

@@ -243,3 +243,14 @@ def test_encode_packed_refusals():
         refused(b, ValueError, "no projection", lambda: enc.encodePacked(inp, adapters))
     refused(b, ValueError, "1 layers for 2", lambda: enc.encodePacked(inp, [{}]))
     refused(b, ValueError, "number per", lambda: enc.encodePacked({**inp, "adapters": None}, [{}, {}]))
+
+
+def test_adapter_entry_points_refuse_null_operands():
+    n, P = F.native(), 1 << 20
+    for dt, K in ((F.HB_F16, 64), (F.HB_F16, 72), (F.HB_F32, 64)):
+        for x, w, y in ((0, P, P), (P, 0, P), (P, P, 0)):
+            with pytest.raises(F.HipError, match="null argument"):
+                n.call("op", "hb_lora_linear", 0, dt, x, K, w, 0, y, 32, 4, 32, K, P, P, P, 2, 8, P)
+        for x, y in ((0, P), (P, 0)):
+            with pytest.raises(F.HipError, match="null argument"):
+                n.call("op", "hb_lora_qlinear", 0, dt, x, K, P, P, 0, 0, y, 32, 4, 32, K, 8, 8, 0, P, P, P, 2, 8, P)
