@@ -466,8 +466,10 @@ constexpr int kUnknown = -3, kNone = -2, kSeveral = -1;  // or the one adapter
 template <int DT>
 __device__ __forceinline__ int lora_dirty(const LoraExt& ext, const int* adapters, int nd, int N, int n) {
   int found = kNone;
+#pragma unroll 1
   for (int o = 0; o < nd; o++) {
     const int a = adapters[o];
+#pragma unroll 1
     for (int r = 0; r < ext.R; r++)
       if (load_f(ext.b, ((int64_t)a * N + n) * ext.R + r, DT) * 0.f != 0.f) {
         if (found != kNone) return kSeveral;
@@ -489,6 +491,7 @@ __device__ __forceinline__ bool lora_past(const LoraExt& ext, int m) {
   if constexpr (DT == HB_F32) return false;
   const int a = ext.index[m];
   if (a < 0 || a >= ext.n) return false;
+#pragma unroll 1
   for (int r = 0; r < ext.R; r++) {
     const int64_t i = (int64_t)m * ext.R + r;
     if (load_f(ext.s, i, DT) * 0.f != 0.f && ext.wide[i] * 0.f == 0.f) return true;
@@ -497,13 +500,16 @@ __device__ __forceinline__ bool lora_past(const LoraExt& ext, int m) {
 }
 
 // One output of a projection with adapters, on its own (slow: see its callers).
+// (These loops are not unrolled: their code lay in the way of lora_stream's, 1% of its time.)
 template <int DT>
 __device__ __forceinline__ float lora_output(const void* X, int64_t ldx, const void* W, const void* bias, int N, int K,
                                              const LoraExt& ext, int m, int n) {
   float sum = 0.f;
+#pragma unroll 4
   for (int k = 0; k < K; k++) sum = fmaf(load_f(X, (int64_t)m * ldx + k, DT), load_f(W, (int64_t)n * K + k, DT), sum);
   const int a = ext.index[m];
   if (a >= 0 && a < ext.n)
+#pragma unroll 1
     for (int r = 0; r < ext.R; r++) {
       const int64_t i = (int64_t)m * ext.R + r;
       float s = load_f(ext.s, i, DT);

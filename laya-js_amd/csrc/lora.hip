@@ -761,7 +761,7 @@ __global__ __launch_bounds__(kStWaves * 64) void lora_stream(const uint16_t* __r
         }
     }
     stored = !odd;
-    if (odd) {
+    if (__builtin_expect(odd, 0)) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       // the zeros of other rows do not keep a non-finite B out of a row's sums (0 *
       // inf), and an inner product may be past the type's range: an output that has come
